@@ -50,7 +50,9 @@ typedef enum {
 typedef enum {
   RAFB200_F32 = 0, RAFB200_F16 = 1, RAFB200_BF16 = 2,
   /* collectives only (the NCCL type map of src/op/dialect/nccl/communication_utils.h:31-48): */
-  RAFB200_F64 = 3, RAFB200_I8 = 4, RAFB200_U8 = 5, RAFB200_I64 = 6
+  RAFB200_F64 = 3, RAFB200_I8 = 4, RAFB200_U8 = 5, RAFB200_I64 = 6,
+  /* token and class ids are RAFB200_I32 or RAFB200_I64 */
+  RAFB200_I32 = 7
 } rafb200_dtype;
 
 RAFB200_API const char* rafb200_last_error(void);
@@ -327,6 +329,64 @@ RAFB200_API int rafb200_fuse_tensor(int k, const void* const* src, const int64_t
 RAFB200_API int rafb200_defuse_tensor(int k, void* const* dst, const int64_t* numel,
                                       const int64_t* offsets, int elem_size, const void* flat,
                                       void* stream);
+
+/* ------------------------------------------------------------------------- */
+/* The two ends of a model                                                    */
+/* ------------------------------------------------------------------------- */
+/* raf.op.embedding with a scale: out[i, :] = scale * x[indices[i], :], rounded once to out_dtype.
+ * x [rows, width] and out [n, width] are compact.  An index outside [0, rows) reads as a row of zeros
+ * (a shard of the table sees the tokens of other shards so). */
+RAFB200_API int rafb200_embedding(const void* x, int x_dtype, int64_t rows, int64_t width,
+                                  const void* indices, int index_dtype, int64_t n, float scale,
+                                  void* out, int out_dtype, void* stream);
+/* raf.op.embedding_dx: dx[r, :] = scale * sum of dy[i, :] over the i with indices[i] == r, zero for the
+ * other rows; accumulate != 0 adds the sums to dx instead and leaves the other rows alone.  Indices equal
+ * to padding_idx and those outside [0, rows) count nothing.
+ * Sums are fp32 and rounded once; their order is fixed by the indices alone, so equal calls give
+ * equal bits.  `workspace` (16-byte aligned, at least rafb200_embedding_dx_workspace_bytes) is written by
+ * the call and holds nothing between calls.  n and rows are below 2^31. */
+RAFB200_API size_t rafb200_embedding_dx_workspace_bytes(int64_t n, int64_t width);
+RAFB200_API int rafb200_embedding_dx(const void* dy, int dy_dtype, const void* indices, int index_dtype,
+                                     int64_t n, int64_t rows, int64_t width, float scale,
+                                     int64_t padding_idx, int accumulate, void* dx, int dx_dtype,
+                                     void* workspace, size_t workspace_bytes, void* stream);
+
+/* Loss of student logits against a teacher's top logits, per row:
+ *   alpha T^2 sum_i p_i (log p_i - log q[ids_i]) + (1 - alpha) (-log r[label])
+ * with p = softmax over the row's present teacher_logits / T, q = softmax(pred / T), r = softmax(pred).
+ *   pred            [n, v], rows ld elements apart, fp32 / fp16 / bf16
+ *   teacher_logits  [n, k] compact, k <= 1024; teacher_ids [n, k]: their classes.  An entry whose class is
+ *                   outside [0, v) is absent; a class may be named more than once.  A row without present
+ *                   entries (or with logits of -infinity only) has no teacher term.
+ *   labels          [n], or NULL (then alpha must be 1).  A row whose label equals ignore_index or lies
+ *                   outside [0, v) has loss 0 and gradient 0, whatever its logits hold.
+ * Logits of -infinity are classes of probability 0; a row of nothing else, +infinity and NaN give NaN.
+ * A term whose weight (alpha, 1 - alpha) is 0 counts nothing. */
+typedef struct {
+  const void* pred;
+  const void* teacher_logits;
+  const void* teacher_ids;
+  const void* labels;
+  int64_t n, v, ld;
+  int64_t ignore_index;
+  double temperature; /* in [2^-20, 2^20] */
+  double alpha;       /* in [0, 1] */
+  int k;
+  int pred_dtype, teacher_dtype, ids_dtype, labels_dtype;
+} rafb200_distill;
+/* loss [n] fp32; stats [n, 4] fp32, 16-byte aligned: what rafb200_distill_loss_dpred takes. */
+RAFB200_API int rafb200_distill_loss(const rafb200_distill* d, float* loss, float* stats, void* stream);
+/* dpred[i, :] = dy[i] * grad_scale * d loss[i] / d pred[i, :], in pred's type, rows ld_dpred elements
+ * apart; what lies between the rows is left alone.  dy: one fp32 weight per row (dy_step 1), one for all rows
+ * (dy_step 0), or NULL for 1.  dpred may be pred itself (same address and ld); any other overlap is
+ * refused. */
+RAFB200_API int rafb200_distill_loss_dpred(const rafb200_distill* d, const float* dy, int dy_step,
+                                           float grad_scale, const float* stats, void* dpred,
+                                           int64_t ld_dpred, void* stream);
+/* Both in one pass, where dy is known beforehand. */
+RAFB200_API int rafb200_distill_loss_with_dpred(const rafb200_distill* d, const float* dy, int dy_step,
+                                                float grad_scale, float* loss, void* dpred,
+                                                int64_t ld_dpred, void* stream);
 
 /* ------------------------------------------------------------------------- */
 /* Communicator and collectives                                               */

@@ -15,6 +15,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("RAFB200_LIB") or os.path.join(HERE, "libraf_b200.so")  # an installed copy elsewhere
 
 F32, F16, BF16 = 0, 1, 2
+I64, I32 = 6, 7
 OPT_SGD, OPT_ADAM, OPT_LANS = 0, 1, 2
 
 STATUS_NAMES = {
@@ -37,6 +38,16 @@ class Hyper(C.Structure):
         ("weight_decay", C.c_float), ("bias_correction", C.c_int), ("grad_averaging", C.c_int),
         ("mode", C.c_int), ("normalize_grad", C.c_int), ("grad_scale", C.c_float),
         ("average", C.c_int),
+    ]
+
+
+class Distill(C.Structure):
+    """struct rafb200_distill."""
+    _fields_ = [
+        ("pred", C.c_void_p), ("teacher_logits", C.c_void_p), ("teacher_ids", C.c_void_p), ("labels", C.c_void_p),
+        ("n", C.c_int64), ("v", C.c_int64), ("ld", C.c_int64), ("ignore_index", C.c_int64),
+        ("temperature", C.c_double), ("alpha", C.c_double), ("k", C.c_int),
+        ("pred_dtype", C.c_int), ("teacher_dtype", C.c_int), ("ids_dtype", C.c_int), ("labels_dtype", C.c_int),
     ]
 
 
@@ -72,6 +83,12 @@ SIGNATURES = {
     "rafb200_group_cast": (_i, [_i, _vp, _i, _vp, _i, _vp, _vp]),
     "rafb200_fuse_tensor": (_i, [_i, _vp, _vp, _vp, _i, _vp, _vp]),
     "rafb200_defuse_tensor": (_i, [_i, _vp, _vp, _vp, _i, _vp, _vp]),
+    "rafb200_embedding": (_i, [_vp, _i, _i64, _i64, _vp, _i, _i64, _f, _vp, _i, _vp]),
+    "rafb200_embedding_dx_workspace_bytes": (_sz, [_i64, _i64]),
+    "rafb200_embedding_dx": (_i, [_vp, _i, _vp, _i, _i64, _i64, _i64, _f, _i64, _i, _vp, _i, _vp, _sz, _vp]),
+    "rafb200_distill_loss": (_i, [_P(Distill), _vp, _vp, _vp]),
+    "rafb200_distill_loss_dpred": (_i, [_P(Distill), _vp, _i, _f, _vp, _vp, _i64, _vp]),
+    "rafb200_distill_loss_with_dpred": (_i, [_P(Distill), _vp, _i, _f, _vp, _vp, _i64, _vp]),
     "rafb200_comm_create": (_i, [_i, _i, _i, C.c_char_p, _i, _P(_vp)]),
     "rafb200_unique_id": (_i, [_vp]),
     "rafb200_comm_create_with_id": (_i, [_i, _i, _i, _vp, _i, _P(_vp)]),

@@ -7,13 +7,14 @@ in the reference (``scripts/src_codegen/def_schema.py:525-536,671-738``), on
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 from typing import List, Optional, Sequence
 
 import torch
 
 from . import _lib
-from ._lib import BF16, F16, F32, check
+from ._lib import BF16, F16, F32, I32, I64, check
 
 _CODES = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
 _NAMES = {"float32": torch.float32, "float16": torch.float16, "bfloat16": torch.bfloat16}
@@ -319,3 +320,272 @@ def defuse_tensor(data, sizes, shapes, shape_indices, stream=None):
         len(outs), _lib.ptr_array([t.data_ptr() for t in outs]), _lib.i64_array(sizes),
         _lib.i64_array(offsets), data.element_size(), data.data_ptr(), stream_ptr(stream)))
     return outs
+
+
+# --------------------------------------------------------------------------- the two ends of a model
+_INDEX = {torch.int64: I64, torch.int32: I32}
+
+
+def _index_code(t) -> int:
+    try:
+        return _INDEX[t.dtype]
+    except KeyError as exc:
+        raise TypeError(f"indices are int32 or int64, not {t.dtype}") from exc
+
+
+def _same_device(*tensors):
+    if any(t.device != tensors[0].device for t in tensors):
+        raise ValueError("tensors must be on one device")
+
+
+def _span(t):
+    """The bytes a tensor of positive strides reaches over."""
+    if t.numel() == 0:
+        return 0, 0
+    last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+
+
+def _check_apart(out, *inputs):
+    lo, hi = _span(out)
+    for t in inputs:
+        a, b = _span(t)
+        if a < hi and lo < b:
+            raise ValueError("out overlaps an input")
+
+
+@contextlib.contextmanager
+def _launching(t, stream):
+    """On the tensor's device and the given stream, for allocations too: what a call allocates there is not
+    handed to another stream's work while the call still runs."""
+    if stream is not None and stream.device != t.device:
+        raise ValueError("the stream belongs to another device than the tensors")
+    with torch.cuda.device(t.device), torch.cuda.stream(stream):
+        yield torch._C._cuda_getCurrentRawStream(t.device.index)
+
+
+class _Embedding(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, indices, scale, padding_idx, dtype):
+        ctx.save_for_backward(indices)
+        ctx.how = x.shape[0], scale, padding_idx, x.dtype
+        return embedding(x.detach(), indices, scale, padding_idx, dtype)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        num_weight, scale, padding_idx, dtype = ctx.how
+        return embedding_dx(dy.contiguous(), *ctx.saved_tensors, num_weight, scale, padding_idx, dtype), None, None, None, None
+
+
+def embedding(x, indices, scale=1.0, padding_idx=None, dtype=None, out=None, stream=None):
+    """raf.op.embedding(x, indices), times ``scale``: ``out[..., :] = scale * x[indices[...], :]``.
+
+    ``x`` is [rows, width] in fp32 / fp16 / bf16, ``indices`` any shape of int32 / int64; the result is of ``dtype``
+    (default: x's), rounded once.  An index outside [0, rows) reads as a row of zeros.  Where ``x`` requires a
+    gradient, backward is :func:`embedding_dx`, for which ``padding_idx`` names an index that counts nothing.
+    """
+    _check_cuda(x, indices)
+    _same_device(x, indices)
+    if x.dim() != 2:
+        raise ValueError("embedding: x is a table, [rows, width]")
+    dtype = x.dtype if dtype is None else torch_dtype(dtype)
+    code, out_code, index = dtype_code(x.dtype), dtype_code(dtype), _index_code(indices)
+    if torch.is_grad_enabled() and x.requires_grad:
+        if out is not None:
+            raise ValueError("embedding: out has no gradient; x must not require one")
+        with _launching(x, stream):  # autograd runs backward on the stream that is current here
+            return _Embedding.apply(x, indices, scale, padding_idx, dtype)
+    shape = indices.shape + x.shape[1:]
+    if out is not None:
+        _check_cuda(out)
+        _same_device(x, out)
+        if out.shape != shape or out.dtype != dtype:
+            raise ValueError(f"embedding: out is to be {tuple(shape)} of {dtype}")
+        _check_apart(out, x, indices)
+        torch.autograd.graph.increment_version(out)
+    with _launching(x, stream) as raw:
+        if out is None:
+            out = torch.empty(shape, dtype=dtype, device=x.device)
+        check(_lib.load().rafb200_embedding(x.data_ptr(), code, x.shape[0], x.shape[1], indices.data_ptr(), index,
+                                            indices.numel(), float(scale), out.data_ptr(), out_code, raw))
+    return out
+
+
+def embedding_dx(dy, indices, num_weight, scale=1.0, padding_idx=None, dtype=None, out=None, accumulate=False, stream=None):
+    """raf.op.embedding_dx(dy, indices, num_weight): the gradient [num_weight, width] of the table,
+    ``dx[r, :] = scale * sum of dy[i, :] over indices[i] == r``, in ``dtype`` (default: dy's, or out's).
+
+    ``out`` takes the result: a gradient that an optimizer or ZeroStep reads.  With ``accumulate`` the sums are
+    added to it (a further micro-batch, a matrix product that shares the table), rounded once to its type, and rows
+    without a token stay as they are.  Indices equal to ``padding_idx`` or outside [0, num_weight) count nothing.
+    The same call gives the same bits: sums run in an order that the indices fix.
+    """
+    _check_cuda(dy, indices)
+    _same_device(dy, indices)
+    if dy.dim() != indices.dim() + 1 or dy.shape[:-1] != indices.shape:
+        raise ValueError("embedding_dx: dy has the shape of indices and one dimension more")
+    num_weight, width = int(num_weight), dy.shape[-1]
+    if num_weight < 0:
+        raise ValueError("embedding_dx: negative num_weight")
+    if dtype is None:
+        dtype = dy.dtype if out is None else out.dtype
+    dtype = torch_dtype(dtype)
+    code, out_code, index = dtype_code(dy.dtype), dtype_code(dtype), _index_code(indices)
+    if out is None:
+        if accumulate:
+            raise ValueError("embedding_dx: accumulate needs the gradient to add to, out")
+    else:
+        _check_cuda(out)
+        _same_device(dy, out)
+        if out.shape != (num_weight, width) or out.dtype != dtype:
+            raise ValueError(f"embedding_dx: out is to be {(num_weight, width)} of {dtype}")
+        _check_apart(out, dy, indices)
+        torch.autograd.graph.increment_version(out)
+    # outside [0, num_weight): nothing is left out
+    padding_idx = -1 if padding_idx is None else int(padding_idx)
+    lib, n = _lib.load(), indices.numel()
+    with _launching(dy, stream) as raw:
+        if out is None:
+            out = torch.empty((num_weight, width), dtype=dtype, device=dy.device)
+        ws = torch.empty(lib.rafb200_embedding_dx_workspace_bytes(n, width), dtype=torch.uint8, device=dy.device)
+        check(lib.rafb200_embedding_dx(dy.data_ptr(), code, indices.data_ptr(), index, n, num_weight, width, float(scale),
+                                       padding_idx, int(bool(accumulate)), out.data_ptr(), out_code, ws.data_ptr(),
+                                       ws.numel(), raw))
+    return out
+
+
+def _rows_of(t, what):
+    """[..., v] as [n, v] with consecutive elements in a row, not copied."""
+    if not t.is_cuda:
+        raise ValueError("raf_b200 operators need CUDA tensors; there is no CPU path")
+    if t.dim() < 1:
+        raise ValueError(f"{what}: at least one dimension")
+    v = t.shape[-1]
+    try:
+        rows = t.view(-1 if t.numel() else t.shape[:-1].numel(), v)
+    except RuntimeError as exc:
+        raise ValueError(f"{what}: rows must lie at one distance from each other") from exc
+    if (v > 1 and rows.stride(1) != 1) or (rows.shape[0] > 1 and rows.stride(0) < v):
+        raise ValueError(f"{what}: a row's elements must be consecutive, and rows must not overlap")
+    return rows, (rows.stride(0) if rows.shape[0] > 1 else v)
+
+
+def _distill_args(pred, teacher_logits, teacher_ids, labels, temperature, alpha, ignore_index):
+    rows, ld = _rows_of(pred, "pred")
+    given = [teacher_logits, teacher_ids] + ([] if labels is None else [labels])
+    _check_cuda(*given)
+    _same_device(pred, *given)
+    lead = pred.shape[:-1]
+    if teacher_logits.dim() != pred.dim() or teacher_logits.shape[:-1] != lead or teacher_ids.shape != teacher_logits.shape:
+        raise ValueError("distill_loss: teacher_logits and teacher_ids have pred's shape up to the last dimension, and each other's")
+    if labels is not None and labels.shape != lead:
+        raise ValueError("distill_loss: labels have pred's shape without the last dimension")
+    if rows.shape[1] == 0 and rows.shape[0]:
+        raise ValueError("distill_loss: no classes")
+    if labels is None and alpha != 1.0:
+        raise ValueError("distill_loss: alpha below 1 needs labels")
+    return _lib.Distill(
+        pred.data_ptr(), teacher_logits.data_ptr(), teacher_ids.data_ptr(), labels.data_ptr() if labels is not None else None,
+        rows.shape[0], max(rows.shape[1], 1), max(ld, 1), int(ignore_index), float(temperature), float(alpha),
+        teacher_logits.shape[-1], dtype_code(pred.dtype), dtype_code(teacher_logits.dtype), _index_code(teacher_ids),
+        _index_code(labels) if labels is not None else I64)
+
+
+def _weights_of(dy, pred):
+    """The address and step of the rows' weights."""
+    if dy is None:
+        return None, 0
+    _check_cuda(dy)
+    _same_device(pred, dy)
+    if dy.dtype != torch.float32:
+        raise TypeError("dy is fp32")
+    if dy.dim() == 0:
+        return dy.data_ptr(), 0
+    if dy.shape != pred.shape[:-1]:
+        raise ValueError("dy has pred's shape without the last dimension, or none")
+    return dy.data_ptr(), 1
+
+
+def _gradient_for(pred, out, others):
+    if out is None:
+        return torch.empty(pred.shape, dtype=pred.dtype, device=pred.device), pred.shape[-1]
+    rows, ld = _rows_of(out, "out")
+    _same_device(pred, out)
+    if out.shape != pred.shape or out.dtype != pred.dtype:
+        raise ValueError(f"out is to be {tuple(pred.shape)} of {pred.dtype}")
+    _check_apart(out, *(t for t in others if t is not None))
+    torch.autograd.graph.increment_version(out)
+    return out, ld
+
+
+class _DistillLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, pred, teacher_logits, teacher_ids, labels, temperature, alpha, ignore_index):
+        loss, stats = distill_loss(pred.detach(), teacher_logits, teacher_ids, labels, temperature, alpha, ignore_index)
+        ctx.save_for_backward(pred, teacher_logits, teacher_ids, stats, labels)
+        ctx.how = temperature, alpha, ignore_index
+        ctx.mark_non_differentiable(stats)
+        return loss, stats
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy, _):
+        return (distill_loss_dpred(dy.contiguous(), *ctx.saved_tensors, *ctx.how),) + (None,) * 6
+
+
+def distill_loss(pred, teacher_logits, teacher_ids, labels=None, temperature=1.0, alpha=1.0, ignore_index=-100, stream=None):
+    """Loss of ``pred`` [..., v] against a teacher's top logits, per row: (loss [...], stats [..., 4]), fp32.
+
+    ``alpha T^2 sum p (log p - log softmax(pred / T)) + (1 - alpha) (-log softmax(pred)[label])`` with p the softmax of
+    the row's ``teacher_logits / T`` [..., k <= 1024] over the classes ``teacher_ids``; an entry whose class is outside
+    [0, v) is absent.  Without ``labels`` alpha is 1.  A row whose label is ``ignore_index`` or outside [0, v) has loss
+    and gradient 0.  Rows of ``pred`` may lie further apart than v (logits padded for a matrix product).
+
+    ``stats`` is what :func:`distill_loss_dpred` takes.  Where ``pred`` requires a gradient, backward calls it.
+    """
+    d = _distill_args(pred, teacher_logits, teacher_ids, labels, temperature, alpha, ignore_index)
+    if torch.is_grad_enabled() and teacher_logits.requires_grad:
+        raise ValueError("distill_loss: the teacher gets no gradient; detach its logits")
+    if torch.is_grad_enabled() and pred.requires_grad:
+        with _launching(pred, stream):
+            return _DistillLoss.apply(pred, teacher_logits, teacher_ids, labels, temperature, alpha, ignore_index)
+    with _launching(pred, stream) as raw:
+        loss = torch.empty(pred.shape[:-1], dtype=torch.float32, device=pred.device)
+        stats = torch.empty(pred.shape[:-1] + (4,), dtype=torch.float32, device=pred.device)
+        check(_lib.load().rafb200_distill_loss(C.byref(d), loss.data_ptr(), stats.data_ptr(), raw))
+    return loss, stats
+
+
+def distill_loss_dpred(dy, pred, teacher_logits, teacher_ids, stats, labels=None, temperature=1.0, alpha=1.0, ignore_index=-100,
+                       grad_scale=1.0, out=None, stream=None):
+    """Gradient of :func:`distill_loss`: ``dy * grad_scale * d loss / d pred``, of pred's shape and type.
+
+    ``dy`` is fp32, one weight per row, one for all rows (0-dimensional), or None for 1; ``grad_scale`` is the loss scale that
+    the optimizers' own ``grad_scale`` takes back.  ``out`` takes the result and may be ``pred`` itself.
+    """
+    d = _distill_args(pred, teacher_logits, teacher_ids, labels, temperature, alpha, ignore_index)
+    weights, step = _weights_of(dy, pred)
+    _check_cuda(stats)
+    _same_device(pred, stats)
+    if stats.shape != pred.shape[:-1] + (4,) or stats.dtype != torch.float32:
+        raise ValueError("distill_loss_dpred: stats are those of distill_loss for this pred")
+    with _launching(pred, stream) as raw:
+        out, ld = _gradient_for(pred, out, (dy, teacher_logits, teacher_ids, stats, labels))
+        check(_lib.load().rafb200_distill_loss_dpred(C.byref(d), weights, step, float(grad_scale), stats.data_ptr(),
+                                                     out.data_ptr(), ld, raw))
+    return out
+
+
+def distill_loss_with_dpred(dy, pred, teacher_logits, teacher_ids, labels=None, temperature=1.0, alpha=1.0, ignore_index=-100,
+                            grad_scale=1.0, out=None, stream=None):
+    """:func:`distill_loss` and :func:`distill_loss_dpred` in one pass over the logits, where the rows' weights ``dy`` are
+    known beforehand: (loss, dpred).  Both are data, part of no autograd graph."""
+    d = _distill_args(pred, teacher_logits, teacher_ids, labels, temperature, alpha, ignore_index)
+    weights, step = _weights_of(dy, pred)
+    with _launching(pred, stream) as raw:
+        loss = torch.empty(pred.shape[:-1], dtype=torch.float32, device=pred.device)
+        out, ld = _gradient_for(pred, out, (dy, teacher_logits, teacher_ids, labels))
+        check(_lib.load().rafb200_distill_loss_with_dpred(C.byref(d), weights, step, float(grad_scale), loss.data_ptr(),
+                                                          out.data_ptr(), ld, raw))
+    return loss, out

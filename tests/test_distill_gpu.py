@@ -1,0 +1,366 @@
+"""The distillation loss and its gradient against the definition in 64 bits.
+
+Where the allowances come from, with u = 2^-24 (half a step of fp32) and A the largest |z - max z| log2(e) / T of a
+row that still matters (2^-126 is flushed to zero):
+  an exponential    its argument is one rounded product and a rounded constant: 2 A u in base 2, 2 A u ln 2 < 2 A u
+                    relative; ex2.approx: 2 ulp = 4 u
+  a sum             a thread adds v / 512 terms of a block's share and merges them over a loop of 4 groups, 32 lanes, 16 warps and 8
+                    blocks: v / 512 + 64 additions, each with a rescaling of 4 u
+  a quotient        both of these, and a rounding
+That is `r` below, relative, for q, r and the teacher's p.  The gradient is a difference of such terms, each off by r of
+itself, and is rounded once to the result's type.  A logarithm (2 ulp of a value below log2(v) + A, which also bounds what
+is subtracted) is off by 4 u (A + log2 v) + r.
+"""
+import math
+
+import pytest
+import torch
+
+from raf_b200 import _lib, op
+
+pytestmark = pytest.mark.gpu
+
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+U = 2.0 ** -24
+IGNORE = -100
+
+
+def make(n, v, k, dtype, seed=0, pad=0, spread=2.0, index=torch.int64, labels=False, offset=0):
+    g = torch.Generator(device="cuda").manual_seed(seed * 1000003 + n * 31 + v * 7 + k)
+    z = torch.randn(n, v, generator=g, device="cuda") * spread
+    room = torch.full((n * (v + pad) + offset,), 77.0, dtype=dtype, device="cuda")
+    pred = room[offset:].view(n, v + pad)[:, :v]
+    pred.copy_(z)
+    ids = torch.rand(n, v, generator=g, device="cuda").argsort(1)[:, :k].to(index).contiguous() if k <= v else torch.randint(0, v, (n, k), generator=g, device="cuda").to(index)
+    teacher = (torch.randn(n, k, generator=g, device="cuda") * spread).to(dtype)
+    lab = torch.randint(0, v, (n,), generator=g, device="cuda").to(index) if labels else None
+    dy = torch.rand(n, generator=g, device="cuda") * 2 - 0.5
+    return pred, teacher, ids, lab, dy
+
+
+def definition(pred, teacher, ids, labels, temperature, alpha, ignore=IGNORE):
+    """(loss, dz / 1, the sum of the absolute values of dz's terms, A)"""
+    z, t, ids = pred.double(), teacher.double() / temperature, ids.long()
+    n, v = z.shape
+    here = (ids >= 0) & (ids < v)
+    at = torch.where(here, ids, torch.zeros_like(ids))
+    t = torch.where(here, t, torch.full_like(t, -math.inf))
+    some = (t > -math.inf).any(1) | t.isnan().any(1)
+    log_p = torch.log_softmax(t, 1)
+    p = torch.where(some[:, None] & (log_p > -math.inf) | log_p.isnan() & some[:, None], log_p.exp(), torch.zeros_like(t))
+    log_q, log_r = torch.log_softmax(z / temperature, 1), torch.log_softmax(z, 1)
+    terms = torch.where(p == 0, torch.zeros_like(p), p * (log_p - log_q.gather(1, at)))
+    weight = torch.zeros_like(z).scatter_add_(1, at, p)
+    loss = torch.zeros(n, dtype=torch.float64, device="cuda")
+    grad, size = torch.zeros_like(z), torch.zeros_like(z)
+    if alpha > 0:
+        loss = loss + alpha * temperature ** 2 * terms.sum(1)
+        q = torch.where(some[:, None], log_q.exp(), torch.zeros_like(z))
+        grad = grad + alpha * temperature * (q - weight)
+        size = size + alpha * temperature * (q + weight)
+    if labels is not None:
+        lab = labels.long()
+        drop = (lab == ignore) | (lab < 0) | (lab >= v)
+        hot = torch.zeros_like(z).scatter_(1, lab.clamp(0, v - 1)[:, None], 1.0)
+        if alpha < 1:
+            loss = loss - (1 - alpha) * log_r.gather(1, lab.clamp(0, v - 1)[:, None])[:, 0]
+            grad = grad + (1 - alpha) * (log_r.exp() - hot)
+            size = size + (1 - alpha) * (log_r.exp() + hot)
+        loss = torch.where(drop, torch.zeros_like(loss), loss)
+        grad = torch.where(drop[:, None], torch.zeros_like(grad), grad)
+    span = (z.amax(1, keepdim=True) - torch.where(z > -math.inf, z, z.amax(1, keepdim=True))).nan_to_num(0, 0, 0).amax(1)
+    return loss, grad, size, span * (math.log2(math.e) / min(temperature, 1.0))
+
+
+def allowances(v, k, far, temperature, alpha):
+    r = (4 + (v / 512 + 64) * 5 + k / 32 * 5 + 8) * U + 4 * far.clamp(max=126) * U
+    # the loss: each of T^2's terms is a difference of logarithms
+    loss = (alpha * temperature ** 2 + 1 - alpha) * ((far + math.log2(v) + 8) * 2 * r + 8 * U * (far + math.log2(v)))
+    return r, loss
+
+
+def check(args, loss=None, grad=None, dy=None, temperature=1.0, alpha=1.0, scale=1.0, ignore=IGNORE):
+    pred, teacher, ids, labels = args
+    want, g, size, far = definition(pred, teacher, ids, labels, temperature, alpha, ignore)
+    t_far = (teacher.double().amax(1) - teacher.double().amin(1)).nan_to_num(0, 0, 0) / temperature * math.log2(math.e) if teacher.shape[1] else far * 0
+    r, allowed = allowances(pred.shape[1], teacher.shape[1], torch.maximum(far, t_far), temperature, alpha)
+    if loss is not None:
+        same = (loss.double() == want) | (loss.isnan() & want.isnan())
+        assert bool((same | ((loss.double() - want).abs() <= allowed)).all()), float(((loss.double() - want).abs() - allowed).max())
+    if grad is not None:
+        w = (torch.ones_like(want) if dy is None else dy.double() * torch.ones_like(want))[:, None] * scale
+        g, size = g * w, size * w.abs()
+        info = torch.finfo(grad.dtype)
+        slack = size * (r[:, None] + 8 * U) + 2.0 ** -125 * w.abs()
+        slack = slack + (g.abs() + slack) * info.eps / 2 + info.smallest_normal * info.eps / 2
+        off = (grad.double() - g).abs()
+        assert bool(((off <= slack) | (g.isnan() & grad.isnan())).all()), float((off - slack).max())
+
+
+CASES = [(1, 1, 1), (2, 5, 3), (3, 17, 17), (1, 50257, 16), (40, 4096, 64), (300, 1000, 5), (7, 30522, 40), (5, 9001, 0), (160, 513, 100), (2, 131072, 33)]
+
+
+@pytest.mark.parametrize("n,v,k", CASES)
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("temperature,alpha", [(1.0, 1.0), (2.0, 0.5), (0.7, 0.25), (1.0, 0.5), (3.0, 0.0)])
+def test_loss_and_gradient(n, v, k, dtype, temperature, alpha):
+    labels = alpha < 1
+    pred, teacher, ids, lab, dy = make(n, v, k, dtype, index=torch.int32 if n % 2 else torch.int64, labels=labels, pad=0 if n % 3 else 7)
+    if labels and n > 2:
+        lab[1], lab[n // 2] = IGNORE, v
+    if k > 2:
+        ids[0, 1] = -1
+        ids[-1, :] = v + 3  # no teacher at all
+    how = dict(labels=lab, temperature=temperature, alpha=alpha)
+    args = (pred, teacher, ids, lab)
+    loss, stats = op.distill_loss(pred, teacher, ids, **how)
+    assert loss.shape == (n,) and loss.dtype == F32
+    check(args, loss, temperature=temperature, alpha=alpha)
+    grad = op.distill_loss_dpred(dy, pred, teacher, ids, stats, grad_scale=64.0, **how)
+    assert grad.shape == pred.shape and grad.dtype == dtype
+    check(args, None, grad, dy, temperature, alpha, 64.0)
+    both = op.distill_loss_with_dpred(dy, pred, teacher, ids, grad_scale=64.0, **how)
+    check(args, both[0], both[1], dy, temperature, alpha, 64.0)
+    assert torch.equal(both[0], loss)
+    again = op.distill_loss_with_dpred(dy, pred, teacher, ids, grad_scale=64.0, **how)
+    assert torch.equal(both[0], again[0]) and torch.equal(both[1].view(torch.uint8), again[1].view(torch.uint8))
+
+
+@pytest.mark.parametrize("v", list(range(1, 36)) + [511, 4095, 4097, 8193])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_every_length_at_every_address(v, dtype):
+    for offset in range(0, 9, 1 if v < 20 else 3):
+        args = make(5, v, min(v, 4), dtype, offset, pad=offset % 4, labels=True, offset=offset)
+        pred, dy = args[0], args[4]
+        room = torch.full((5 * (v + 3) + 5,), 9.0, dtype=dtype, device="cuda")
+        out = room[5:].view(5, v + 3)[:, :v]
+        how = dict(labels=args[3], temperature=2.0, alpha=0.5)
+        loss, stats = op.distill_loss(pred, *args[1:3], **how)
+        check(args[:4], loss, None, None, 2.0, 0.5)
+        for call in (lambda o: op.distill_loss_dpred(dy, pred, *args[1:3], stats, out=o, **how),
+                     lambda o: op.distill_loss_with_dpred(dy, pred, *args[1:3], out=o, **how)[1]):
+            room.fill_(9.0)
+            assert call(out) is out
+            check(args[:4], None, out, dy, 2.0, 0.5)
+            assert bool((room[:5] == 9).all()) and bool((room[5:].view(5, v + 3)[:, v:] == 9).all())
+            check(args[:4], None, call(None), dy, 2.0, 0.5)
+
+
+@pytest.mark.parametrize("n,v", [(3, 50257), (200, 1001), (2, 33)])
+@pytest.mark.parametrize("dtype", [F32, F16])
+def test_the_gradient_may_take_the_place_of_the_logits(n, v, dtype):
+    pred, teacher, ids, lab, dy = make(n, v, 9, dtype, pad=5, labels=True)
+    how = dict(labels=lab, temperature=1.5, alpha=0.3)
+    stats = op.distill_loss(pred, teacher, ids, **how)[1]
+    want = op.distill_loss_with_dpred(dy, pred, teacher, ids, **how)
+    alone = op.distill_loss_dpred(dy, pred, teacher, ids, stats, **how)
+    for call, expect in ((lambda z: op.distill_loss_with_dpred(dy, z, teacher, ids, out=z, **how)[1], want[1]),
+                         (lambda z: op.distill_loss_dpred(dy, z, teacher, ids, stats, out=z, **how), alone)):
+        copy = torch.full((n, v + 5), 77.0, dtype=dtype, device="cuda")
+        z = copy[:, :v]
+        z.copy_(pred)
+        assert call(z) is z
+        check((pred, teacher, ids, lab), None, z, dy, 1.5, 0.3)
+        assert bool((copy[:, v:] == 77).all())
+
+
+def test_a_class_named_twice():
+    pred, teacher, ids, lab, dy = make(6, 300, 8, F32, labels=True)
+    ids[:, 3] = ids[:, 0]
+    ids[1, :] = 5
+    ids[2, 7] = ids[2, 0]
+    lab[2] = ids[2, 0]
+    lab[3] = ids[3, 5]
+    for alpha in (1.0, 0.5):
+        args = (pred, teacher, ids, lab)
+        how = dict(labels=lab, temperature=2.0, alpha=alpha)
+        loss, stats = op.distill_loss(*args[:3], **how)
+        check(args, loss, op.distill_loss_dpred(dy, *args[:3], stats, **how), dy, 2.0, alpha)
+        both = op.distill_loss_with_dpred(dy, *args[:3], **how)
+        check(args, both[0], both[1], dy, 2.0, alpha)
+
+
+@pytest.mark.parametrize("k", [1, 31, 33, 1000, 1024])
+def test_long_lists_of_entries(k):
+    pred, teacher, ids, lab, dy = make(3, 2000, k, BF16)
+    both = op.distill_loss_with_dpred(dy, pred, teacher, ids, temperature=2.0)
+    check((pred, teacher, ids, None), both[0], both[1], dy, 2.0)
+    ids.fill_(7)  # all of them one class
+    both = op.distill_loss_with_dpred(dy, pred, teacher, ids, temperature=2.0)
+    check((pred, teacher, ids, None), both[0], both[1], dy, 2.0)
+
+
+def test_masked_logits():
+    """Classes at -infinity or at the type's lowest value, in the student and in the teacher."""
+    for dtype in (F32, F16, BF16):
+        for low in (-math.inf, torch.finfo(dtype).min):
+            pred, teacher, ids, lab, dy = make(6, 5003, 6, dtype, labels=True)
+            pred[:, 100:4000] = low
+            pred[1, :4990] = low
+            ids[0], ids[1] = torch.arange(5, 11, device="cuda"), torch.arange(4990, 4996, device="cuda")
+            ids[2:] = torch.randint(4000, 5003, ids[2:].shape, device="cuda")
+            teacher[0, 2:] = -math.inf
+            teacher[3] = -math.inf  # no teacher
+            lab.copy_(torch.arange(4990, 4996, device="cuda"))
+            for alpha, temperature in ((1.0, 2.0), (0.5, 2.0), (0.5, 1.0)):
+                how = dict(labels=lab, temperature=temperature, alpha=alpha)
+                both = op.distill_loss_with_dpred(dy, pred, teacher, ids, **how)
+                assert bool(both[1].isfinite().all()) and bool(both[0].isfinite().all())
+                if low == -math.inf:
+                    check((pred, teacher, ids, lab), both[0], both[1], dy, temperature, alpha)
+                else:  # the lowest value is as good as -infinity: its exponential is 0
+                    z = torch.where(pred == low, torch.full_like(pred, -math.inf), pred)
+                    same = op.distill_loss_with_dpred(dy, z, teacher, ids, **how)
+                    assert torch.equal(both[0], same[0]) and torch.equal(both[1], same[1])
+
+
+def test_infinities_and_nan_stay_in_their_rows():
+    pred, teacher, ids, lab, dy = make(9, 3001, 4, F32, labels=True)
+    clean = op.distill_loss_with_dpred(dy, pred, teacher, ids, labels=lab, alpha=0.5)
+    pred[1, 17] = math.nan
+    pred[2, 3000] = math.inf
+    pred[3] = -math.inf
+    pred[4] = math.nan
+    lab[4] = IGNORE  # a row that is left out may hold anything
+    teacher[5, 1] = math.nan
+    teacher[6, 0] = math.inf
+    lab[7] = -5
+    pred[8, ids[8, 0]] = -math.inf  # a class the teacher wants, and that cannot be
+    loss, grad = op.distill_loss_with_dpred(dy, pred, teacher, ids, labels=lab, alpha=0.5)
+    two = op.distill_loss(pred, teacher, ids, labels=lab, alpha=0.5)
+    apart = op.distill_loss_dpred(dy, pred, teacher, ids, two[1], labels=lab, alpha=0.5)
+    for x, d in ((loss, grad), (two[0], apart)):
+        assert bool(x[[1, 2, 3, 5, 6]].isnan().all()) and bool((x[[4, 7]] == 0).all()) and float(x[8]) == math.inf
+        assert bool((d[[4, 7]] == 0).all()) and bool(d[[1, 2, 3, 5, 6]].isnan().any(1).all()) and bool(d[8].isfinite().all())
+        assert float(x[0]) == float(clean[0][0])
+    assert torch.equal(grad[0], clean[1][0])
+
+
+def test_a_term_without_weight_counts_nothing():
+    pred, teacher, ids, lab, dy = make(4, 700, 5, F32, labels=True)
+    pred[0, ids[0, 0]] = -math.inf
+    pred[1, lab[1]] = -math.inf
+    hard = op.distill_loss_with_dpred(dy, pred, teacher, ids, labels=lab, alpha=0.0, temperature=2.0)
+    soft = op.distill_loss_with_dpred(dy, pred, teacher, ids, labels=lab, alpha=1.0, temperature=2.0)
+    assert float(hard[0][1]) == math.inf and bool(hard[0][[0, 2, 3]].isfinite().all()) and bool(hard[1].isfinite().all())
+    assert float(soft[0][0]) == math.inf and bool(soft[0][[1, 2, 3]].isfinite().all()) and bool(soft[1].isfinite().all())
+    assert torch.equal(soft[1][2:], op.distill_loss_with_dpred(dy, pred, teacher, ids, temperature=2.0)[1][2:])
+
+
+@pytest.mark.parametrize("shift", [0.0, 300.0, -3000.0])
+def test_only_differences_of_logits_count(shift):
+    """fp32 logits far from zero: their own spacing is 2^-12 at 3000, what is computed from them keeps fp32's steps."""
+    pred, teacher, ids, lab, dy = make(8, 4000, 12, F32, labels=True)
+    pred += shift
+    teacher += shift
+    for temperature, alpha in ((1.0, 0.5), (4.0, 0.5)):
+        both = op.distill_loss_with_dpred(dy, pred, teacher, ids, labels=lab, temperature=temperature, alpha=alpha)
+        check((pred, teacher, ids, lab), both[0], both[1], dy, temperature, alpha)
+
+
+def test_more_than_32_bits_of_elements():
+    n, v = 90000, 50257
+    if torch.cuda.get_device_properties(0).total_memory < 60 << 30:
+        pytest.skip("needs 60 GB")
+    pred = torch.zeros(n, v, dtype=BF16, device="cuda")
+    rows = torch.tensor([0, 85462, 89998, 89999], device="cuda")  # the 2^32nd element is in row 85461
+    pred[rows] = torch.randn(4, v, device="cuda").to(BF16)
+    teacher, ids = torch.randn(n, 5, device="cuda"), torch.randint(0, v, (n, 5), device="cuda")
+    loss, stats = op.distill_loss(pred, teacher, ids, temperature=2.0)
+    args = (pred[rows], teacher[rows], ids[rows], None)
+    check(args, loss[rows], temperature=2.0)
+    grad = op.distill_loss_dpred(None, pred, teacher, ids, stats, temperature=2.0)
+    check(args, None, grad[rows], None, 2.0)
+    assert torch.equal(op.distill_loss_with_dpred(None, pred, teacher, ids, temperature=2.0, out=grad)[0], loss)
+    check(args, None, grad[rows], None, 2.0)
+
+
+def test_weights_of_rows_and_shapes():
+    pred, teacher, ids, lab, dy = make(12, 800, 4, F32, labels=True)
+    how = dict(temperature=2.0, alpha=0.5)
+    for lead in ((12,), (3, 4), (2, 1, 6)):
+        z, t, i, y, w = pred.view(*lead, 800), teacher.view(*lead, 4), ids.view(*lead, 4), lab.view(lead), dy.view(lead)
+        loss, stats = op.distill_loss(z, t, i, y, **how)
+        assert loss.shape == lead and stats.shape == lead + (4,)
+        grad = op.distill_loss_dpred(w, z, t, i, stats, y, **how)
+        check((pred, teacher, ids, lab), loss.view(-1), grad.view(12, 800), dy, 2.0, 0.5)
+    padded = torch.zeros(3, 4, 832, device="cuda")[..., :800]
+    padded.copy_(pred.view(3, 4, 800))
+    assert torch.equal(op.distill_loss(padded, teacher.view(3, 4, 4), ids.view(3, 4, 4), lab.view(3, 4), **how)[0].view(-1),
+                       op.distill_loss(pred, teacher, ids, lab, **how)[0])
+    one = torch.tensor(0.25, device="cuda")
+    assert torch.equal(op.distill_loss_with_dpred(one, pred, teacher, ids)[1], op.distill_loss_with_dpred(None, pred, teacher, ids, grad_scale=0.25)[1])
+    single = op.distill_loss(pred[0], teacher[0], ids[0])[0]
+    assert single.shape == () and float(single) == float(op.distill_loss(pred[:1], teacher[:1], ids[:1])[0])
+    empty = op.distill_loss_with_dpred(None, pred[:0], teacher[:0], ids[:0])
+    assert empty[0].shape == (0,) and empty[1].shape == (0, 800)
+
+
+def test_backward_is_dpred_and_the_slope():
+    pred, teacher, ids, lab, dy = make(5, 600, 7, F32, labels=True)
+    how = dict(labels=lab, temperature=2.0, alpha=0.4)
+    z = pred.clone().requires_grad_()
+    loss, stats = op.distill_loss(z, teacher, ids, **how)
+    assert not stats.requires_grad
+    (loss * dy).sum().backward()
+    assert torch.equal(z.grad, op.distill_loss_dpred(dy, pred, teacher, ids, stats, **how))
+    z.grad = None
+    op.distill_loss(z, teacher, ids, **how)[0].mean().backward()  # a gradient that is broadcast
+    mean = z.grad
+    # differences of the loss, in fp32: steps of 2^-6, whose third order is 2^-12 of a second derivative below 4
+    step = torch.zeros_like(pred)
+    for j in (int(ids[2, 0]), int(lab[2]), 11):
+        step.zero_()
+        step[2, j] = 2.0 ** -6
+        up, down = (op.distill_loss(pred + d, teacher, ids, **how)[0][2].double() for d in (step, -step))
+        assert abs(float((up - down) * 32 / 5) - float(mean[2, j])) < 2e-4
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(torch.autograd.grad(op.distill_loss(z, teacher, ids)[0].sum(), z, create_graph=True)[0].sum(), z)
+
+
+def test_streams_and_graphs():
+    pred, teacher, ids, lab, dy = make(20, 3000, 7, BF16, labels=True)
+    how = dict(labels=lab, temperature=2.0, alpha=0.4)
+    want = op.distill_loss_with_dpred(dy, pred, teacher, ids, **how)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    got = op.distill_loss_with_dpred(dy, pred, teacher, ids, stream=side, **how)
+    loss, stats = op.distill_loss(pred, teacher, ids, stream=side, **how)
+    alone = op.distill_loss_dpred(dy, pred, teacher, ids, stats, stream=side, **how)
+    side.synchronize()
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]) and torch.equal(loss, want[0])
+    check((pred, teacher, ids, lab), None, alone, dy, 2.0, 0.4)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = op.distill_loss_with_dpred(dy, pred, teacher, ids, **how)
+    pred.copy_(torch.randn(pred.shape, device="cuda"))
+    graph.replay()
+    check((pred, teacher, ids, lab), captured[0], captured[1], dy, 2.0, 0.4)
+
+
+def test_refusals_on_the_gpu():
+    pred, teacher, ids, lab, dy = make(6, 40, 3, F32, labels=True)
+    stats = op.distill_loss(pred, teacher, ids)[1]
+    big = torch.zeros(6, 2000, 1025, device="cuda")[0]
+    bad = [lambda: op.distill_loss(pred.t(), teacher, ids), lambda: op.distill_loss(pred, teacher[:5], ids), lambda: op.distill_loss(pred, teacher, ids[:, :2]),
+           lambda: op.distill_loss(pred, teacher, ids, alpha=0.5), lambda: op.distill_loss(pred, teacher, ids, lab[:5], alpha=0.5),
+           lambda: op.distill_loss(pred, teacher, ids.cpu()), lambda: op.distill_loss(pred.expand(6, 6, 40), teacher, ids),
+           lambda: op.distill_loss(pred[:1].expand(6, 40), teacher, ids), lambda: op.distill_loss(pred[:, :0], teacher, ids),
+           lambda: op.distill_loss(pred, teacher.clone().requires_grad_(), ids),
+           lambda: op.distill_loss_dpred(dy[:4], pred, teacher, ids, stats), lambda: op.distill_loss_dpred(dy, pred, teacher, ids, stats[:5]),
+           lambda: op.distill_loss_dpred(dy, pred, teacher, ids, stats, out=pred.half()), lambda: op.distill_loss_dpred(dy, pred, teacher, ids, stats, out=pred[:5]),
+           lambda: op.distill_loss_with_dpred(dy, pred, teacher, ids, out=torch.zeros(40, 6, device="cuda").t())]
+    for call in bad:
+        with pytest.raises(ValueError):
+            call()
+    for call in (lambda: op.distill_loss(pred.double(), teacher, ids), lambda: op.distill_loss(pred, teacher, ids.float()),
+                 lambda: op.distill_loss(pred, teacher.double(), ids), lambda: op.distill_loss_dpred(dy.half(), pred, teacher, ids, stats)):
+        with pytest.raises(TypeError):
+            call()
+    for call in (lambda: op.distill_loss(pred, teacher, ids, temperature=0.0), lambda: op.distill_loss(pred, teacher, ids, temperature=math.nan),
+                 lambda: op.distill_loss(pred, teacher, ids, lab, alpha=1.5), lambda: op.distill_loss(big, big, torch.zeros(2000, 1025, dtype=torch.int32, device="cuda"))):
+        with pytest.raises(_lib.RafB200Error):
+            call()
+    room = torch.zeros(6, 80, device="cuda")
+    with pytest.raises(_lib.RafB200Error, match="overlaps"):
+        op.distill_loss_with_dpred(dy, room[:, :40], teacher, ids, out=room[:, 40:])
