@@ -415,7 +415,7 @@ int rafb200_embedding_dx(const void* dy, int dy_dtype, const void* indices, int 
     const int64_t each = (int64_t)kSortBlocks * kSortThreads * 64;  // four stores a thread
     clusters += (unsigned)std::min<int64_t>((so.fill_bytes + each - 1) / each, kFillClusters);
   }
-  RAFB200_CUDA(cudaFuncSetAttribute(embedding_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSortSmem));
+  if (const int rc = allow_smem<embedding_sort_kernel>(kSortSmem)) return rc;
   RAFB200_CUDA(launch_cluster(embedding_sort_kernel, kSortBlocks, clusters * kSortBlocks, kSortThreads, kSortSmem, s, so));
   if (n == 0) return RAFB200_OK;
 

@@ -1,6 +1,7 @@
 // What the operators at the ends of a model (embedding.cu, distill.cu) share: index loads, groups of VEC
 // elements at any alignment, launches of thread-block clusters.
 #pragma once
+#include <atomic>
 #include <cstring>
 #include <type_traits>
 
@@ -150,6 +151,18 @@ inline cudaError_t launch_cluster(void (*kernel)(Params...), unsigned cluster, u
   cfg.attrs = attr;
   cfg.numAttrs = 2;
   return cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);
+}
+
+// Lets the kernel take `bytes` of dynamic shared memory on the current device, asked of the driver when they grow.
+template <auto kKernel>
+inline int allow_smem(size_t bytes) {
+  static std::atomic<size_t> granted[64];
+  int device = 0;
+  RAFB200_CUDA(cudaGetDevice(&device));
+  if (bytes <= 48 * 1024 || (device < 64 && granted[device].load(std::memory_order_relaxed) >= bytes)) return RAFB200_OK;
+  RAFB200_CUDA(cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+  if (device < 64) granted[device].store(bytes, std::memory_order_relaxed);
+  return RAFB200_OK;
 }
 
 // Calls f with a value of the element type of a dtype code (checked before).

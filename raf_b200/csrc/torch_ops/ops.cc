@@ -13,6 +13,7 @@
 #include <c10/core/GradMode.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -34,6 +35,12 @@ struct {
   decltype(&rafb200_group_cast) group_cast;
   decltype(&rafb200_fuse_tensor) fuse_tensor;
   decltype(&rafb200_defuse_tensor) defuse_tensor;
+  decltype(&rafb200_embedding) embedding;
+  decltype(&rafb200_embedding_dx) embedding_dx;
+  decltype(&rafb200_embedding_dx_workspace_bytes) embedding_dx_workspace_bytes;
+  decltype(&rafb200_distill_loss) distill_loss;
+  decltype(&rafb200_distill_loss_dpred) distill_loss_dpred;
+  decltype(&rafb200_distill_loss_with_dpred) distill_loss_with_dpred;
 } abi;
 
 PyObject* bind(PyObject*, PyObject* path) {
@@ -49,7 +56,11 @@ PyObject* bind(PyObject*, PyObject* path) {
   if (!find(abi.sgd_to, "rafb200_sgd_to") || !find(abi.sgd_many, "rafb200_sgd_many") ||
       !find(abi.lans_many, "rafb200_lans_many") ||
       !find(abi.group_cast, "rafb200_group_cast") || !find(abi.fuse_tensor, "rafb200_fuse_tensor") ||
-      !find(abi.defuse_tensor, "rafb200_defuse_tensor"))
+      !find(abi.defuse_tensor, "rafb200_defuse_tensor") || !find(abi.embedding, "rafb200_embedding") ||
+      !find(abi.embedding_dx, "rafb200_embedding_dx") ||
+      !find(abi.embedding_dx_workspace_bytes, "rafb200_embedding_dx_workspace_bytes") ||
+      !find(abi.distill_loss, "rafb200_distill_loss") || !find(abi.distill_loss_dpred, "rafb200_distill_loss_dpred") ||
+      !find(abi.distill_loss_with_dpred, "rafb200_distill_loss_with_dpred"))
     return nullptr;
   Py_RETURN_NONE;
 }
@@ -446,6 +457,178 @@ PyObject* defuse_tensor(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return wrapped_list(outs);
 }
 
+int index_code_of(at::ScalarType t) { return t == at::kLong ? RAFB200_I64 : t == at::kInt ? RAFB200_I32 : -1; }
+
+// A dtype argument: torch.float32 and so on, or None for `otherwise`; another type or a name is handed back.
+bool type_of(PyObject* o, at::ScalarType otherwise, at::ScalarType* type) {
+  if (o != Py_None && !THPDtype_Check(o)) return false;
+  *type = o == Py_None ? otherwise : reinterpret_cast<THPDtype*>(o)->scalar_type;
+  return code_of(*type) >= 0;
+}
+
+Range range_of(const at::Tensor& t, bool written) {
+  const uintptr_t p = reinterpret_cast<uintptr_t>(t.const_data_ptr());
+  return {p, p + t.numel() * t.element_size(), written};
+}
+
+// embedding(x, indices, scale, dtype) -> tensor
+PyObject* embedding(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 4) return nothing();
+  c10::DeviceIndex dev = -1;
+  const at::Tensor *x = data_only(a[0], dev), *ids = plain(a[1], dev);
+  at::ScalarType type;
+  if (!x || !ids || x->dim() != 2 || !type_of(a[3], x->scalar_type(), &type)) return nothing();
+  const int code = code_of(x->scalar_type()), index = index_code_of(ids->scalar_type());
+  const double scale = PyFloat_AsDouble(a[2]);
+  if (PyErr_Occurred()) {
+    PyErr_Clear();
+    return nothing();
+  }
+  if (code < 0 || index < 0) return nothing();
+  c10::SmallVector<int64_t, 6> shape(ids->sizes().begin(), ids->sizes().end());
+  shape.push_back(x->size(1));
+  at::Tensor out;
+  int rc;
+  {
+    NoGil released;
+    out = new_tensor(shape, type);
+    rc = abi.embedding(x->const_data_ptr(), code, x->size(0), x->size(1), ids->const_data_ptr(), index, ids->numel(), (float)scale,
+                       out.mutable_data_ptr(), code_of(type), current_stream(dev));
+  }
+  if (rc != RAFB200_OK) return PyLong_FromLong(rc);
+  return THPVariable_Wrap(std::move(out));
+}
+
+// embedding_dx(dy, indices, num_weight, scale, padding_idx or None, dtype, out or None, accumulate) -> tensor
+PyObject* embedding_dx(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 8 || !PyLong_Check(a[2])) return nothing();
+  c10::DeviceIndex dev = -1;
+  const at::Tensor *dy = data_only(a[0], dev), *ids = plain(a[1], dev), *given = a[6] == Py_None ? nullptr : plain(a[6], dev);
+  if (!dy || !ids || (a[6] != Py_None && !given)) return nothing();
+  at::ScalarType type;
+  if (!type_of(a[5], given ? given->scalar_type() : dy->scalar_type(), &type)) return nothing();
+  const int code = code_of(dy->scalar_type()), index = index_code_of(ids->scalar_type());
+  const long long rows = PyLong_AsLongLong(a[2]), padding = a[4] == Py_None ? -1 : PyLong_AsLongLong(a[4]);
+  const double scale = PyFloat_AsDouble(a[3]);
+  const int accumulate = PyObject_IsTrue(a[7]);
+  if (PyErr_Occurred()) {
+    PyErr_Clear();
+    return nothing();
+  }
+  if (code < 0 || index < 0 || rows < 0 || rows >= (1ll << 31) || dy->dim() != ids->dim() + 1 ||
+      dy->sizes().slice(0, ids->dim()) != ids->sizes() || (accumulate && !given))
+    return nothing();
+  const int64_t width = dy->size(-1);
+  int64_t numel;
+  if (__builtin_mul_overflow((int64_t)rows, width, &numel) || numel > (int64_t(1) << 50)) return nothing();
+  if (given) {
+    std::vector<Range> ranges{range_of(*given, true), range_of(*dy, false), range_of(*ids, false)};
+    if (given->dim() != 2 || given->size(0) != rows || given->size(1) != width || given->scalar_type() != type || overlap(ranges))
+      return nothing();
+  }
+  PyObject* held = given ? Py_NewRef(a[6]) : nullptr;
+  at::Tensor made;
+  int rc;
+  {
+    NoGil released;
+    if (!given) made = new_tensor({(int64_t)rows, width}, type);
+    const at::Tensor& out = given ? *given : made;
+    const size_t bytes = abi.embedding_dx_workspace_bytes(ids->numel(), width);
+    c10::DataPtr workspace;
+    if (bytes) workspace = c10::cuda::CUDACachingAllocator::get()->allocate(bytes);
+    if (given) given->unsafeGetTensorImpl()->bump_version();
+    rc = abi.embedding_dx(dy->const_data_ptr(), code, ids->const_data_ptr(), index, ids->numel(), rows, width, (float)scale, padding,
+                          accumulate, out.mutable_data_ptr(), code_of(type), workspace.get(), bytes, current_stream(dev));
+  }
+  if (rc != RAFB200_OK) {
+    Py_XDECREF(held);
+    return PyLong_FromLong(rc);
+  }
+  return given ? held : THPVariable_Wrap(std::move(made));
+}
+
+// distill(dy or None, pred, teacher_logits, teacher_ids, stats or None, labels or None, temperature, alpha, ignore_index, grad_scale, what)
+// what 0: (loss, stats); 1: dpred from stats; 2: (loss, dpred)
+PyObject* distill(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 11) return nothing();
+  c10::DeviceIndex dev = -1;
+  const long what = PyLong_AsLong(a[10]);
+  const long long ignore = PyLong_AsLongLong(a[8]);
+  const double temperature = PyFloat_AsDouble(a[6]), alpha = PyFloat_AsDouble(a[7]), grad_scale = PyFloat_AsDouble(a[9]);
+  if (PyErr_Occurred()) {
+    PyErr_Clear();
+    return nothing();
+  }
+  auto optional = [&](PyObject* o, const at::Tensor*& t) {
+    t = o == Py_None ? nullptr : plain(o, dev);
+    return o == Py_None || t;
+  };
+  const at::Tensor *teacher = data_only(a[2], dev), *ids = plain(a[3], dev), *dy, *stats, *labels;
+  if (!teacher || !ids || !optional(a[0], dy) || !optional(a[4], stats) || !optional(a[5], labels)) return nothing();
+  // pred: dense, or rows of a matrix further apart
+  if (!THPVariable_CheckExact(a[1])) return nothing();
+  const at::Tensor& pred = THPVariable_Unpack(a[1]);
+  if (!pred.defined() || pred.layout() != at::kStrided || !pred.is_cuda() || pred.key_set().has_any(kWrapped) ||
+      pred.device().index() != dev || pred._fw_grad(0).defined() || (what != 1 && pred.requires_grad() && c10::GradMode::is_enabled()))
+    return nothing();
+  const int64_t dims = pred.dim();
+  if (dims < 1 || pred.size(-1) < 1 || teacher->dim() != dims || ids->sizes() != teacher->sizes()) return nothing();
+  const int64_t v = pred.size(-1), rows = pred.numel() / v;
+  int64_t ld = v;
+  if (!pred.is_contiguous()) {
+    if (dims != 2 || (v > 1 && pred.stride(1) != 1) || (rows > 1 && pred.stride(0) < v)) return nothing();
+    if (rows > 1) ld = pred.stride(0);
+  }
+  const at::IntArrayRef lead = pred.sizes().slice(0, dims - 1);
+  if (teacher->sizes().slice(0, dims - 1) != lead || (labels && labels->sizes() != lead)) return nothing();
+  if (dy && (dy->scalar_type() != at::kFloat || (dy->dim() != 0 && dy->sizes() != lead))) return nothing();
+  c10::SmallVector<int64_t, 6> stats_shape(lead.begin(), lead.end());
+  stats_shape.push_back(4);
+  if (what == 1 && (!stats || stats->scalar_type() != at::kFloat || stats->sizes() != at::IntArrayRef(stats_shape))) return nothing();
+  rafb200_distill d{};
+  d.pred = pred.const_data_ptr();
+  d.teacher_logits = teacher->const_data_ptr();
+  d.teacher_ids = ids->const_data_ptr();
+  d.labels = labels ? labels->const_data_ptr() : nullptr;
+  d.n = rows;
+  d.v = v;
+  d.ld = ld;
+  d.ignore_index = ignore;
+  d.temperature = temperature;
+  d.alpha = alpha;
+  d.pred_dtype = code_of(pred.scalar_type());
+  d.teacher_dtype = code_of(teacher->scalar_type());
+  d.ids_dtype = index_code_of(ids->scalar_type());
+  d.labels_dtype = labels ? index_code_of(labels->scalar_type()) : RAFB200_I64;
+  if (teacher->size(-1) > 0x7fffffff || d.pred_dtype < 0 || d.teacher_dtype < 0 || d.ids_dtype < 0 || d.labels_dtype < 0 ||
+      (!labels && alpha != 1.0))
+    return nothing();
+  d.k = (int)teacher->size(-1);
+  const float* weights = dy ? dy->const_data_ptr<float>() : nullptr;
+  const int step = dy && dy->dim() != 0;
+  at::Tensor loss, other;  // other: stats or dpred
+  int rc;
+  {
+    NoGil released;
+    void* stream = current_stream(dev);
+    if (what != 1) loss = new_tensor(lead, at::kFloat);
+    other = what == 0 ? new_tensor(stats_shape, at::kFloat) : new_tensor(pred.sizes(), pred.scalar_type());
+    if (what == 0)
+      rc = abi.distill_loss(&d, loss.mutable_data_ptr<float>(), other.mutable_data_ptr<float>(), stream);
+    else if (what == 1)
+      rc = abi.distill_loss_dpred(&d, weights, step, (float)grad_scale, stats->const_data_ptr<float>(), other.mutable_data_ptr(), v, stream);
+    else
+      rc = abi.distill_loss_with_dpred(&d, weights, step, (float)grad_scale, loss.mutable_data_ptr<float>(), other.mutable_data_ptr(), v, stream);
+  }
+  if (rc != RAFB200_OK) return PyLong_FromLong(rc);
+  if (what == 1) return THPVariable_Wrap(std::move(other));
+  PyObject* out = PyTuple_New(2);
+  if (!out) return nullptr;
+  PyTuple_SET_ITEM(out, 0, THPVariable_Wrap(std::move(loss)));
+  PyTuple_SET_ITEM(out, 1, THPVariable_Wrap(std::move(other)));
+  return out;
+}
+
 using Fast = PyObject* (*)(PyObject*, PyObject* const*, Py_ssize_t);
 
 // A C++ exception (the allocator out of memory, first of all) becomes the Python exception that
@@ -472,6 +655,9 @@ PyMethodDef kMethods[] = {
     {"fuse_tensor", fast<fuse_tensor>(), METH_FASTCALL, "raf.op.fuse_tensor"},
     {"defuse_tensor", fast<defuse_tensor>(), METH_FASTCALL,
      "raf.op.defuse_tensor"},
+    {"embedding", fast<embedding>(), METH_FASTCALL, "raf.op.embedding"},
+    {"embedding_dx", fast<embedding_dx>(), METH_FASTCALL, "raf.op.embedding_dx"},
+    {"distill", fast<distill>(), METH_FASTCALL, "the distillation loss and its gradient"},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_ops", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};

@@ -385,6 +385,12 @@ def embedding(x, indices, scale=1.0, padding_idx=None, dtype=None, out=None, str
     (default: x's), rounded once.  An index outside [0, rows) reads as a row of zeros.  Where ``x`` requires a
     gradient, backward is :func:`embedding_dx`, for which ``padding_idx`` names an index that counts nothing.
     """
+    if out is None and stream is None:
+        r = _lib.ops().embedding(x, indices, scale, dtype)
+        if isinstance(r, torch.Tensor):
+            return r
+        if r is not None:
+            check(r)
     _check_cuda(x, indices)
     _same_device(x, indices)
     if x.dim() != 2:
@@ -421,6 +427,12 @@ def embedding_dx(dy, indices, num_weight, scale=1.0, padding_idx=None, dtype=Non
     without a token stay as they are.  Indices equal to ``padding_idx`` or outside [0, num_weight) count nothing.
     The same call gives the same bits: sums run in an order that the indices fix.
     """
+    if stream is None:
+        r = _lib.ops().embedding_dx(dy, indices, num_weight, scale, padding_idx, dtype, out, accumulate)
+        if isinstance(r, torch.Tensor):
+            return r
+        if r is not None:
+            check(r)
     _check_cuda(dy, indices)
     _same_device(dy, indices)
     if dy.dim() != indices.dim() + 1 or dy.shape[:-1] != indices.shape:
@@ -544,6 +556,12 @@ def distill_loss(pred, teacher_logits, teacher_ids, labels=None, temperature=1.0
 
     ``stats`` is what :func:`distill_loss_dpred` takes.  Where ``pred`` requires a gradient, backward calls it.
     """
+    if stream is None:
+        r = _lib.ops().distill(None, pred, teacher_logits, teacher_ids, None, labels, temperature, alpha, ignore_index, 1.0, 0)
+        if r.__class__ is tuple:
+            return r
+        if r is not None:
+            check(r)
     d = _distill_args(pred, teacher_logits, teacher_ids, labels, temperature, alpha, ignore_index)
     if torch.is_grad_enabled() and teacher_logits.requires_grad:
         raise ValueError("distill_loss: the teacher gets no gradient; detach its logits")
@@ -564,6 +582,12 @@ def distill_loss_dpred(dy, pred, teacher_logits, teacher_ids, stats, labels=None
     ``dy`` is fp32, one weight per row, one for all rows (0-dimensional), or None for 1; ``grad_scale`` is the loss scale that
     the optimizers' own ``grad_scale`` takes back.  ``out`` takes the result and may be ``pred`` itself.
     """
+    if out is None and stream is None:
+        r = _lib.ops().distill(dy, pred, teacher_logits, teacher_ids, stats, labels, temperature, alpha, ignore_index, grad_scale, 1)
+        if isinstance(r, torch.Tensor):
+            return r
+        if r is not None:
+            check(r)
     d = _distill_args(pred, teacher_logits, teacher_ids, labels, temperature, alpha, ignore_index)
     weights, step = _weights_of(dy, pred)
     _check_cuda(stats)
@@ -581,6 +605,12 @@ def distill_loss_with_dpred(dy, pred, teacher_logits, teacher_ids, labels=None, 
                             grad_scale=1.0, out=None, stream=None):
     """:func:`distill_loss` and :func:`distill_loss_dpred` in one pass over the logits, where the rows' weights ``dy`` are
     known beforehand: (loss, dpred).  Both are data, part of no autograd graph."""
+    if out is None and stream is None:
+        r = _lib.ops().distill(dy, pred, teacher_logits, teacher_ids, None, labels, temperature, alpha, ignore_index, grad_scale, 2)
+        if r.__class__ is tuple:
+            return r
+        if r is not None:
+            check(r)
     d = _distill_args(pred, teacher_logits, teacher_ids, labels, temperature, alpha, ignore_index)
     weights, step = _weights_of(dy, pred)
     with _launching(pred, stream) as raw:
