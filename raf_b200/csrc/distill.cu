@@ -17,12 +17,20 @@
 
 namespace rafb200 {
 
-constexpr int kDistillThreads = 512;
+// Bound: HBM in the sweeps over the logits, as long as an element takes few instructions: at 6.45 TB/s an SM has 22
+// issue slots per 32 elements of 2 bytes read and written, and an exponential fills the special-function unit for 8 of
+// them.  So two elements are computed by one instruction (f32x2), maxima are taken on the raw pairs, and where the second
+// exponential is a small power of the first (T = 2 or 4) it is multiplied out.
+constexpr int kDistillThreads = 256;
 constexpr int kDistillWarps = kDistillThreads / 32;
 constexpr int kDistillUnroll = 4;
 constexpr int kMaxTeacher = 1024;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
+
+// How exp(z - m) follows from exp((z - m) / T): not needed (or T = 1), an exponential of its own, the square (T = 2),
+// the fourth power (T = 4).
+enum Second { kNone, kOwn, kSquare, kFourth };
 
 struct DistillArgs {
   const void* pred;
@@ -31,7 +39,7 @@ struct DistillArgs {
   Ids labels;       // p == nullptr: none
   const float* dy;  // one weight per row (dy_step 1), one for all (0), or nullptr: 1
   float* loss;
-  float4* stats;    // per row: maximum, sum of exponentials at the temperature, the same at one, 0
+  float4* stats;    // per row: maximum, sum of exponentials at the temperature, the same at one, sum of the teacher's weights - 1
   void* out;
   int64_t n, v, ld, ld_out, ignore;
   int k, teacher_type, dy_step;
@@ -44,6 +52,90 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+
+// Two fp32 numbers in a register pair.
+struct Two {
+  uint64_t r;
+  __device__ __forceinline__ Two() {}
+  __device__ __forceinline__ Two(float lo, float hi) { asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi)); }
+  __device__ __forceinline__ float lo() const {
+    float a, b;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(r));
+    return a;
+  }
+  __device__ __forceinline__ float hi() const {
+    float a, b;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(r));
+    return b;
+  }
+};
+__device__ __forceinline__ Two operator+(Two a, Two b) {
+  Two c;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(c.r) : "l"(a.r), "l"(b.r));
+  return c;
+}
+__device__ __forceinline__ Two operator*(Two a, Two b) {
+  Two c;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(c.r) : "l"(a.r), "l"(b.r));
+  return c;
+}
+__device__ __forceinline__ Two fma2(Two a, Two b, Two d) {
+  Two c;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(c.r) : "l"(a.r), "l"(b.r), "l"(d.r));
+  return c;
+}
+__device__ __forceinline__ Two ex2(Two a) { return Two(ex2(a.lo()), ex2(a.hi())); }
+
+// The elements of 16 bytes: their number, pair j of them, and the largest.
+template <typename T>
+struct Raw {
+  static constexpr int kPer = 16 / sizeof(T);
+  static __device__ __forceinline__ uint32_t word(const uint4& r, int i) { return i == 0 ? r.x : i == 1 ? r.y : i == 2 ? r.z : r.w; }
+  static __device__ __forceinline__ Two pair(const uint4& r, int j) {
+    if constexpr (sizeof(T) == 4) {
+      return Two(__uint_as_float(word(r, 2 * j)), __uint_as_float(word(r, 2 * j + 1)));
+    } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+      return Two(__uint_as_float(word(r, j) << 16), __uint_as_float(word(r, j) & 0xffff0000u));
+    } else {
+      const uint32_t w = word(r, j);
+      __half2 h;
+      memcpy(&h, &w, 4);
+      const float2 f = __half22float2(h);
+      return Two(f.x, f.y);
+    }
+  }
+  // pairwise maxima of the raw words; NaN gives way to numbers (their exponentials carry it on)
+  static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+    if constexpr (sizeof(T) == 4) {
+      return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+    } else {
+      using P = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+      P x, y;
+      memcpy(&x, &a, 4);
+      memcpy(&y, &b, 4);
+      x = __hmax2(x, y);
+      memcpy(&a, &x, 4);
+      return a;
+    }
+  }
+  static __device__ __forceinline__ uint32_t max2(const uint4& r) { return max2(max2(r.x, r.y), max2(r.z, r.w)); }
+  static __device__ __forceinline__ float max1(uint32_t w) {
+    if constexpr (sizeof(T) == 4) return __uint_as_float(w);
+    const Two p = pair(make_uint4(w, w, w, w), 0);
+    return fmaxf(p.lo(), p.hi());
+  }
+  static __device__ __forceinline__ uint32_t put(Two p) {  // 16-bit types: a pair rounded into a word
+    uint32_t w;
+    if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(p.lo(), p.hi());
+      memcpy(&w, &h, 4);
+    } else {
+      const __half2 h = __floats2half2_rn(p.lo(), p.hi());
+      memcpy(&w, &h, 4);
+    }
+    return w;
+  }
+};
 
 __device__ __forceinline__ float load_teacher(const DistillArgs& a, int64_t i) {
   if (a.teacher_type == RAFB200_F32) return static_cast<const float*>(a.teacher)[i];
@@ -59,7 +151,7 @@ struct Running {
 __device__ __forceinline__ float base_of(float top) { return top == -INFINITY ? 0.f : top; }
 __device__ __forceinline__ float power(float z, float base, float c) { return ex2((z - base) * c); }
 
-template <bool TWO>
+template <Second S>
 __device__ __forceinline__ Running merge(const Running& x, const Running& y, float c) {
   Running r;
   r.top = fmaxf(x.top, y.top);
@@ -67,24 +159,29 @@ __device__ __forceinline__ Running merge(const Running& x, const Running& y, flo
   // sums over -infinity alone are 0, or NaN, and stay it, whatever the distance of the maxima
   r.soft = x.soft * (x.top == -INFINITY ? 1.f : ex2(dx * c)) + y.soft * (y.top == -INFINITY ? 1.f : ex2(dy * c));
   r.hard = 0.f;
-  if (TWO)
+  if (S != kNone)
     r.hard = x.hard * (x.top == -INFINITY ? 1.f : ex2(dx * kLog2e)) + y.hard * (y.top == -INFINITY ? 1.f : ex2(dy * kLog2e));
   return r;
 }
 
-// A block's part of a row: 16-byte groups [from, to) of the aligned middle; the elements in front of
-// the middle are the first block's, those behind it the last one's.
+// A block's part of a row: groups [from, to) of 16 bytes of the part that is aligned at `p`; the elements in front of
+// that part are the first block's, those behind it the last one's.  With `trim` the first and the last group
+// count to those.
 template <typename T>
 struct Slice {
-  static constexpr int kPer = 16 / sizeof(T);
-  int64_t head, from, to, body;  // elements in front; groups; first element behind the middle
-  int edge;                      // elements of this block outside the middle: thread i < edge takes edge_at(i)
-  int64_t v;
+  static constexpr int kPer = Raw<T>::kPer;
+  int64_t head, from, to, body;  // elements in front; groups; first element behind
+  int edge;                      // elements of this block outside the groups: thread i < edge takes edge_at(i)
   int first;                     // of them in front
 
-  __device__ __forceinline__ Slice(const T* row, int64_t v_, int slice, int slices) : v(v_) {
-    head = min((int64_t)((-(intptr_t)row & 15) / sizeof(T)), v);
-    const int64_t groups = (v - head) / kPer, each = (groups + slices - 1) / slices;
+  __device__ __forceinline__ Slice(const T* p, int64_t v, int slice, int slices, bool trim) {
+    head = min((int64_t)((-(intptr_t)p & 15) / sizeof(T)), v);
+    int64_t groups = (v - head) / kPer;
+    if (trim && groups > 0) {
+      head += kPer;
+      groups = max(groups - 2, (int64_t)0);
+    }
+    const int64_t each = (groups + slices - 1) / slices;
     from = min(slice * each, groups);
     to = min(from + each, groups);
     body = head + groups * kPer;
@@ -111,8 +208,8 @@ struct Entries {
   static size_t bytes(int k) { return (size_t)(k + 1) * 12; }
 };
 
-// softmax over the present entries; the sum of the weights (1 or 0), and with `loss` sum p (log p - log q).  One warp.
-__device__ __forceinline__ float weigh(const Entries& e, int k, float c, float base, float log2_soft, bool want, float* kl) {
+// softmax over the present entries; the sum of the weights (1 or 0), and with `kl` sum p (log p - log q).  One warp.
+__device__ __forceinline__ float weigh(const Entries& e, int k, float c, float base, float log2_soft, float* kl) {
   const int lane = threadIdx.x & 31;
   float top = -INFINITY;
   for (int i = lane; i < k; i += 32)
@@ -130,10 +227,10 @@ __device__ __forceinline__ float weigh(const Entries& e, int k, float c, float b
   for (int i = lane; i < k; i += 32) {
     const float t = (e.p[i] - t_base) * c;
     const float w = e.at[i] >= 0 && some ? ex2(t) * inv : 0.f;
-    if (want && !(w == 0.f)) part = fmaf(w, (t - log2_sum) - ((e.z[i] - base) * c - log2_soft), part);  // log2 p - log2 q
+    if (kl && !(w == 0.f)) part = fmaf(w, (t - log2_sum) - ((e.z[i] - base) * c - log2_soft), part);  // log2 p - log2 q
     e.p[i] = w;
   }
-  if (want) *kl = warp_sum(part) * kLn2;
+  if (kl) *kl = warp_sum(part) * kLn2;
   return isnan(sum) ? sum : some ? 1.f : 0.f;
 }
 
@@ -152,59 +249,114 @@ __device__ __forceinline__ void load_entries(const DistillArgs& a, const Entries
 // teach * (sum of p), and minus hit at the label.
 struct Coefficients {
   float c, base, soft, hard, teach, hit;
-  template <bool TWO>
+  template <Second S>
   __device__ __forceinline__ float at(float z) const {
-    float g = soft * power(z, base, c);
-    if (TWO) g = fmaf(hard, power(z, base, kLog2e), g);
-    return g;
+    const float e = power(z, base, c);
+    if (S == kNone) return soft * e;
+    if (S == kOwn) return fmaf(hard, power(z, base, kLog2e), soft * e);
+    const float f = S == kFourth ? e * e * e : e;
+    return fmaf(hard, f, soft) * e;
+  }
+  template <Second S>
+  __device__ __forceinline__ Two at(Two z) const {
+    const Two x = z + Two(-base, -base), e = ex2(x * Two(c, c)), w(soft, soft);
+    if (S == kNone) return w * e;
+    if (S == kOwn) return fma2(Two(hard, hard), ex2(x * Two(kLog2e, kLog2e)), w * e);
+    const Two f = S == kFourth ? e * e * e : e;
+    return fma2(Two(hard, hard), f, w) * e;
   }
 };
 
-template <bool TWO>
-__device__ __forceinline__ Coefficients coefficients(const DistillArgs& a, int64_t row, float4 stats, float some, bool labels) {
+template <Second S>
+__device__ __forceinline__ Coefficients coefficients(const DistillArgs& a, int64_t row, float4 stats, bool labels) {
   const float w = (a.dy ? a.dy[row * a.dy_step] : 1.f) * a.grad_scale;
   Coefficients co;
   co.c = a.c;
   co.base = base_of(stats.x);
   co.teach = w * a.soft_grad;
   co.hit = labels ? w * a.hard : 0.f;
-  co.soft = co.teach * some / stats.y;
+  co.soft = co.teach * (stats.w + 1.f) / stats.y;
   co.hard = co.hit / stats.z;
-  if (!TWO) {  // one exponential serves both terms, or there is one term only
+  if (S == kNone) {  // one exponential serves both terms, or there is one term only
     co.soft += labels ? co.hit / stats.y : 0.f;
     co.hard = 0.f;
   }
   return co;
 }
 
-// The gradient of a slice: `get(i)` is the group of 16 bytes i, `edge` this thread's element outside the middle.
-template <typename T, bool TWO, typename Get>
-__device__ __forceinline__ void write_slice(const Slice<T>& s, T* out, const Coefficients& co, float edge, const Get& get) {
+// 16 bytes from an address that is 4 Q + r bytes (r = bits / 8, 0 or 2) behind a 16-byte boundary.
+template <int Q>
+__device__ __forceinline__ uint4 load_shifted(const char* p, uint32_t bits) {
+  if constexpr (Q < 0) {
+    return *reinterpret_cast<const uint4*>(p);
+  } else {
+    const uint4* q = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(p) & ~uintptr_t(15));
+    const uint4 a = q[0], b = q[1];
+    const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+    return make_uint4(__funnelshift_r(w[Q], w[Q + 1], bits), __funnelshift_r(w[Q + 1], w[Q + 2], bits),
+                      __funnelshift_r(w[Q + 2], w[Q + 3], bits), __funnelshift_r(w[Q + 3], w[(Q + 4) & 7], bits));
+  }
+}
+
+// The gradient of the groups of a slice, which is aligned at `out`.
+template <typename T, Second S, int Q>
+__device__ __forceinline__ void write_groups(const Slice<T>& s, const T* z, T* out, const Coefficients& co) {
   constexpr int per = Slice<T>::kPer;
-  T* middle = out + s.head;
-  const bool aligned = (reinterpret_cast<uintptr_t>(middle) & 15) == 0;
-  for (int64_t i = s.from + threadIdx.x; i < s.to; i += kDistillThreads) {
-    float z[per];
-    Group<T, 8>::template unpack<T>(get(i), z);
+  const char* from = reinterpret_cast<const char*>(z + s.head);
+  uint4* to = reinterpret_cast<uint4*>(out + s.head);
+  const uint32_t bits = (reinterpret_cast<uintptr_t>(from) & 3) * 8;
+  for (int64_t i0 = s.from + threadIdx.x; i0 < s.to; i0 += kDistillThreads * kDistillUnroll) {
+    uint4 raw[kDistillUnroll];
 #pragma unroll
-    for (int j = 0; j < per; ++j) z[j] = co.at<TWO>(z[j]);
-    if (aligned) {
-      reinterpret_cast<uint4*>(middle)[i] = Group<T, 8>::template pack<T>(z);
-    } else {
+    for (int u = 0; u < kDistillUnroll; ++u)
+      if (i0 + u * kDistillThreads < s.to) raw[u] = load_shifted<Q>(from + (i0 + u * kDistillThreads) * 16, bits);
 #pragma unroll
-      for (int j = 0; j < per; ++j) middle[i * per + j] = Elem<T>::from_f32(z[j]);
+    for (int u = 0; u < kDistillUnroll; ++u) {
+      if (i0 + u * kDistillThreads >= s.to) break;
+      uint4 r;
+      if constexpr (sizeof(T) == 4) {
+        const Two a = co.at<S>(Raw<T>::pair(raw[u], 0)), b = co.at<S>(Raw<T>::pair(raw[u], 1));
+        r = make_uint4(__float_as_uint(a.lo()), __float_as_uint(a.hi()), __float_as_uint(b.lo()), __float_as_uint(b.hi()));
+      } else {
+        r = make_uint4(Raw<T>::put(co.at<S>(Raw<T>::pair(raw[u], 0))), Raw<T>::put(co.at<S>(Raw<T>::pair(raw[u], 1))),
+                       Raw<T>::put(co.at<S>(Raw<T>::pair(raw[u], 2))), Raw<T>::put(co.at<S>(Raw<T>::pair(raw[u], 3))));
+      }
+      to[i0 + u * kDistillThreads] = r;
     }
   }
-  if ((int)threadIdx.x < s.edge) out[s.edge_at(threadIdx.x)] = Elem<T>::from_f32(co.at<TWO>(edge));
+}
+
+// z and out lie at the same distance from a 16-byte boundary: nothing is shifted.
+template <typename T>
+__device__ __forceinline__ bool alike(const T* z, const T* out) {
+  return ((reinterpret_cast<uintptr_t>(z) ^ reinterpret_cast<uintptr_t>(out)) & 15) == 0;
+}
+
+template <typename T, Second S>
+__device__ __forceinline__ void write_slice(const Slice<T>& s, const T* z, T* out, const Coefficients& co) {
+  if (alike(z, out)) {
+    write_groups<T, S, -1>(s, z, out, co);
+  } else {
+    switch ((reinterpret_cast<uintptr_t>(z + s.head) & 15) >> 2) {
+      case 0: write_groups<T, S, 0>(s, z, out, co); break;
+      case 1: write_groups<T, S, 1>(s, z, out, co); break;
+      case 2: write_groups<T, S, 2>(s, z, out, co); break;
+      default: write_groups<T, S, 3>(s, z, out, co); break;
+    }
+  }
+  if ((int)threadIdx.x < s.edge) {
+    const int64_t j = s.edge_at(threadIdx.x);
+    out[j] = Elem<T>::from_f32(co.at<S>(Elem<T>::to_f32(z[j])));
+  }
 }
 
 // The elements that the teacher or the label names, once each however often they are named.
-template <typename T, bool TWO>
+template <typename T, Second S>
 __device__ __forceinline__ void write_entries(const DistillArgs& a, const Entries& e, const Slice<T>& s, T* out, const Coefficients& co,
-                                              bool first_slice, bool last_slice) {
+                                              int slice) {
   for (int i = threadIdx.x; i <= a.k; i += kDistillThreads) {
     const int j = e.at[i];
-    if (j < 0 || !s.owns(j, first_slice, last_slice)) continue;
+    if (j < 0 || !s.owns(j, slice == 0, slice == a.slices - 1)) continue;
     bool again = false;
     float p = e.p[i];
     for (int q = 0; q <= a.k; ++q) {
@@ -213,7 +365,7 @@ __device__ __forceinline__ void write_entries(const DistillArgs& a, const Entrie
       p += e.p[q];
     }
     if (again) continue;
-    float g = co.at<TWO>(e.z[i]) - co.teach * p;
+    float g = co.at<S>(e.z[i]) - co.teach * p;
     if (e.at[a.k] == j) g -= co.hit;
     out[j] = Elem<T>::from_f32(g);
   }
@@ -221,15 +373,15 @@ __device__ __forceinline__ void write_entries(const DistillArgs& a, const Entrie
 
 template <typename T>
 __device__ __forceinline__ void zero_slice(const Slice<T>& s, T* out) {
-  for (int64_t i = s.from * Slice<T>::kPer + threadIdx.x; i < s.to * Slice<T>::kPer; i += kDistillThreads)
-    out[s.head + i] = Elem<T>::from_f32(0.f);
+  uint4* to = reinterpret_cast<uint4*>(out + s.head);
+  for (int64_t i = s.from + threadIdx.x; i < s.to; i += kDistillThreads) to[i] = make_uint4(0, 0, 0, 0);
   if ((int)threadIdx.x < s.edge) out[s.edge_at(threadIdx.x)] = Elem<T>::from_f32(0.f);
 }
 
 // Loss, and with GRAD the gradient, of a row by a cluster of `slices` blocks: one pass with a running maximum and its
-// sums, joined over threads, warps and blocks.
-template <typename T, bool TWO, bool GRAD>
-__global__ void __launch_bounds__(kDistillThreads) distill_kernel(DistillArgs a) {
+// sums, joined over threads, warps and blocks; the gradient reads the row again, which the L2 still holds.
+template <typename T, Second S, bool GRAD>
+__global__ void __launch_bounds__(kDistillThreads, 4) distill_kernel(DistillArgs a) {
   constexpr int per = Slice<T>::kPer;
   extern __shared__ char smem[];
   __shared__ Running warps[kDistillWarps];
@@ -242,64 +394,71 @@ __global__ void __launch_bounds__(kDistillThreads) distill_kernel(DistillArgs a)
   const int64_t row = blockIdx.x / a.slices;
   const int slice = blockIdx.x % a.slices;
   const T* z = static_cast<const T*>(a.pred) + row * a.ld;
-  const Slice<T> s(z, a.v, slice, a.slices);
   T* out = GRAD ? static_cast<T*>(a.out) + row * a.ld_out : nullptr;
   const bool labels = a.labels.p != nullptr;
   const int64_t label = labels ? a.labels[row] : -1;
   if (labels && (label == a.ignore || (uint64_t)label >= (uint64_t)a.v)) {  // the same for every block of the cluster
     if (slice == 0 && tid == 0) {
       a.loss[row] = 0.f;
-      if (a.stats) a.stats[row] = make_float4(0.f, 1.f, 1.f, 0.f);
+      if (a.stats) a.stats[row] = make_float4(0.f, 1.f, 1.f, -1.f);
     }
-    if (GRAD) zero_slice(s, out);
+    if (GRAD) zero_slice(Slice<T>(out, a.v, slice, a.slices, false), out);
     return;
   }
   load_entries(a, e, row, z, label);
 
   Running run{-INFINITY, 0.f, 0.f};
+  const Slice<T> s(z, a.v, slice, a.slices, false);
   const uint4* middle = reinterpret_cast<const uint4*>(z + s.head);
-  const T lowest = Elem<T>::from_f32(-INFINITY);
-  const uint32_t pad = sizeof(T) == 4 ? __float_as_uint(-INFINITY) : (uint32_t)reinterpret_cast<const uint16_t&>(lowest) * 0x10001u;
+  const uint32_t low = sizeof(T) == 4 ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;  // -infinity
+  Two soft(0.f, 0.f), hard(0.f, 0.f);
   for (int64_t i0 = s.from + tid; i0 < s.to; i0 += kDistillThreads * kDistillUnroll) {
     uint4 raw[kDistillUnroll];
+    uint32_t most = low;
 #pragma unroll
     for (int u = 0; u < kDistillUnroll; ++u) {
       const int64_t i = i0 + u * kDistillThreads;
-      raw[u] = i < s.to ? middle[i] : make_uint4(pad, pad, pad, pad);
+      raw[u] = i < s.to ? middle[i] : make_uint4(low, low, low, low);
     }
-    float f[kDistillUnroll * per];
-    float top = run.top;
 #pragma unroll
-    for (int u = 0; u < kDistillUnroll; ++u) Group<T, 8>::template unpack<T>(raw[u], f + u * per);
+    for (int u = 0; u < kDistillUnroll; ++u) most = Raw<T>::max2(most, Raw<T>::max2(raw[u]));
+    const float top = fmaxf(run.top, Raw<T>::max1(most)), base = base_of(top), from = base_of(run.top) - base;
+    const float fs = run.top == -INFINITY ? 1.f : ex2(from * a.c), fh = run.top == -INFINITY ? 1.f : ex2(from * kLog2e);
+    run.top = top;
+    soft = soft * Two(fs, fs);
+    if (S != kNone) hard = hard * Two(fh, fh);
+    const Two nb(-base, -base), c2(a.c, a.c);
 #pragma unroll
-    for (int j = 0; j < kDistillUnroll * per; ++j) top = fmaxf(top, f[j]);
-    Running next = merge<TWO>(run, Running{top, 0.f, 0.f}, a.c);
-    const float base = base_of(top);
+    for (int u = 0; u < kDistillUnroll; ++u) {
+      if (i0 + u * kDistillThreads >= s.to) break;
 #pragma unroll
-    for (int j = 0; j < kDistillUnroll * per; ++j) {
-      next.soft += power(f[j], base, a.c);
-      if (TWO) next.hard += power(f[j], base, kLog2e);
+      for (int j = 0; j < per / 2; ++j) {
+        const Two x = Raw<T>::pair(raw[u], j) + nb, p = ex2(x * c2);
+        soft = soft + p;
+        if (S == kOwn) hard = hard + ex2(x * Two(kLog2e, kLog2e));
+        if (S == kSquare) hard = fma2(p, p, hard);
+        if (S == kFourth) hard = fma2(p * p, p * p, hard);
+      }
     }
-    run = next;
   }
-  float edge = 0.f;
+  run.soft = soft.lo() + soft.hi();
+  run.hard = hard.lo() + hard.hi();
   if (tid < s.edge) {
-    edge = Elem<T>::to_f32(z[s.edge_at(tid)]);
-    const float base = base_of(edge);
-    run = merge<TWO>(run, Running{edge, power(edge, base, a.c), TWO ? power(edge, base, kLog2e) : 0.f}, a.c);
+    const float edge = Elem<T>::to_f32(z[s.edge_at(tid)]), base = base_of(edge);
+    run = merge<S>(run, Running{edge, power(edge, base, a.c), S != kNone ? power(edge, base, kLog2e) : 0.f}, a.c);
   }
 #pragma unroll
   for (int d = 16; d; d >>= 1) {
     const Running other{__shfl_xor_sync(0xffffffffu, run.top, d), __shfl_xor_sync(0xffffffffu, run.soft, d),
-                        TWO ? __shfl_xor_sync(0xffffffffu, run.hard, d) : 0.f};
+                        S != kNone ? __shfl_xor_sync(0xffffffffu, run.hard, d) : 0.f};
     // the lower lane's sums first, on both sides
-    run = lane & d ? merge<TWO>(other, run, a.c) : merge<TWO>(run, other, a.c);
+    run = lane & d ? merge<S>(other, run, a.c) : merge<S>(run, other, a.c);
   }
   if (lane == 0) warps[warp] = run;
   __syncthreads();
   if (tid == 0) {
     run = warps[0];
-    for (int w = 1; w < kDistillWarps; ++w) run = merge<TWO>(run, warps[w], a.c);
+    for (int w = 1; w < kDistillWarps; ++w) run = merge<S>(run, warps[w], a.c);
     whole = run;
   }
   if (a.slices > 1) {
@@ -311,7 +470,7 @@ __global__ void __launch_bounds__(kDistillThreads) distill_kernel(DistillArgs a)
         other.top = __uint_as_float(cluster_load(&whole.top, r));
         other.soft = __uint_as_float(cluster_load(&whole.soft, r));
         other.hard = __uint_as_float(cluster_load(&whole.hard, r));
-        run = merge<TWO>(run, other, a.c);
+        run = merge<S>(run, other, a.c);
       }
     }
     cluster_sync();  // read by all before one of them overwrites it or ends
@@ -320,11 +479,11 @@ __global__ void __launch_bounds__(kDistillThreads) distill_kernel(DistillArgs a)
   __syncthreads();
   run = whole;
   const float base = base_of(run.top);
-  const float4 stats = make_float4(run.top, run.soft, TWO ? run.hard : run.soft, 0.f);
+  float4 stats = make_float4(run.top, run.soft, S != kNone ? run.hard : run.soft, 0.f);
   if (warp == 0) {
     float kl = 0.f;
-    const float some = weigh(e, a.k, a.c, base, log2f(run.soft), true, &kl);
-    if (lane == 0) some_s = some;
+    stats.w = weigh(e, a.k, a.c, base, log2f(run.soft), &kl) - 1.f;
+    if (lane == 0) some_s = stats.w;
     if (lane == 0 && slice == 0) {
       float loss = a.soft_loss > 0.f ? a.soft_loss * kl : 0.f;  // a term without weight counts nothing, infinite or not
       if (labels && a.hard > 0.f) loss += a.hard * kLn2 * (log2f(stats.z) - (e.z[a.k] - base) * kLog2e);
@@ -334,46 +493,42 @@ __global__ void __launch_bounds__(kDistillThreads) distill_kernel(DistillArgs a)
   }
   if (!GRAD) return;
   __syncthreads();
-  const Coefficients co = coefficients<TWO>(a, row, stats, some_s, labels);
-  write_slice<T, TWO>(s, out, co, edge, [&](int64_t i) { return middle[i]; });
+  stats.w = some_s;
+  const Coefficients co = coefficients<S>(a, row, stats, labels);
+  const Slice<T> so(out, a.v, slice, a.slices, !alike(z, out));
+  write_slice<T, S>(so, z, out, co);
   __syncthreads();
-  write_entries<T, TWO>(a, e, s, out, co, slice == 0, slice == a.slices - 1);
+  write_entries<T, S>(a, e, so, out, co, slice);
 }
 
 // The gradient from the statistics that the forward pass has left.
-template <typename T, bool TWO>
-__global__ void __launch_bounds__(kDistillThreads) distill_dpred_kernel(DistillArgs a) {
+template <typename T, Second S>
+__global__ void __launch_bounds__(kDistillThreads, 4) distill_dpred_kernel(DistillArgs a) {
   extern __shared__ char smem[];
-  __shared__ float some_s;
   const Entries e(smem, a.k);
   grid_dependency_trigger();
   grid_dependency_wait();
   const int64_t row = blockIdx.x / a.slices;
   const int slice = blockIdx.x % a.slices;
   const T* z = static_cast<const T*>(a.pred) + row * a.ld;
-  const Slice<T> s(z, a.v, slice, a.slices);
   T* out = static_cast<T*>(a.out) + row * a.ld_out;
+  const Slice<T> s(out, a.v, slice, a.slices, !alike(z, out));
   const bool labels = a.labels.p != nullptr;
   const int64_t label = labels ? a.labels[row] : -1;
   if (labels && (label == a.ignore || (uint64_t)label >= (uint64_t)a.v)) {
-    zero_slice(s, out);
+    zero_slice(Slice<T>(out, a.v, slice, a.slices, false), out);
     return;
   }
   const float4 stats = a.stats[row];
-  // in place another block may have overwritten what its own slice names: those entries are not used here
+  // in place: this block's entries before any of it is overwritten (another block's are not used here)
   load_entries(a, e, row, z, label);
-  const float edge = (int)threadIdx.x < s.edge ? Elem<T>::to_f32(z[s.edge_at(threadIdx.x)]) : 0.f;
+  if (a.out == a.pred) __syncthreads();
+  const Coefficients co = coefficients<S>(a, row, stats, labels);
+  write_slice<T, S>(s, z, out, co);
   __syncthreads();
-  if (threadIdx.x < 32) {
-    const float some = weigh(e, a.k, a.c, 0.f, 0.f, false, nullptr);
-    if (threadIdx.x == 0) some_s = some;
-  }
+  if (threadIdx.x < 32) weigh(e, a.k, a.c, 0.f, 0.f, nullptr);
   __syncthreads();
-  const Coefficients co = coefficients<TWO>(a, row, stats, some_s, labels);
-  const uint4* middle = reinterpret_cast<const uint4*>(z + s.head);
-  write_slice<T, TWO>(s, out, co, edge, [&](int64_t i) { return middle[i]; });
-  __syncthreads();
-  write_entries<T, TWO>(a, e, s, out, co, slice == 0, slice == a.slices - 1);
+  write_entries<T, S>(a, e, s, out, co, slice);
 }
 
 static int check_args(const rafb200_distill* d, const char* who) {
@@ -411,8 +566,10 @@ static DistillArgs device_args(const rafb200_distill* d) {
   return a;
 }
 
-// Two exponentials an element where both terms count and their temperatures differ.
-static bool two_exps(const rafb200_distill* d) { return d->labels && d->alpha < 1.0 && d->temperature != 1.0; }
+static Second second_of(const rafb200_distill* d) {
+  if (!d->labels || d->alpha == 1.0 || d->temperature == 1.0) return kNone;  // one term, or both at one temperature
+  return d->temperature == 2.0 ? kSquare : d->temperature == 4.0 ? kFourth : kOwn;
+}
 
 static int row_slices(const rafb200_distill* d) {
   int slices = 1;
@@ -424,7 +581,12 @@ static int row_slices(const rafb200_distill* d) {
 template <typename F>
 static int with_case(const rafb200_distill* d, const F& f) {
   return with_type(d->pred_dtype, [&](auto t) {
-    return two_exps(d) ? f(t, std::integral_constant<bool, true>{}) : f(t, std::integral_constant<bool, false>{});
+    switch (second_of(d)) {
+      case kNone: return f(t, std::integral_constant<Second, kNone>{});
+      case kOwn: return f(t, std::integral_constant<Second, kOwn>{});
+      case kSquare: return f(t, std::integral_constant<Second, kSquare>{});
+      default: return f(t, std::integral_constant<Second, kFourth>{});
+    }
   });
 }
 
@@ -442,8 +604,8 @@ int rafb200_distill_loss(const rafb200_distill* d, float* loss, float* stats, vo
   a.loss = loss;
   a.stats = reinterpret_cast<float4*>(stats);
   a.slices = row_slices(d);
-  return with_case(d, [&](auto t, auto two) {
-    RAFB200_CUDA(launch_cluster(distill_kernel<decltype(t), decltype(two)::value, false>, a.slices, (unsigned)(d->n * a.slices),
+  return with_case(d, [&](auto t, auto second) {
+    RAFB200_CUDA(launch_cluster(distill_kernel<decltype(t), decltype(second)::value, false>, a.slices, (unsigned)(d->n * a.slices),
                                 kDistillThreads, Entries::bytes(d->k), static_cast<cudaStream_t>(stream), a));
     return (int)RAFB200_OK;
   });
@@ -472,8 +634,8 @@ int rafb200_distill_loss_dpred(const rafb200_distill* d, const float* dy, int dy
   a.out = dpred;
   a.ld_out = ld_dpred;
   a.slices = row_slices(d);
-  return with_case(d, [&](auto t, auto two) {
-    RAFB200_CUDA(launch_dependent(distill_dpred_kernel<decltype(t), decltype(two)::value>, dim3((unsigned)(d->n * a.slices)),
+  return with_case(d, [&](auto t, auto second) {
+    RAFB200_CUDA(launch_dependent(distill_dpred_kernel<decltype(t), decltype(second)::value>, dim3((unsigned)(d->n * a.slices)),
                                   kDistillThreads, Entries::bytes(d->k), static_cast<cudaStream_t>(stream), a));
     return (int)RAFB200_OK;
   });
@@ -493,8 +655,8 @@ int rafb200_distill_loss_with_dpred(const rafb200_distill* d, const float* dy, i
   a.out = dpred;
   a.ld_out = ld_dpred;
   a.slices = row_slices(d);
-  return with_case(d, [&](auto t, auto two) {
-    RAFB200_CUDA(launch_cluster(distill_kernel<decltype(t), decltype(two)::value, true>, a.slices, (unsigned)(d->n * a.slices),
+  return with_case(d, [&](auto t, auto second) {
+    RAFB200_CUDA(launch_cluster(distill_kernel<decltype(t), decltype(second)::value, true>, a.slices, (unsigned)(d->n * a.slices),
                                 kDistillThreads, Entries::bytes(d->k), static_cast<cudaStream_t>(stream), a));
     return (int)RAFB200_OK;
   });

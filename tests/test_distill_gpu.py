@@ -102,7 +102,7 @@ CASES = [(1, 1, 1), (2, 5, 3), (3, 17, 17), (1, 50257, 16), (40, 4096, 64), (300
 
 @pytest.mark.parametrize("n,v,k", CASES)
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
-@pytest.mark.parametrize("temperature,alpha", [(1.0, 1.0), (2.0, 0.5), (0.7, 0.25), (1.0, 0.5), (3.0, 0.0)])
+@pytest.mark.parametrize("temperature,alpha", [(1.0, 1.0), (2.0, 0.5), (0.7, 0.25), (1.0, 0.5), (3.0, 0.0), (4.0, 0.3)])
 def test_loss_and_gradient(n, v, k, dtype, temperature, alpha):
     labels = alpha < 1
     pred, teacher, ids, lab, dy = make(n, v, k, dtype, index=torch.int32 if n % 2 else torch.int64, labels=labels, pad=0 if n % 3 else 7)
