@@ -21,9 +21,10 @@ namespace rafb200 {
 // issue slots per 32 elements of 2 bytes read and written, and an exponential fills the special-function unit for 8 of
 // them.  So two elements are computed by one instruction (f32x2), maxima are taken on the raw pairs, and where the second
 // exponential is a small power of the first (T = 2 or 4) it is multiplied out.
-constexpr int kDistillThreads = 256;
+constexpr int kDistillThreads = 128;
 constexpr int kDistillWarps = kDistillThreads / 32;
 constexpr int kDistillUnroll = 4;
+constexpr int kDistillBlocks = 8;  // resident blocks of an SM: 64 registers a thread
 constexpr int kMaxTeacher = 1024;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
@@ -44,7 +45,7 @@ struct DistillArgs {
   int64_t n, v, ld, ld_out, ignore;
   int k, teacher_type, dy_step;
   float c, soft_loss, soft_grad, hard, grad_scale;  // log2(e) / T, alpha T^2, alpha T, 1 - alpha
-  int slices;       // blocks of a row
+  int slices_log;   // a row has 2^slices_log blocks
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -151,17 +152,15 @@ struct Running {
 __device__ __forceinline__ float base_of(float top) { return top == -INFINITY ? 0.f : top; }
 __device__ __forceinline__ float power(float z, float base, float c) { return ex2((z - base) * c); }
 
+// The sums of `x`, relative to its maximum, relative to a maximum that is no smaller.
 template <Second S>
-__device__ __forceinline__ Running merge(const Running& x, const Running& y, float c) {
-  Running r;
-  r.top = fmaxf(x.top, y.top);
-  const float base = base_of(r.top), dx = base_of(x.top) - base, dy = base_of(y.top) - base;
-  // sums over -infinity alone are 0, or NaN, and stay it, whatever the distance of the maxima
-  r.soft = x.soft * (x.top == -INFINITY ? 1.f : ex2(dx * c)) + y.soft * (y.top == -INFINITY ? 1.f : ex2(dy * c));
-  r.hard = 0.f;
-  if (S != kNone)
-    r.hard = x.hard * (x.top == -INFINITY ? 1.f : ex2(dx * kLog2e)) + y.hard * (y.top == -INFINITY ? 1.f : ex2(dy * kLog2e));
-  return r;
+__device__ __forceinline__ void rebase(Running& x, float top, float c) {
+  if (x.top != -INFINITY) {  // sums over -infinity alone are 0, or NaN, and stay it
+    const float d = x.top - top;
+    x.soft *= ex2(d * c);
+    if (S != kNone) x.hard *= ex2(d * kLog2e);
+  }
+  x.top = top;
 }
 
 // A block's part of a row: groups [from, to) of 16 bytes of the part that is aligned at `p`; the elements in front of
@@ -170,29 +169,29 @@ __device__ __forceinline__ Running merge(const Running& x, const Running& y, flo
 template <typename T>
 struct Slice {
   static constexpr int kPer = Raw<T>::kPer;
-  int64_t head, from, to, body;  // elements in front; groups; first element behind
-  int edge;                      // elements of this block outside the groups: thread i < edge takes edge_at(i)
-  int first;                     // of them in front
+  int head, from, to, body;  // elements in front; groups; first element behind
+  int edge;                  // elements of this block outside the groups: thread i < edge takes edge_at(i)
+  int first;                 // of them in front
 
-  __device__ __forceinline__ Slice(const T* p, int64_t v, int slice, int slices, bool trim) {
-    head = min((int64_t)((-(intptr_t)p & 15) / sizeof(T)), v);
-    int64_t groups = (v - head) / kPer;
+  __device__ __forceinline__ Slice(const T* p, int v, int slice, int slices_log, bool trim) {
+    head = min((int)((-(intptr_t)p & 15) / sizeof(T)), v);
+    int groups = (v - head) / kPer;
     if (trim && groups > 0) {
       head += kPer;
-      groups = max(groups - 2, (int64_t)0);
+      groups = max(groups - 2, 0);
     }
-    const int64_t each = (groups + slices - 1) / slices;
+    const int each = (groups + (1 << slices_log) - 1) >> slices_log;
     from = min(slice * each, groups);
     to = min(from + each, groups);
     body = head + groups * kPer;
-    first = slice == 0 ? (int)head : 0;
-    edge = first + (slice == slices - 1 ? (int)(v - body) : 0);
+    first = slice == 0 ? head : 0;
+    edge = first + (slice + 1 == 1 << slices_log ? v - body : 0);
   }
-  __device__ __forceinline__ int64_t edge_at(int i) const { return i < first ? i : body + (i - first); }
-  __device__ __forceinline__ bool owns(int64_t j, bool first_slice, bool last_slice) const {
+  __device__ __forceinline__ int edge_at(int i) const { return i < first ? i : body + (i - first); }
+  __device__ __forceinline__ bool owns(int j, bool first_slice, bool last_slice) const {
     if (j < head) return first_slice;
     if (j >= body) return last_slice;
-    const int64_t g = (j - head) / kPer;
+    const int g = (j - head) / kPer;
     return g >= from && g < to;
   }
 };
@@ -234,16 +233,34 @@ __device__ __forceinline__ float weigh(const Entries& e, int k, float c, float b
   return isnan(sum) ? sum : some ? 1.f : 0.f;
 }
 
+// A thread's first entry is asked for before the logits are swept (`begin`), and its logit is looked up behind them, when
+// the caches hold it (`end`): neither keeps the sweep waiting.
 template <typename T>
-__device__ __forceinline__ void load_entries(const DistillArgs& a, const Entries& e, int64_t row, const T* z, int64_t label) {
-  for (int i = threadIdx.x; i <= a.k; i += kDistillThreads) {
-    const int64_t j = i < a.k ? a.ids[row * a.k + i] : label;
-    const bool in = (uint64_t)j < (uint64_t)a.v;
-    e.at[i] = in ? (int)j : -1;
-    e.p[i] = i < a.k ? load_teacher(a, row * a.k + i) : 0.f;
-    e.z[i] = in ? Elem<T>::to_f32(z[j]) : 0.f;
+struct Fetch {
+  int64_t at = -1;
+  float t = 0.f;
+  __device__ __forceinline__ void begin(const DistillArgs& a, int64_t row, int64_t label) {
+    const int i = threadIdx.x;
+    if (i < a.k) {
+      at = a.ids[row * a.k + i];
+      t = load_teacher(a, row * a.k + i);
+    } else if (i == a.k) {
+      at = label;
+    }
   }
-}
+  __device__ __forceinline__ void end(const DistillArgs& a, const Entries& e, int64_t row, const T* z, int64_t label) {
+    for (int i = threadIdx.x; i <= a.k; i += kDistillThreads) {
+      if (i != (int)threadIdx.x) {
+        at = i < a.k ? a.ids[row * a.k + i] : label;
+        t = i < a.k ? load_teacher(a, row * a.k + i) : 0.f;
+      }
+      const bool in = (uint64_t)at < (uint64_t)a.v;
+      e.at[i] = in ? (int)at : -1;
+      e.p[i] = t;
+      e.z[i] = in ? Elem<T>::to_f32(z[at]) : 0.f;
+    }
+  }
+};
 
 // What a gradient is made of: dz = soft * 2^((z - base) c) + hard * 2^((z - base) log2e), at the entries minus
 // teach * (sum of p), and minus hit at the label.
@@ -305,14 +322,12 @@ __device__ __forceinline__ void write_groups(const Slice<T>& s, const T* z, T* o
   const char* from = reinterpret_cast<const char*>(z + s.head);
   uint4* to = reinterpret_cast<uint4*>(out + s.head);
   const uint32_t bits = (reinterpret_cast<uintptr_t>(from) & 3) * 8;
-  for (int64_t i0 = s.from + threadIdx.x; i0 < s.to; i0 += kDistillThreads * kDistillUnroll) {
-    uint4 raw[kDistillUnroll];
+  auto groups = [&](int i0, auto count) {
+    uint4 raw[count.value];
 #pragma unroll
-    for (int u = 0; u < kDistillUnroll; ++u)
-      if (i0 + u * kDistillThreads < s.to) raw[u] = load_shifted<Q>(from + (i0 + u * kDistillThreads) * 16, bits);
+    for (int u = 0; u < count.value; ++u) raw[u] = load_shifted<Q>(from + (int64_t)(i0 + u * kDistillThreads) * 16, bits);
 #pragma unroll
-    for (int u = 0; u < kDistillUnroll; ++u) {
-      if (i0 + u * kDistillThreads >= s.to) break;
+    for (int u = 0; u < count.value; ++u) {
       uint4 r;
       if constexpr (sizeof(T) == 4) {
         const Two a = co.at<S>(Raw<T>::pair(raw[u], 0)), b = co.at<S>(Raw<T>::pair(raw[u], 1));
@@ -323,7 +338,11 @@ __device__ __forceinline__ void write_groups(const Slice<T>& s, const T* z, T* o
       }
       to[i0 + u * kDistillThreads] = r;
     }
-  }
+  };
+  int i = s.from + threadIdx.x;
+  for (; i + (kDistillUnroll - 1) * kDistillThreads < s.to; i += kDistillUnroll * kDistillThreads)
+    groups(i, std::integral_constant<int, kDistillUnroll>{});
+  for (; i < s.to; i += kDistillThreads) groups(i, std::integral_constant<int, 1>{});
 }
 
 // z and out lie at the same distance from a 16-byte boundary: nothing is shifted.
@@ -345,7 +364,7 @@ __device__ __forceinline__ void write_slice(const Slice<T>& s, const T* z, T* ou
     }
   }
   if ((int)threadIdx.x < s.edge) {
-    const int64_t j = s.edge_at(threadIdx.x);
+    const int j = s.edge_at(threadIdx.x);
     out[j] = Elem<T>::from_f32(co.at<S>(Elem<T>::to_f32(z[j])));
   }
 }
@@ -356,7 +375,7 @@ __device__ __forceinline__ void write_entries(const DistillArgs& a, const Entrie
                                               int slice) {
   for (int i = threadIdx.x; i <= a.k; i += kDistillThreads) {
     const int j = e.at[i];
-    if (j < 0 || !s.owns(j, slice == 0, slice == a.slices - 1)) continue;
+    if (j < 0 || !s.owns(j, slice == 0, slice + 1 == 1 << a.slices_log)) continue;
     bool again = false;
     float p = e.p[i];
     for (int q = 0; q <= a.k; ++q) {
@@ -374,14 +393,14 @@ __device__ __forceinline__ void write_entries(const DistillArgs& a, const Entrie
 template <typename T>
 __device__ __forceinline__ void zero_slice(const Slice<T>& s, T* out) {
   uint4* to = reinterpret_cast<uint4*>(out + s.head);
-  for (int64_t i = s.from + threadIdx.x; i < s.to; i += kDistillThreads) to[i] = make_uint4(0, 0, 0, 0);
+  for (int i = s.from + threadIdx.x; i < s.to; i += kDistillThreads) to[i] = make_uint4(0, 0, 0, 0);
   if ((int)threadIdx.x < s.edge) out[s.edge_at(threadIdx.x)] = Elem<T>::from_f32(0.f);
 }
 
 // Loss, and with GRAD the gradient, of a row by a cluster of `slices` blocks: one pass with a running maximum and its
 // sums, joined over threads, warps and blocks; the gradient reads the row again, which the L2 still holds.
 template <typename T, Second S, bool GRAD>
-__global__ void __launch_bounds__(kDistillThreads, 4) distill_kernel(DistillArgs a) {
+__global__ void __launch_bounds__(kDistillThreads, kDistillBlocks) distill_kernel(DistillArgs a) {
   constexpr int per = Slice<T>::kPer;
   extern __shared__ char smem[];
   __shared__ Running warps[kDistillWarps];
@@ -390,9 +409,9 @@ __global__ void __launch_bounds__(kDistillThreads, 4) distill_kernel(DistillArgs
   const Entries e(smem, a.k);
   grid_dependency_trigger();
   grid_dependency_wait();
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int64_t row = blockIdx.x / a.slices;
-  const int slice = blockIdx.x % a.slices;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, slices = 1 << a.slices_log;
+  const int64_t row = blockIdx.x >> a.slices_log;
+  const int slice = blockIdx.x & (slices - 1);
   const T* z = static_cast<const T*>(a.pred) + row * a.ld;
   T* out = GRAD ? static_cast<T*>(a.out) + row * a.ld_out : nullptr;
   const bool labels = a.labels.p != nullptr;
@@ -402,82 +421,96 @@ __global__ void __launch_bounds__(kDistillThreads, 4) distill_kernel(DistillArgs
       a.loss[row] = 0.f;
       if (a.stats) a.stats[row] = make_float4(0.f, 1.f, 1.f, -1.f);
     }
-    if (GRAD) zero_slice(Slice<T>(out, a.v, slice, a.slices, false), out);
+    if (GRAD) zero_slice(Slice<T>(out, (int)a.v, slice, a.slices_log, false), out);
     return;
   }
-  load_entries(a, e, row, z, label);
+  Fetch<T> fetch;
+  fetch.begin(a, row, label);
 
   Running run{-INFINITY, 0.f, 0.f};
-  const Slice<T> s(z, a.v, slice, a.slices, false);
-  const uint4* middle = reinterpret_cast<const uint4*>(z + s.head);
-  const uint32_t low = sizeof(T) == 4 ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;  // -infinity
-  Two soft(0.f, 0.f), hard(0.f, 0.f);
-  for (int64_t i0 = s.from + tid; i0 < s.to; i0 += kDistillThreads * kDistillUnroll) {
-    uint4 raw[kDistillUnroll];
-    uint32_t most = low;
+  const Slice<T> s(z, (int)a.v, slice, a.slices_log, false);
+  {
+    const uint4* middle = reinterpret_cast<const uint4*>(z + s.head);
+    Two soft(0.f, 0.f), hard(0.f, 0.f);
+    auto groups = [&](int i0, auto count) {
+      uint4 raw[count.value];
 #pragma unroll
-    for (int u = 0; u < kDistillUnroll; ++u) {
-      const int64_t i = i0 + u * kDistillThreads;
-      raw[u] = i < s.to ? middle[i] : make_uint4(low, low, low, low);
-    }
+      for (int u = 0; u < count.value; ++u) raw[u] = middle[i0 + u * kDistillThreads];
+      uint32_t most = Raw<T>::max2(raw[0]);
 #pragma unroll
-    for (int u = 0; u < kDistillUnroll; ++u) most = Raw<T>::max2(most, Raw<T>::max2(raw[u]));
-    const float top = fmaxf(run.top, Raw<T>::max1(most)), base = base_of(top), from = base_of(run.top) - base;
-    const float fs = run.top == -INFINITY ? 1.f : ex2(from * a.c), fh = run.top == -INFINITY ? 1.f : ex2(from * kLog2e);
-    run.top = top;
-    soft = soft * Two(fs, fs);
-    if (S != kNone) hard = hard * Two(fh, fh);
-    const Two nb(-base, -base), c2(a.c, a.c);
-#pragma unroll
-    for (int u = 0; u < kDistillUnroll; ++u) {
-      if (i0 + u * kDistillThreads >= s.to) break;
-#pragma unroll
-      for (int j = 0; j < per / 2; ++j) {
-        const Two x = Raw<T>::pair(raw[u], j) + nb, p = ex2(x * c2);
-        soft = soft + p;
-        if (S == kOwn) hard = hard + ex2(x * Two(kLog2e, kLog2e));
-        if (S == kSquare) hard = fma2(p, p, hard);
-        if (S == kFourth) hard = fma2(p * p, p * p, hard);
+      for (int u = 1; u < count.value; ++u) most = Raw<T>::max2(most, Raw<T>::max2(raw[u]));
+      const float top = fmaxf(run.top, Raw<T>::max1(most)), base = base_of(top);
+      if (top != run.top) {
+        const float d = run.top - top;  // -infinity at first: the sums are 0 and stay it, or NaN
+        const float fs = run.top == -INFINITY ? 1.f : ex2(d * a.c), fh = run.top == -INFINITY ? 1.f : ex2(d * kLog2e);
+        soft = soft * Two(fs, fs);
+        if (S != kNone) hard = hard * Two(fh, fh);
+        run.top = top;
       }
-    }
+      const Two nb(-base, -base), c2(a.c, a.c);
+#pragma unroll
+      for (int u = 0; u < count.value; ++u) {
+#pragma unroll
+        for (int j = 0; j < per / 2; ++j) {
+          const Two x = Raw<T>::pair(raw[u], j) + nb, p = ex2(x * c2);
+          soft = soft + p;
+          if (S == kOwn) hard = hard + ex2(x * Two(kLog2e, kLog2e));
+          if (S == kSquare) hard = fma2(p, p, hard);
+          if (S == kFourth) hard = fma2(p * p, p * p, hard);
+        }
+      }
+    };
+    int i = s.from + tid;
+    for (; i + (kDistillUnroll - 1) * kDistillThreads < s.to; i += kDistillUnroll * kDistillThreads)
+      groups(i, std::integral_constant<int, kDistillUnroll>{});
+    for (; i < s.to; i += kDistillThreads) groups(i, std::integral_constant<int, 1>{});
+    run.soft = soft.lo() + soft.hi();
+    run.hard = hard.lo() + hard.hi();
   }
-  run.soft = soft.lo() + soft.hi();
-  run.hard = hard.lo() + hard.hi();
   if (tid < s.edge) {
-    const float edge = Elem<T>::to_f32(z[s.edge_at(tid)]), base = base_of(edge);
-    run = merge<S>(run, Running{edge, power(edge, base, a.c), S != kNone ? power(edge, base, kLog2e) : 0.f}, a.c);
+    const float edge = Elem<T>::to_f32(z[s.edge_at(tid)]);
+    rebase<S>(run, fmaxf(run.top, edge), a.c);
+    const float base = base_of(run.top);
+    run.soft += power(edge, base, a.c);
+    if (S != kNone) run.hard += power(edge, base, kLog2e);
   }
+  fetch.end(a, e, row, z, label);
+  // the block's maximum first, then sums relative to it
+  float top = run.top;
 #pragma unroll
-  for (int d = 16; d; d >>= 1) {
-    const Running other{__shfl_xor_sync(0xffffffffu, run.top, d), __shfl_xor_sync(0xffffffffu, run.soft, d),
-                        S != kNone ? __shfl_xor_sync(0xffffffffu, run.hard, d) : 0.f};
-    // the lower lane's sums first, on both sides
-    run = lane & d ? merge<S>(other, run, a.c) : merge<S>(run, other, a.c);
-  }
-  if (lane == 0) warps[warp] = run;
+  for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+  if (lane == 0) warps[warp].top = top;
   __syncthreads();
-  if (tid == 0) {
-    run = warps[0];
-    for (int w = 1; w < kDistillWarps; ++w) run = merge<S>(run, warps[w], a.c);
-    whole = run;
+#pragma unroll
+  for (int w = 0; w < kDistillWarps; ++w) top = fmaxf(top, warps[w].top);
+  rebase<S>(run, top, a.c);
+  run.soft = warp_sum(run.soft);
+  if (S != kNone) run.hard = warp_sum(run.hard);
+  if (lane == 0) {
+    warps[warp].soft = run.soft;
+    warps[warp].hard = run.hard;
   }
-  if (a.slices > 1) {
-    cluster_sync();
-    if (tid < 32) {
-      run = Running{-INFINITY, 0.f, 0.f};
-      for (int r = 0; r < a.slices; ++r) {
-        Running other;
-        other.top = __uint_as_float(cluster_load(&whole.top, r));
-        other.soft = __uint_as_float(cluster_load(&whole.soft, r));
-        other.hard = __uint_as_float(cluster_load(&whole.hard, r));
-        run = merge<S>(run, other, a.c);
-      }
-    }
-    cluster_sync();  // read by all before one of them overwrites it or ends
+  __syncthreads();
+  run = Running{top, 0.f, 0.f};
+#pragma unroll
+  for (int w = 0; w < kDistillWarps; ++w) {
+    run.soft += warps[w].soft;
+    run.hard += warps[w].hard;
+  }
+  if (a.slices_log) {
     if (tid == 0) whole = run;
+    cluster_sync();
+    for (int r = 0; r < slices; ++r) top = fmaxf(top, __uint_as_float(cluster_load(&whole.top, r)));
+    run = Running{top, 0.f, 0.f};
+    for (int r = 0; r < slices; ++r) {
+      Running other{__uint_as_float(cluster_load(&whole.top, r)), __uint_as_float(cluster_load(&whole.soft, r)),
+                    __uint_as_float(cluster_load(&whole.hard, r))};
+      rebase<S>(other, top, a.c);
+      run.soft += other.soft;
+      run.hard += other.hard;
+    }
+    cluster_sync();  // read by all before one of them overwrites its logits or ends
   }
-  __syncthreads();
-  run = whole;
   const float base = base_of(run.top);
   float4 stats = make_float4(run.top, run.soft, S != kNone ? run.hard : run.soft, 0.f);
   if (warp == 0) {
@@ -495,7 +528,7 @@ __global__ void __launch_bounds__(kDistillThreads, 4) distill_kernel(DistillArgs
   __syncthreads();
   stats.w = some_s;
   const Coefficients co = coefficients<S>(a, row, stats, labels);
-  const Slice<T> so(out, a.v, slice, a.slices, !alike(z, out));
+  const Slice<T> so(out, (int)a.v, slice, a.slices_log, !alike(z, out));
   write_slice<T, S>(so, z, out, co);
   __syncthreads();
   write_entries<T, S>(a, e, so, out, co, slice);
@@ -503,28 +536,33 @@ __global__ void __launch_bounds__(kDistillThreads, 4) distill_kernel(DistillArgs
 
 // The gradient from the statistics that the forward pass has left.
 template <typename T, Second S>
-__global__ void __launch_bounds__(kDistillThreads, 4) distill_dpred_kernel(DistillArgs a) {
+__global__ void __launch_bounds__(kDistillThreads, kDistillBlocks) distill_dpred_kernel(DistillArgs a) {
   extern __shared__ char smem[];
   const Entries e(smem, a.k);
   grid_dependency_trigger();
   grid_dependency_wait();
-  const int64_t row = blockIdx.x / a.slices;
-  const int slice = blockIdx.x % a.slices;
+  const int64_t row = blockIdx.x >> a.slices_log;
+  const int slice = blockIdx.x & ((1 << a.slices_log) - 1);
   const T* z = static_cast<const T*>(a.pred) + row * a.ld;
   T* out = static_cast<T*>(a.out) + row * a.ld_out;
-  const Slice<T> s(out, a.v, slice, a.slices, !alike(z, out));
   const bool labels = a.labels.p != nullptr;
   const int64_t label = labels ? a.labels[row] : -1;
   if (labels && (label == a.ignore || (uint64_t)label >= (uint64_t)a.v)) {
-    zero_slice(Slice<T>(out, a.v, slice, a.slices, false), out);
+    zero_slice(Slice<T>(out, (int)a.v, slice, a.slices_log, false), out);
     return;
   }
   const float4 stats = a.stats[row];
-  // in place: this block's entries before any of it is overwritten (another block's are not used here)
-  load_entries(a, e, row, z, label);
-  if (a.out == a.pred) __syncthreads();
+  Fetch<T> fetch;
+  fetch.begin(a, row, label);
+  const bool in_place = a.out == a.pred;
+  if (in_place) {  // this block's entries before any of it is overwritten (another block's are not used here)
+    fetch.end(a, e, row, z, label);
+    __syncthreads();
+  }
+  const Slice<T> s(out, (int)a.v, slice, a.slices_log, !alike(z, out));
   const Coefficients co = coefficients<S>(a, row, stats, labels);
   write_slice<T, S>(s, z, out, co);
+  if (!in_place) fetch.end(a, e, row, z, label);
   __syncthreads();
   if (threadIdx.x < 32) weigh(e, a.k, a.c, 0.f, 0.f, nullptr);
   __syncthreads();
@@ -562,7 +600,6 @@ static DistillArgs device_args(const rafb200_distill* d) {
   a.soft_loss = (float)(d->alpha * d->temperature * d->temperature);
   a.soft_grad = (float)(d->alpha * d->temperature);
   a.hard = (float)(1.0 - d->alpha);
-  a.slices = 1;
   return a;
 }
 
@@ -571,11 +608,12 @@ static Second second_of(const rafb200_distill* d) {
   return d->temperature == 2.0 ? kSquare : d->temperature == 4.0 ? kFourth : kOwn;
 }
 
-static int row_slices(const rafb200_distill* d) {
-  int slices = 1;
+// Blocks of a row, as a power of two: few rows are cut until every SM has work, while a thread keeps a group.
+static int row_slices_log(const rafb200_distill* d) {
+  int log = 0;
   const int64_t groups = d->v * dtype_size(d->pred_dtype) / 16;
-  while (slices < 8 && d->n * slices * 2 <= 148 * 2 && groups / (slices * 2) >= kDistillThreads) slices *= 2;
-  return slices;
+  while (log < 3 && (d->n << (log + 1)) <= 148 * 2 && groups >> (log + 1) >= kDistillThreads) ++log;
+  return log;
 }
 
 template <typename F>
@@ -603,9 +641,9 @@ int rafb200_distill_loss(const rafb200_distill* d, float* loss, float* stats, vo
   DistillArgs a = device_args(d);
   a.loss = loss;
   a.stats = reinterpret_cast<float4*>(stats);
-  a.slices = row_slices(d);
+  a.slices_log = row_slices_log(d);
   return with_case(d, [&](auto t, auto second) {
-    RAFB200_CUDA(launch_cluster(distill_kernel<decltype(t), decltype(second)::value, false>, a.slices, (unsigned)(d->n * a.slices),
+    RAFB200_CUDA(launch_cluster(distill_kernel<decltype(t), decltype(second)::value, false>, 1u << a.slices_log, (unsigned)(d->n << a.slices_log),
                                 kDistillThreads, Entries::bytes(d->k), static_cast<cudaStream_t>(stream), a));
     return (int)RAFB200_OK;
   });
@@ -633,9 +671,9 @@ int rafb200_distill_loss_dpred(const rafb200_distill* d, const float* dy, int dy
   a.stats = reinterpret_cast<float4*>(const_cast<float*>(stats));
   a.out = dpred;
   a.ld_out = ld_dpred;
-  a.slices = row_slices(d);
+  a.slices_log = row_slices_log(d);
   return with_case(d, [&](auto t, auto second) {
-    RAFB200_CUDA(launch_dependent(distill_dpred_kernel<decltype(t), decltype(second)::value>, dim3((unsigned)(d->n * a.slices)),
+    RAFB200_CUDA(launch_dependent(distill_dpred_kernel<decltype(t), decltype(second)::value>, dim3((unsigned)(d->n << a.slices_log)),
                                   kDistillThreads, Entries::bytes(d->k), static_cast<cudaStream_t>(stream), a));
     return (int)RAFB200_OK;
   });
@@ -654,9 +692,9 @@ int rafb200_distill_loss_with_dpred(const rafb200_distill* d, const float* dy, i
   a.loss = loss;
   a.out = dpred;
   a.ld_out = ld_dpred;
-  a.slices = row_slices(d);
+  a.slices_log = row_slices_log(d);
   return with_case(d, [&](auto t, auto second) {
-    RAFB200_CUDA(launch_cluster(distill_kernel<decltype(t), decltype(second)::value, true>, a.slices, (unsigned)(d->n * a.slices),
+    RAFB200_CUDA(launch_cluster(distill_kernel<decltype(t), decltype(second)::value, true>, 1u << a.slices_log, (unsigned)(d->n << a.slices_log),
                                 kDistillThreads, Entries::bytes(d->k), static_cast<cudaStream_t>(stream), a));
     return (int)RAFB200_OK;
   });
