@@ -11,6 +11,7 @@
 // Exponentials are those of base 2 of (z - m) c with m the row's maximum and c = log2(e) / T: the difference first, so that
 // neither the product overflows at a type's lowest values (masks) nor logits far from zero lose digits.  Sums are fp32,
 // in a fixed order.
+#include <algorithm>
 #include <cmath>
 
 #include "model_io.cuh"
@@ -21,10 +22,9 @@ namespace rafb200 {
 // issue slots per 32 elements of 2 bytes read and written, and an exponential fills the special-function unit for 8 of
 // them.  So two elements are computed by one instruction (f32x2), maxima are taken on the raw pairs, and where the second
 // exponential is a small power of the first (T = 2 or 4) it is multiplied out.
-constexpr int kDistillThreads = 128;
-constexpr int kDistillWarps = kDistillThreads / 32;
-constexpr int kDistillUnroll = 4;
-constexpr int kDistillBlocks = 8;  // resident blocks of an SM: 64 registers a thread
+constexpr int kDistillUnroll = 4;  // the rests of one to three groups are written out
+constexpr int kDistillRing = 3 * kDistillUnroll;  // groups of a thread on their way in
+constexpr int kSweepThreads = 1024;  // of an SM, at least
 constexpr int kMaxTeacher = 1024;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
@@ -163,104 +163,104 @@ __device__ __forceinline__ void rebase(Running& x, float top, float c) {
   x.top = top;
 }
 
-// A block's part of a row: groups [from, to) of 16 bytes of the part that is aligned at `p`; the elements in front of
-// that part are the first block's, those behind it the last one's.  With `trim` the first and the last group
-// count to those.
+// A block's part of a row: elements [begin, end), of which `groups` groups of 16 bytes from element `at` on are aligned
+// in memory.  The row's first and last elements, which no aligned group holds, are the first and the last block's.
 template <typename T>
 struct Slice {
   static constexpr int kPer = Raw<T>::kPer;
-  int head, from, to, body;  // elements in front; groups; first element behind
-  int edge;                  // elements of this block outside the groups: thread i < edge takes edge_at(i)
-  int first;                 // of them in front
+  int begin, end, at, groups;
 
-  __device__ __forceinline__ Slice(const T* p, int v, int slice, int slices_log, bool trim) {
-    head = min((int)((-(intptr_t)p & 15) / sizeof(T)), v);
-    int groups = (v - head) / kPer;
-    if (trim && groups > 0) {
-      head += kPer;
-      groups = max(groups - 2, 0);
-    }
-    const int each = (groups + (1 << slices_log) - 1) >> slices_log;
-    from = min(slice * each, groups);
-    to = min(from + each, groups);
-    body = head + groups * kPer;
-    first = slice == 0 ? head : 0;
-    edge = first + (slice + 1 == 1 << slices_log ? v - body : 0);
+  __device__ __forceinline__ Slice() {}
+  __device__ __forceinline__ Slice(const T* p, int v, int slice, int slices_log) {
+    const int head = min((int)((-(intptr_t)p & 15) / sizeof(T)), v), all = (v - head) / kPer;
+    const int each = (all + (1 << slices_log) - 1) >> slices_log, from = min(slice * each, all);
+    groups = min(each, all - from);
+    at = head + from * kPer;
+    begin = slice ? at : 0;
+    end = slice + 1 == 1 << slices_log ? v : at + groups * kPer;
   }
-  __device__ __forceinline__ int edge_at(int i) const { return i < first ? i : body + (i - first); }
-  __device__ __forceinline__ bool owns(int j, bool first_slice, bool last_slice) const {
-    if (j < head) return first_slice;
-    if (j >= body) return last_slice;
-    const int g = (j - head) / kPer;
-    return g >= from && g < to;
+  // The same elements, in groups that are aligned at `p` and whose bytes this slice's groups hold.
+  __device__ __forceinline__ Slice aligned_at(const T* p) const {
+    Slice s;
+    s.begin = begin;
+    s.end = end;
+    s.at = at + (int)((-(intptr_t)(p + at) & 15) / sizeof(T));
+    s.groups = max(at + groups * kPer - s.at, 0) / kPer;
+    if (s.groups == 0) s.at = at;
+    return s;
   }
+  // Elements outside the groups: thread i < edges() takes edge_at(i).
+  __device__ __forceinline__ int edges() const { return end - begin - groups * kPer; }
+  __device__ __forceinline__ int edge_at(int i) const { return begin + i < at ? begin + i : begin + i + groups * kPer; }
+  __device__ __forceinline__ bool owns(int j) const { return j >= begin && j < end; }
 };
 
-// The teacher's entries of a row in shared memory: class (-1: absent), weight p, student's logit there.
-// Entry k is the label, with weight 0.
+// Copies 16 bytes to shared memory without waiting; a thread waits for all but its last N batches of copies.
+__device__ __forceinline__ void copy_async(void* to, const void* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// The teacher's entries of a row in shared memory: class (-1: absent), weight p, its logarithm of base 2, student's logit
+// there.  Entry k is the label, with weight 0.
 struct Entries {
   int* at;
   float* p;
+  float* log_p;
   float* z;
   __device__ __forceinline__ Entries(void* smem, int k)
-      : at(static_cast<int*>(smem)), p(reinterpret_cast<float*>(at + k + 1)), z(p + k + 1) {}
-  static size_t bytes(int k) { return (size_t)(k + 1) * 12; }
+      : at(static_cast<int*>(smem)), p(reinterpret_cast<float*>(at + k + 1)), log_p(p + k + 1), z(log_p + k + 1) {}
+  static __host__ __device__ __forceinline__ size_t bytes(int k) { return (size_t)(k + 1) * 16; }
 };
 
-// softmax over the present entries; the sum of the weights (1 or 0), and with `kl` sum p (log p - log q).  One warp.
-__device__ __forceinline__ float weigh(const Entries& e, int k, float c, float base, float log2_soft, float* kl) {
+// softmax over the present entries, whose logits p holds before; returns the sum of the weights, 1 or 0 (or NaN).  One warp.
+__device__ __forceinline__ float weigh(const Entries& e, int k, float c) {
   const int lane = threadIdx.x & 31;
   float top = -INFINITY;
   for (int i = lane; i < k; i += 32)
     if (e.at[i] >= 0) top = fmaxf(top, e.p[i]);
 #pragma unroll
   for (int s = 16; s; s >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
-  const float t_base = base_of(top);
+  const float base = base_of(top);
   float sum = 0.f;
   for (int i = lane; i < k; i += 32)
-    if (e.at[i] >= 0) sum += power(e.p[i], t_base, c);
+    if (e.at[i] >= 0) sum += power(e.p[i], base, c);
   sum = warp_sum(sum);
   const bool some = sum != 0.f;  // false: no teacher, or all of it at -infinity
   const float inv = some ? 1.f / sum : 0.f, log2_sum = log2f(sum);
-  float part = 0.f;
   for (int i = lane; i < k; i += 32) {
-    const float t = (e.p[i] - t_base) * c;
-    const float w = e.at[i] >= 0 && some ? ex2(t) * inv : 0.f;
-    if (kl && !(w == 0.f)) part = fmaf(w, (t - log2_sum) - ((e.z[i] - base) * c - log2_soft), part);  // log2 p - log2 q
-    e.p[i] = w;
+    const float t = (e.p[i] - base) * c;
+    e.log_p[i] = t - log2_sum;
+    e.p[i] = e.at[i] >= 0 && some ? ex2(t) * inv : 0.f;
   }
-  if (kl) *kl = warp_sum(part) * kLn2;
+  __syncwarp();
   return isnan(sum) ? sum : some ? 1.f : 0.f;
 }
 
-// A thread's first entry is asked for before the logits are swept (`begin`), and its logit is looked up behind them, when
-// the caches hold it (`end`): neither keeps the sweep waiting.
+// sum p (log p - log q).  One warp.
+__device__ __forceinline__ float divergence(const Entries& e, int k, float c, float base, float log2_soft) {
+  float part = 0.f;
+  for (int i = threadIdx.x & 31; i < k; i += 32)
+    if (!(e.p[i] == 0.f)) part = fmaf(e.p[i], e.log_p[i] - ((e.z[i] - base) * c - log2_soft), part);
+  return warp_sum(part) * kLn2;
+}
+
+// Fills in the entries of a row.  One warp.
 template <typename T>
-struct Fetch {
-  int64_t at = -1;
-  float t = 0.f;
-  __device__ __forceinline__ void begin(const DistillArgs& a, int64_t row, int64_t label) {
-    const int i = threadIdx.x;
-    if (i < a.k) {
-      at = a.ids[row * a.k + i];
-      t = load_teacher(a, row * a.k + i);
-    } else if (i == a.k) {
-      at = label;
-    }
+__device__ __forceinline__ void load_entries(const DistillArgs& a, const Entries& e, int64_t row, const T* z, int64_t label) {
+  for (int i = threadIdx.x & 31; i <= a.k; i += 32) {
+    const int64_t j = i < a.k ? a.ids[row * a.k + i] : label;
+    const bool in = (uint64_t)j < (uint64_t)a.v;
+    e.at[i] = in ? (int)j : -1;
+    e.p[i] = i < a.k ? load_teacher(a, row * a.k + i) : 0.f;
+    e.z[i] = in ? Elem<T>::to_f32(z[j]) : 0.f;
   }
-  __device__ __forceinline__ void end(const DistillArgs& a, const Entries& e, int64_t row, const T* z, int64_t label) {
-    for (int i = threadIdx.x; i <= a.k; i += kDistillThreads) {
-      if (i != (int)threadIdx.x) {
-        at = i < a.k ? a.ids[row * a.k + i] : label;
-        t = i < a.k ? load_teacher(a, row * a.k + i) : 0.f;
-      }
-      const bool in = (uint64_t)at < (uint64_t)a.v;
-      e.at[i] = in ? (int)at : -1;
-      e.p[i] = t;
-      e.z[i] = in ? Elem<T>::to_f32(z[at]) : 0.f;
-    }
-  }
-};
+  __syncwarp();
+}
 
 // What a gradient is made of: dz = soft * 2^((z - base) c) + hard * 2^((z - base) log2e), at the entries minus
 // teach * (sum of p), and minus hit at the label.
@@ -285,8 +285,8 @@ struct Coefficients {
 };
 
 template <Second S>
-__device__ __forceinline__ Coefficients coefficients(const DistillArgs& a, int64_t row, float4 stats, bool labels) {
-  const float w = (a.dy ? a.dy[row * a.dy_step] : 1.f) * a.grad_scale;
+__device__ __forceinline__ Coefficients coefficients(const DistillArgs& a, float weight, float4 stats, bool labels) {
+  const float w = weight * a.grad_scale;
   Coefficients co;
   co.c = a.c;
   co.base = base_of(stats.x);
@@ -301,7 +301,7 @@ __device__ __forceinline__ Coefficients coefficients(const DistillArgs& a, int64
   return co;
 }
 
-// 16 bytes from an address that is 4 Q + r bytes (r = bits / 8, 0 or 2) behind a 16-byte boundary.
+// 16 bytes from an address that is 4 Q + r bytes (r = bits / 8, 0 or 2) behind a 16-byte boundary; Q < 0: at one.
 template <int Q>
 __device__ __forceinline__ uint4 load_shifted(const char* p, uint32_t bits) {
   if constexpr (Q < 0) {
@@ -315,34 +315,66 @@ __device__ __forceinline__ uint4 load_shifted(const char* p, uint32_t bits) {
   }
 }
 
-// The gradient of the groups of a slice, which is aligned at `out`.
-template <typename T, Second S, int Q>
-__device__ __forceinline__ void write_groups(const Slice<T>& s, const T* z, T* out, const Coefficients& co) {
-  constexpr int per = Slice<T>::kPer;
-  const char* from = reinterpret_cast<const char*>(z + s.head);
-  uint4* to = reinterpret_cast<uint4*>(out + s.head);
-  const uint32_t bits = (reinterpret_cast<uintptr_t>(from) & 3) * 8;
-  auto groups = [&](int i0, auto count) {
-    uint4 raw[count.value];
+// The groups of a slice on their way through shared memory, kDistillRing places a thread that go round: each is read by the
+// thread alone that asked for it, so no registers are bound by what is on its way, and no barrier is needed.
+template <typename T, int NT>
+struct Stream {
+  static constexpr int kAhead = kDistillRing / kDistillUnroll, kStep = kDistillUnroll * NT, kPlaces = kDistillRing * NT;
+  const uint4* source;
+  uint4 *first, *place;
+  int groups;
+  __device__ __forceinline__ Stream(const Slice<T>& s, const T* z, uint4* image)
+      : source(reinterpret_cast<const uint4*>(z + s.at)), first(image + threadIdx.x), place(first), groups(s.groups) {}
+  __device__ __forceinline__ void ask(int i, uint4* to) {  // a batch, this thread's groups from i on
 #pragma unroll
-    for (int u = 0; u < count.value; ++u) raw[u] = load_shifted<Q>(from + (int64_t)(i0 + u * kDistillThreads) * 16, bits);
+    for (int u = 0; u < kDistillUnroll; ++u)
+      if (i + u * NT < groups) copy_async(to + u * NT, source + i + u * NT);
+    copy_commit();
+  }
+  __device__ __forceinline__ void begin() {
 #pragma unroll
-    for (int u = 0; u < count.value; ++u) {
-      uint4 r;
-      if constexpr (sizeof(T) == 4) {
-        const Two a = co.at<S>(Raw<T>::pair(raw[u], 0)), b = co.at<S>(Raw<T>::pair(raw[u], 1));
-        r = make_uint4(__float_as_uint(a.lo()), __float_as_uint(a.hi()), __float_as_uint(b.lo()), __float_as_uint(b.hi()));
-      } else {
-        r = make_uint4(Raw<T>::put(co.at<S>(Raw<T>::pair(raw[u], 0))), Raw<T>::put(co.at<S>(Raw<T>::pair(raw[u], 1))),
-                       Raw<T>::put(co.at<S>(Raw<T>::pair(raw[u], 2))), Raw<T>::put(co.at<S>(Raw<T>::pair(raw[u], 3))));
-      }
-      to[i0 + u * kDistillThreads] = r;
+    for (int b = 0; b < kAhead; ++b) ask(threadIdx.x + b * kStep, first + b * kStep);
+  }
+  // use(i, where group i lies, number of this thread's groups from i on) for every batch
+  template <typename Use>
+  __device__ __forceinline__ void run(const Use& use) {
+    for (int i = threadIdx.x; i < groups; i += kStep) {
+      copy_wait<kAhead - 1>();
+      use(i, place, (groups - i + NT - 1) / NT);
+      ask(i + kAhead * kStep, place);
+      place = place == first + (kAhead - 1) * kStep ? first : place + kStep;
     }
-  };
-  int i = s.from + threadIdx.x;
-  for (; i + (kDistillUnroll - 1) * kDistillThreads < s.to; i += kDistillUnroll * kDistillThreads)
-    groups(i, std::integral_constant<int, kDistillUnroll>{});
-  for (; i < s.to; i += kDistillThreads) groups(i, std::integral_constant<int, 1>{});
+    copy_wait<0>();
+    place = first;
+  }
+};
+
+// The gradient of COUNT groups, NT apart; `from` holds the bytes of the first.
+template <typename T, Second S, int NT, int Q, int COUNT>
+__device__ __forceinline__ void write_groups(const char* from, uint32_t bits, uint4* to, const Coefficients& co) {
+  uint4 raw[COUNT];
+#pragma unroll
+  for (int u = 0; u < COUNT; ++u) raw[u] = load_shifted<Q>(from + u * NT * 16, bits);
+#pragma unroll
+  for (int u = 0; u < COUNT; ++u) {
+    uint4 r;
+    if constexpr (sizeof(T) == 4) {
+      const Two a = co.at<S>(Raw<T>::pair(raw[u], 0)), b = co.at<S>(Raw<T>::pair(raw[u], 1));
+      r = make_uint4(__float_as_uint(a.lo()), __float_as_uint(a.hi()), __float_as_uint(b.lo()), __float_as_uint(b.hi()));
+    } else {
+      r = make_uint4(Raw<T>::put(co.at<S>(Raw<T>::pair(raw[u], 0))), Raw<T>::put(co.at<S>(Raw<T>::pair(raw[u], 1))),
+                     Raw<T>::put(co.at<S>(Raw<T>::pair(raw[u], 2))), Raw<T>::put(co.at<S>(Raw<T>::pair(raw[u], 3))));
+    }
+    to[u * NT] = r;
+  }
+}
+// A batch of them, `left` from the first on: the rest together, for one wait for memory.
+template <typename T, Second S, int NT, int Q>
+__device__ __forceinline__ void write_batch(const char* from, uint32_t bits, uint4* to, int left, const Coefficients& co) {
+  if (left >= kDistillUnroll) write_groups<T, S, NT, Q, kDistillUnroll>(from, bits, to, co);
+  else if (left == 1) write_groups<T, S, NT, Q, 1>(from, bits, to, co);
+  else if (left == 2) write_groups<T, S, NT, Q, 2>(from, bits, to, co);
+  else if (left == 3) write_groups<T, S, NT, Q, 3>(from, bits, to, co);
 }
 
 // z and out lie at the same distance from a 16-byte boundary: nothing is shifted.
@@ -351,35 +383,49 @@ __device__ __forceinline__ bool alike(const T* z, const T* out) {
   return ((reinterpret_cast<uintptr_t>(z) ^ reinterpret_cast<uintptr_t>(out)) & 15) == 0;
 }
 
-template <typename T, Second S>
-__device__ __forceinline__ void write_slice(const Slice<T>& s, const T* z, T* out, const Coefficients& co) {
-  if (alike(z, out)) {
-    write_groups<T, S, -1>(s, z, out, co);
-  } else {
-    switch ((reinterpret_cast<uintptr_t>(z + s.head) & 15) >> 2) {
-      case 0: write_groups<T, S, 0>(s, z, out, co); break;
-      case 1: write_groups<T, S, 1>(s, z, out, co); break;
-      case 2: write_groups<T, S, 2>(s, z, out, co); break;
-      default: write_groups<T, S, 3>(s, z, out, co); break;
-    }
+// The gradient of a slice of z.  `edge` is this thread's element outside the groups.
+template <typename T, Second S, int NT, int Q>
+__device__ __forceinline__ void write_batches(const Slice<T>& s, const T* z, T* out, const Coefficients& co) {
+  const char* from = reinterpret_cast<const char*>(z + s.at);
+  uint4* to = reinterpret_cast<uint4*>(out + s.at);
+  const uint32_t bits = (reinterpret_cast<uintptr_t>(from) & 3) * 8;
+  for (int i = threadIdx.x; i < s.groups; i += kDistillUnroll * NT)
+    write_batch<T, S, NT, Q>(from + (int64_t)i * 16, bits, to + i, (s.groups - i + NT - 1) / NT, co);
+}
+template <typename T, Second S, int NT>
+__device__ __forceinline__ void write_slice(const Slice<T>& in, const T* z, float edge, T* out, const Coefficients& co, Stream<T, NT>& stream) {
+  if (alike(z, out)) {  // the stream has begun
+    uint4* to = reinterpret_cast<uint4*>(out + in.at);
+    stream.run([&](int i, const uint4* place, int left) {
+      write_batch<T, S, NT, -1>(reinterpret_cast<const char*>(place), 0, to + i, left, co);
+    });
+    if ((int)threadIdx.x < in.edges()) out[in.edge_at(threadIdx.x)] = Elem<T>::from_f32(co.at<S>(edge));
+    return;
   }
-  if ((int)threadIdx.x < s.edge) {
+  const Slice<T> s = in.aligned_at(out);
+  switch ((reinterpret_cast<uintptr_t>(z + s.at) & 15) >> 2) {
+    case 0: write_batches<T, S, NT, 0>(s, z, out, co); break;
+    case 1: write_batches<T, S, NT, 1>(s, z, out, co); break;
+    case 2: write_batches<T, S, NT, 2>(s, z, out, co); break;
+    default: write_batches<T, S, NT, 3>(s, z, out, co); break;
+  }
+  if ((int)threadIdx.x < s.edges()) {
     const int j = s.edge_at(threadIdx.x);
     out[j] = Elem<T>::from_f32(co.at<S>(Elem<T>::to_f32(z[j])));
   }
 }
 
-// The elements that the teacher or the label names, once each however often they are named.
+// The elements that the teacher or the label names, once each however often they are named.  One warp.
 template <typename T, Second S>
-__device__ __forceinline__ void write_entries(const DistillArgs& a, const Entries& e, const Slice<T>& s, T* out, const Coefficients& co,
-                                              int slice) {
-  for (int i = threadIdx.x; i <= a.k; i += kDistillThreads) {
+__device__ __forceinline__ void write_entries(const DistillArgs& a, const Entries& e, const Slice<T>& s, T* out, const Coefficients& co) {
+  for (int i = threadIdx.x & 31; i <= a.k; i += 32) {
     const int j = e.at[i];
-    if (j < 0 || !s.owns(j, slice == 0, slice + 1 == 1 << a.slices_log)) continue;
+    if (j < 0 || !s.owns(j)) continue;
     bool again = false;
     float p = e.p[i];
+#pragma unroll 4
     for (int q = 0; q <= a.k; ++q) {
-      if (q == i || e.at[q] != j) continue;
+      if (e.at[q] != j || q == i) continue;
       again |= q < i;
       p += e.p[q];
     }
@@ -390,183 +436,251 @@ __device__ __forceinline__ void write_entries(const DistillArgs& a, const Entrie
   }
 }
 
-template <typename T>
+template <typename T, int NT>
 __device__ __forceinline__ void zero_slice(const Slice<T>& s, T* out) {
-  uint4* to = reinterpret_cast<uint4*>(out + s.head);
-  for (int i = s.from + threadIdx.x; i < s.to; i += kDistillThreads) to[i] = make_uint4(0, 0, 0, 0);
-  if ((int)threadIdx.x < s.edge) out[s.edge_at(threadIdx.x)] = Elem<T>::from_f32(0.f);
+  uint4* to = reinterpret_cast<uint4*>(out + s.at);
+  for (int i = threadIdx.x; i < s.groups; i += NT) to[i] = make_uint4(0, 0, 0, 0);
+  if ((int)threadIdx.x < s.edges()) out[s.edge_at(threadIdx.x)] = Elem<T>::from_f32(0.f);
 }
 
-// Loss, and with GRAD the gradient, of a row by a cluster of `slices` blocks: one pass with a running maximum and its
-// sums, joined over threads, warps and blocks; the gradient reads the row again, which the L2 still holds.
-template <typename T, Second S, bool GRAD>
-__global__ void __launch_bounds__(kDistillThreads, kDistillBlocks) distill_kernel(DistillArgs a) {
-  constexpr int per = Slice<T>::kPer;
-  extern __shared__ char smem[];
-  __shared__ Running warps[kDistillWarps];
-  __shared__ Running whole;
-  __shared__ float some_s;
-  const Entries e(smem, a.k);
-  grid_dependency_trigger();
-  grid_dependency_wait();
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, slices = 1 << a.slices_log;
-  const int64_t row = blockIdx.x >> a.slices_log;
-  const int slice = blockIdx.x & (slices - 1);
-  const T* z = static_cast<const T*>(a.pred) + row * a.ld;
-  T* out = GRAD ? static_cast<T*>(a.out) + row * a.ld_out : nullptr;
-  const bool labels = a.labels.p != nullptr;
-  const int64_t label = labels ? a.labels[row] : -1;
-  if (labels && (label == a.ignore || (uint64_t)label >= (uint64_t)a.v)) {  // the same for every block of the cluster
-    if (slice == 0 && tid == 0) {
-      a.loss[row] = 0.f;
-      if (a.stats) a.stats[row] = make_float4(0.f, 1.f, 1.f, -1.f);
-    }
-    if (GRAD) zero_slice(Slice<T>(out, (int)a.v, slice, a.slices_log, false), out);
-    return;
-  }
-  Fetch<T> fetch;
-  fetch.begin(a, row, label);
-
+// Running maximum and sums of a thread's groups.
+template <typename T, Second S>
+struct Sweep {
   Running run{-INFINITY, 0.f, 0.f};
-  const Slice<T> s(z, (int)a.v, slice, a.slices_log, false);
-  {
-    const uint4* middle = reinterpret_cast<const uint4*>(z + s.head);
-    Two soft(0.f, 0.f), hard(0.f, 0.f);
-    auto groups = [&](int i0, auto count) {
-      uint4 raw[count.value];
+  Two soft{0.f, 0.f}, hard{0.f, 0.f};
+
+  template <int COUNT>
+  __device__ __forceinline__ void add(const uint4* from, int step, float c) {
+    uint4 raw[COUNT];
 #pragma unroll
-      for (int u = 0; u < count.value; ++u) raw[u] = middle[i0 + u * kDistillThreads];
-      uint32_t most = Raw<T>::max2(raw[0]);
+    for (int u = 0; u < COUNT; ++u) raw[u] = from[u * step];
+    uint32_t most = Raw<T>::max2(raw[0]);
 #pragma unroll
-      for (int u = 1; u < count.value; ++u) most = Raw<T>::max2(most, Raw<T>::max2(raw[u]));
-      const float top = fmaxf(run.top, Raw<T>::max1(most)), base = base_of(top);
-      if (top != run.top) {
-        const float d = run.top - top;  // -infinity at first: the sums are 0 and stay it, or NaN
-        const float fs = run.top == -INFINITY ? 1.f : ex2(d * a.c), fh = run.top == -INFINITY ? 1.f : ex2(d * kLog2e);
-        soft = soft * Two(fs, fs);
-        if (S != kNone) hard = hard * Two(fh, fh);
-        run.top = top;
+    for (int u = 1; u < COUNT; ++u) most = Raw<T>::max2(most, Raw<T>::max2(raw[u]));
+    const float top = fmaxf(run.top, Raw<T>::max1(most)), base = base_of(top);
+    if (top != run.top) {
+      const float d = run.top - top;  // -infinity at first: the sums are 0 and stay it, or NaN
+      const float fs = run.top == -INFINITY ? 1.f : ex2(d * c), fh = run.top == -INFINITY ? 1.f : ex2(d * kLog2e);
+      soft = soft * Two(fs, fs);
+      if (S != kNone) hard = hard * Two(fh, fh);
+      run.top = top;
+    }
+    const Two nb(-base, -base), c2(c, c);
+#pragma unroll
+    for (int u = 0; u < COUNT; ++u) {
+#pragma unroll
+      for (int j = 0; j < Raw<T>::kPer / 2; ++j) {
+        const Two x = Raw<T>::pair(raw[u], j) + nb, p = ex2(x * c2);
+        soft = soft + p;
+        if (S == kOwn) hard = hard + ex2(x * Two(kLog2e, kLog2e));
+        if (S == kSquare) hard = fma2(p, p, hard);
+        if (S == kFourth) hard = fma2(p * p, p * p, hard);
       }
-      const Two nb(-base, -base), c2(a.c, a.c);
-#pragma unroll
-      for (int u = 0; u < count.value; ++u) {
-#pragma unroll
-        for (int j = 0; j < per / 2; ++j) {
-          const Two x = Raw<T>::pair(raw[u], j) + nb, p = ex2(x * c2);
-          soft = soft + p;
-          if (S == kOwn) hard = hard + ex2(x * Two(kLog2e, kLog2e));
-          if (S == kSquare) hard = fma2(p, p, hard);
-          if (S == kFourth) hard = fma2(p * p, p * p, hard);
-        }
-      }
-    };
-    int i = s.from + tid;
-    for (; i + (kDistillUnroll - 1) * kDistillThreads < s.to; i += kDistillUnroll * kDistillThreads)
-      groups(i, std::integral_constant<int, kDistillUnroll>{});
-    for (; i < s.to; i += kDistillThreads) groups(i, std::integral_constant<int, 1>{});
+    }
+  }
+  // The groups of a batch that exist, `left` of them from the first on.
+  __device__ __forceinline__ void batch(const uint4* from, int step, int left, float c) {
+    if (left >= kDistillUnroll) add<kDistillUnroll>(from, step, c);
+    else if (left == 1) add<1>(from, step, c);
+    else if (left == 2) add<2>(from, step, c);
+    else if (left == 3) add<3>(from, step, c);
+  }
+  __device__ __forceinline__ void edge(float z, float c) {
+    rebase<S>(run, fmaxf(run.top, z), c);
+    const float base = base_of(run.top);
+    run.soft += power(z, base, c);
+    if (S != kNone) run.hard += power(z, base, kLog2e);
+  }
+  __device__ __forceinline__ void finish() {
     run.soft = soft.lo() + soft.hi();
     run.hard = hard.lo() + hard.hi();
   }
-  if (tid < s.edge) {
-    const float edge = Elem<T>::to_f32(z[s.edge_at(tid)]);
-    rebase<S>(run, fmaxf(run.top, edge), a.c);
-    const float base = base_of(run.top);
-    run.soft += power(edge, base, a.c);
-    if (S != kNone) run.hard += power(edge, base, kLog2e);
-  }
-  fetch.end(a, e, row, z, label);
-  // the block's maximum first, then sums relative to it
+};
+
+// What the warps of a block, and the blocks of a cluster, tell one another about a row.
+template <int WARPS>
+struct Exchange {
+  float tops[WARPS];
+  float2 sums[WARPS];
+  Running whole;
+  float some;    // sum of the teacher's weights - 1
+  float4 stats;
+};
+
+// A block is NT threads that sweep the logits, and a warp that sees to the teacher's entries meanwhile.
+template <int N>
+__device__ __forceinline__ void bar_sync(int id) {
+  asm volatile("bar.sync %0, %1;" ::"r"(id), "n"(N) : "memory");
+}
+template <int N>
+__device__ __forceinline__ void bar_arrive(int id) {
+  asm volatile("bar.arrive %0, %1;" ::"r"(id), "n"(N) : "memory");
+}
+enum { kSweepers = 1, kWeighed = 2, kWritten = 3 };  // barriers
+
+// Joins the sweeping threads' sums of a row: the block's maximum first and then sums relative to it.
+template <Second S, int NT>
+__device__ __forceinline__ float4 join(Exchange<NT / 32>& x, Running run, const DistillArgs& a) {
+  constexpr int kWarps = NT / 32;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   float top = run.top;
 #pragma unroll
   for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-  if (lane == 0) warps[warp].top = top;
-  __syncthreads();
+  if (lane == 0) x.tops[warp] = top;
+  bar_sync<NT>(kSweepers);
 #pragma unroll
-  for (int w = 0; w < kDistillWarps; ++w) top = fmaxf(top, warps[w].top);
+  for (int w = 0; w < kWarps; ++w) top = fmaxf(top, x.tops[w]);
   rebase<S>(run, top, a.c);
   run.soft = warp_sum(run.soft);
   if (S != kNone) run.hard = warp_sum(run.hard);
-  if (lane == 0) {
-    warps[warp].soft = run.soft;
-    warps[warp].hard = run.hard;
-  }
-  __syncthreads();
+  if (lane == 0) x.sums[warp] = make_float2(run.soft, run.hard);
+  bar_sync<NT + 32>(kWeighed);
   run = Running{top, 0.f, 0.f};
 #pragma unroll
-  for (int w = 0; w < kDistillWarps; ++w) {
-    run.soft += warps[w].soft;
-    run.hard += warps[w].hard;
+  for (int w = 0; w < kWarps; ++w) {
+    run.soft += x.sums[w].x;
+    run.hard += x.sums[w].y;
   }
   if (a.slices_log) {
-    if (tid == 0) whole = run;
+    if (threadIdx.x == 0) x.whole = run;
     cluster_sync();
-    for (int r = 0; r < slices; ++r) top = fmaxf(top, __uint_as_float(cluster_load(&whole.top, r)));
-    run = Running{top, 0.f, 0.f};
-    for (int r = 0; r < slices; ++r) {
-      Running other{__uint_as_float(cluster_load(&whole.top, r)), __uint_as_float(cluster_load(&whole.soft, r)),
-                    __uint_as_float(cluster_load(&whole.hard, r))};
-      rebase<S>(other, top, a.c);
-      run.soft += other.soft;
-      run.hard += other.hard;
+    Running all{-INFINITY, 0.f, 0.f};
+    for (int r = 0; r >> a.slices_log == 0; ++r) all.top = fmaxf(all.top, __uint_as_float(cluster_load(&x.whole.top, r)));
+    for (int r = 0; r >> a.slices_log == 0; ++r) {
+      Running part{__uint_as_float(cluster_load(&x.whole.top, r)), __uint_as_float(cluster_load(&x.whole.soft, r)),
+                   S != kNone ? __uint_as_float(cluster_load(&x.whole.hard, r)) : 0.f};
+      rebase<S>(part, all.top, a.c);
+      all.soft += part.soft;
+      all.hard += part.hard;
     }
-    cluster_sync();  // read by all before one of them overwrites its logits or ends
+    run = all;
+    cluster_sync();  // read by all before one of them overwrites its logits, joins its next row or ends
   }
-  const float base = base_of(run.top);
-  float4 stats = make_float4(run.top, run.soft, S != kNone ? run.hard : run.soft, 0.f);
-  if (warp == 0) {
-    float kl = 0.f;
-    stats.w = weigh(e, a.k, a.c, base, log2f(run.soft), &kl) - 1.f;
-    if (lane == 0) some_s = stats.w;
-    if (lane == 0 && slice == 0) {
-      float loss = a.soft_loss > 0.f ? a.soft_loss * kl : 0.f;  // a term without weight counts nothing, infinite or not
-      if (labels && a.hard > 0.f) loss += a.hard * kLn2 * (log2f(stats.z) - (e.z[a.k] - base) * kLog2e);
-      a.loss[row] = loss;
-      if (a.stats) a.stats[row] = stats;
+  return make_float4(run.top, run.soft, S != kNone ? run.hard : run.soft, x.some);
+}
+
+// The loss of a row, by one warp.
+__device__ __forceinline__ void put_loss(const DistillArgs& a, const Entries& e, int64_t row, const float4& stats, bool labels) {
+  const float base = base_of(stats.x), kl = divergence(e, a.k, a.c, base, log2f(stats.y));
+  if ((threadIdx.x & 31) != 0) return;
+  float loss = a.soft_loss > 0.f ? a.soft_loss * kl : 0.f;  // a term without weight counts nothing, infinite or not
+  if (labels && a.hard > 0.f) loss += a.hard * kLn2 * (log2f(stats.z) - (e.z[a.k] - base) * kLog2e);
+  a.loss[row] = loss;
+  if (a.stats) a.stats[row] = stats;
+}
+
+__device__ __forceinline__ bool left_out(const DistillArgs& a, int64_t label) {
+  return label == a.ignore || (uint64_t)label >= (uint64_t)a.v;
+}
+
+template <typename T, int NT, bool GRAD>
+__device__ __forceinline__ void leave_out(const DistillArgs& a, int64_t row, int slice) {
+  if (slice == 0 && threadIdx.x == 0) {
+    a.loss[row] = 0.f;
+    if (a.stats) a.stats[row] = make_float4(0.f, 1.f, 1.f, -1.f);
+  }
+  T* out = static_cast<T*>(a.out) + row * a.ld_out;
+  if (GRAD) zero_slice<T, NT>(Slice<T>(out, (int)a.v, slice, a.slices_log), out);
+}
+
+// Loss, and with GRAD the gradient, of a row by a cluster of 2^slices_log blocks: one pass with a running maximum and its
+// sums, joined over threads, warps and blocks.
+// GRAD reads the logits a second time, from the L2: the launch sees to it that it holds what the resident blocks work on.
+// XXX
+template <typename T, Second S, bool GRAD, int NT>
+__global__ void __launch_bounds__(NT + 32, kSweepThreads / NT) distill_kernel(DistillArgs a) {
+  extern __shared__ uint4 image[];
+  __shared__ Exchange<NT / 32> exchange;
+  grid_dependency_trigger();
+  grid_dependency_wait();
+  const int tid = threadIdx.x;
+  const int64_t row = blockIdx.x >> a.slices_log;
+  const int slice = blockIdx.x & ((1 << a.slices_log) - 1);
+  const bool labels = a.labels.p != nullptr;
+  const int64_t label = labels ? a.labels[row] : -1;
+  if (labels && left_out(a, label)) {  // the same for every block of the cluster
+    if (tid < NT) leave_out<T, NT, GRAD>(a, row, slice);
+    return;
+  }
+  const T* z = static_cast<const T*>(a.pred) + row * a.ld;
+  T* out = static_cast<T*>(a.out) + row * a.ld_out;
+  const Slice<T> s(z, (int)a.v, slice, a.slices_log);
+
+  if (tid >= NT) {  // the warp of the entries
+    const Entries e(image + Stream<T, NT>::kPlaces, a.k);
+    const float weight = GRAD && a.dy ? a.dy[row * a.dy_step] : 1.f;
+    load_entries(a, e, row, z, label);
+    const float some = weigh(e, a.k, a.c);
+    if (tid == NT) exchange.some = some - 1.f;
+    __syncwarp();
+    bar_arrive<NT + 32>(kWeighed);
+    if (a.slices_log) {
+      cluster_sync();
+      cluster_sync();
     }
+    bar_sync<NT + 32>(kWritten);
+    const float4 stats = exchange.stats;
+    if (GRAD) write_entries<T, S>(a, e, s, out, coefficients<S>(a, weight, stats, labels));
+    if (slice == 0) put_loss(a, e, row, stats, labels);
+    return;
   }
-  if (!GRAD) return;
-  __syncthreads();
-  stats.w = some_s;
-  const Coefficients co = coefficients<S>(a, row, stats, labels);
-  const Slice<T> so(out, (int)a.v, slice, a.slices_log, !alike(z, out));
-  write_slice<T, S>(so, z, out, co);
-  __syncthreads();
-  write_entries<T, S>(a, e, so, out, co, slice);
+
+  Stream<T, NT> stream(s, z, image);
+  stream.begin();
+  const float edge = tid < s.edges() ? Elem<T>::to_f32(z[s.edge_at(tid)]) : 0.f;
+  const float weight = GRAD && a.dy ? a.dy[row * a.dy_step] : 1.f;
+  Sweep<T, S> sweep;
+  stream.run([&](int, const uint4* place, int left) { sweep.batch(place, NT, left, a.c); });
+  if (GRAD && alike(z, out)) stream.begin();
+  sweep.finish();
+  if (tid < s.edges()) sweep.edge(edge, a.c);
+  const float4 stats = join<S, NT>(exchange, sweep.run, a);
+  if (tid == 0) exchange.stats = stats;
+  if (GRAD) write_slice<T, S, NT>(s, z, edge, out, coefficients<S>(a, weight, stats, labels), stream);
+  bar_arrive<NT + 32>(kWritten);
 }
 
 // The gradient from the statistics that the forward pass has left.
+constexpr int kDpredThreads = 128;
 template <typename T, Second S>
-__global__ void __launch_bounds__(kDistillThreads, kDistillBlocks) distill_dpred_kernel(DistillArgs a) {
-  extern __shared__ char smem[];
-  const Entries e(smem, a.k);
+__global__ void __launch_bounds__(kDpredThreads + 32, 6) distill_dpred_kernel(DistillArgs a) {
+  constexpr int NT = kDpredThreads;
+  extern __shared__ uint4 image[];
   grid_dependency_trigger();
   grid_dependency_wait();
   const int64_t row = blockIdx.x >> a.slices_log;
-  const int slice = blockIdx.x & ((1 << a.slices_log) - 1);
+  const int slice = blockIdx.x & ((1 << a.slices_log) - 1), tid = threadIdx.x;
   const T* z = static_cast<const T*>(a.pred) + row * a.ld;
   T* out = static_cast<T*>(a.out) + row * a.ld_out;
   const bool labels = a.labels.p != nullptr;
   const int64_t label = labels ? a.labels[row] : -1;
-  if (labels && (label == a.ignore || (uint64_t)label >= (uint64_t)a.v)) {
-    zero_slice(Slice<T>(out, (int)a.v, slice, a.slices_log, false), out);
+  if (labels && left_out(a, label)) {
+    if (tid < NT) zero_slice<T, NT>(Slice<T>(out, (int)a.v, slice, a.slices_log), out);
     return;
   }
+  const Slice<T> s(z, (int)a.v, slice, a.slices_log);
   const float4 stats = a.stats[row];
-  Fetch<T> fetch;
-  fetch.begin(a, row, label);
+  const float weight = a.dy ? a.dy[row * a.dy_step] : 1.f;
   const bool in_place = a.out == a.pred;
-  if (in_place) {  // this block's entries before any of it is overwritten (another block's are not used here)
-    fetch.end(a, e, row, z, label);
-    __syncthreads();
+  if (tid < NT) {
+    const float edge = tid < s.edges() ? Elem<T>::to_f32(z[s.edge_at(tid)]) : 0.f;
+    Stream<T, NT> stream(s, z, image);
+    if (alike(z, out)) stream.begin();
+    const Coefficients co = coefficients<S>(a, weight, stats, labels);
+    if (in_place) bar_sync<NT + 32>(kWeighed);  // the entries of this slice are read (those of others are not used here)
+    write_slice<T, S, NT>(s, z, edge, out, co, stream);
+    bar_arrive<NT + 32>(kWritten);
+    return;
   }
-  const Slice<T> s(out, (int)a.v, slice, a.slices_log, !alike(z, out));
-  const Coefficients co = coefficients<S>(a, row, stats, labels);
-  write_slice<T, S>(s, z, out, co);
-  if (!in_place) fetch.end(a, e, row, z, label);
-  __syncthreads();
-  if (threadIdx.x < 32) weigh(e, a.k, a.c, 0.f, 0.f, nullptr);
-  __syncthreads();
-  write_entries<T, S>(a, e, s, out, co, slice);
+  const Entries e(image + Stream<T, NT>::kPlaces, a.k);
+  load_entries(a, e, row, z, label);
+  if (in_place) bar_arrive<NT + 32>(kWeighed);
+  bool mine = false;
+  for (int i = tid - NT; i <= a.k; i += 32) mine |= e.at[i] >= 0 && s.owns(e.at[i]);
+  mine = __any_sync(0xffffffffu, mine);
+  if (mine) weigh(e, a.k, a.c);
+  bar_sync<NT + 32>(kWritten);
+  if (mine) write_entries<T, S>(a, e, s, out, coefficients<S>(a, weight, stats, labels));
 }
 
 static int check_args(const rafb200_distill* d, const char* who) {
@@ -608,12 +722,19 @@ static Second second_of(const rafb200_distill* d) {
   return d->temperature == 2.0 ? kSquare : d->temperature == 4.0 ? kFourth : kOwn;
 }
 
-// Blocks of a row, as a power of two: few rows are cut until every SM has work, while a thread keeps a group.
-static int row_slices_log(const rafb200_distill* d) {
-  int log = 0;
-  const int64_t groups = d->v * dtype_size(d->pred_dtype) / 16;
-  while (log < 3 && (d->n << (log + 1)) <= 148 * 2 && groups >> (log + 1) >= kDistillThreads) ++log;
-  return log;
+constexpr int64_t kMostGroups = 110 * 1024 / 16;
+static int64_t row_groups(const rafb200_distill* d) { return d->v * dtype_size(d->pred_dtype) / 16; }
+
+template <typename T, Second S, bool GRAD, int NT>
+static int launch_rows(const rafb200_distill* d, DistillArgs a, cudaStream_t s) {
+  const size_t smem = (size_t)kDistillRing * NT * 16 + Entries::bytes(d->k);
+  // few rows are cut until every SM has work, while a thread keeps a group
+  while (a.slices_log < 3 && (d->n << (a.slices_log + 1)) <= 148 * 2 && row_groups(d) >> (a.slices_log + 1) >= NT) ++a.slices_log;
+  // what the resident blocks hold of the logits, to be read again, is to stay in the L2
+  while (GRAD && a.slices_log < 3 && row_groups(d) >> a.slices_log > kMostGroups) ++a.slices_log;
+  if (const int rc = allow_smem<distill_kernel<T, S, GRAD, NT>>(smem)) return rc;
+  RAFB200_CUDA(launch_cluster(distill_kernel<T, S, GRAD, NT>, 1u << a.slices_log, (unsigned)(d->n << a.slices_log), NT + 32, smem, s, a));
+  return RAFB200_OK;
 }
 
 template <typename F>
@@ -641,11 +762,9 @@ int rafb200_distill_loss(const rafb200_distill* d, float* loss, float* stats, vo
   DistillArgs a = device_args(d);
   a.loss = loss;
   a.stats = reinterpret_cast<float4*>(stats);
-  a.slices_log = row_slices_log(d);
   return with_case(d, [&](auto t, auto second) {
-    RAFB200_CUDA(launch_cluster(distill_kernel<decltype(t), decltype(second)::value, false>, 1u << a.slices_log, (unsigned)(d->n << a.slices_log),
-                                kDistillThreads, Entries::bytes(d->k), static_cast<cudaStream_t>(stream), a));
-    return (int)RAFB200_OK;
+    if (row_groups(d) >= 4096) return launch_rows<decltype(t), decltype(second)::value, false, 256>(d, a, static_cast<cudaStream_t>(stream));
+    return launch_rows<decltype(t), decltype(second)::value, false, 128>(d, a, static_cast<cudaStream_t>(stream));
   });
 }
 
@@ -671,10 +790,17 @@ int rafb200_distill_loss_dpred(const rafb200_distill* d, const float* dy, int dy
   a.stats = reinterpret_cast<float4*>(const_cast<float*>(stats));
   a.out = dpred;
   a.ld_out = ld_dpred;
-  a.slices_log = row_slices_log(d);
+  // few rows are cut until every SM has its six blocks: blocks beyond that cost more than they even out (777 rows of 50257
+  // in fp16: 37 us whole, 45 us in eight parts; 100 rows: 20 us whole, 12 us in eight)
+  while (a.slices_log < 6 && d->n << (a.slices_log + 1) <= 148 * 6 && row_groups(d) >> (a.slices_log + 1) >= kDpredThreads * kDistillUnroll)
+    ++a.slices_log;
   return with_case(d, [&](auto t, auto second) {
-    RAFB200_CUDA(launch_dependent(distill_dpred_kernel<decltype(t), decltype(second)::value>, dim3((unsigned)(d->n << a.slices_log)),
-                                  kDistillThreads, Entries::bytes(d->k), static_cast<cudaStream_t>(stream), a));
+    using T = decltype(t);
+    constexpr Second S = decltype(second)::value;
+    const size_t smem = Stream<T, kDpredThreads>::kPlaces * 16 + Entries::bytes(d->k);
+    if (const int rc = allow_smem<distill_dpred_kernel<T, S>>(smem)) return rc;
+    RAFB200_CUDA(launch_dependent(distill_dpred_kernel<T, S>, dim3((unsigned)(d->n << a.slices_log)), kDpredThreads + 32, smem,
+                                  static_cast<cudaStream_t>(stream), a));
     return (int)RAFB200_OK;
   });
 }
@@ -692,11 +818,9 @@ int rafb200_distill_loss_with_dpred(const rafb200_distill* d, const float* dy, i
   a.loss = loss;
   a.out = dpred;
   a.ld_out = ld_dpred;
-  a.slices_log = row_slices_log(d);
   return with_case(d, [&](auto t, auto second) {
-    RAFB200_CUDA(launch_cluster(distill_kernel<decltype(t), decltype(second)::value, true>, 1u << a.slices_log, (unsigned)(d->n << a.slices_log),
-                                kDistillThreads, Entries::bytes(d->k), static_cast<cudaStream_t>(stream), a));
-    return (int)RAFB200_OK;
+    if (row_groups(d) >= 2048) return launch_rows<decltype(t), decltype(second)::value, true, 256>(d, a, static_cast<cudaStream_t>(stream));
+    return launch_rows<decltype(t), decltype(second)::value, true, 128>(d, a, static_cast<cudaStream_t>(stream));
   });
 }
 
