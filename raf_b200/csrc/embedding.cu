@@ -53,19 +53,11 @@ __global__ void __launch_bounds__(kLookupThreads)
 // ---- gradient ---------------------------------------------------------------------
 //   dx[r, :] (+)= scale * sum over the n with id_n = r of dy[n, :]
 // Three launches, every sum in an order that the tokens alone fix:
-//   1. the tokens are sorted, stably, by one cluster of eight blocks, while the other clusters write the zeros of rows
-//      without a token;
-//   2. a warp walks a chunk of the sorted tokens for 32 * VEC columns and keeps the sum of the present row in registers.
-//      A row whose tokens all lie in one chunk is written here; a row cut by a chunk's border leaves partial sums;
-//   3. the rows that were cut are joined, chunk after chunk.
-constexpr int kSortBlocks = 8;
-constexpr int kSortThreads = 1024;
-constexpr int kSortWarps = kSortThreads / 32;
-constexpr int kDigitBits = 9;  // two passes for tables of up to 2^18 - 1 rows; the counters of 32 warps take 64 KB
-constexpr int kDigits = 1 << kDigitBits;
-constexpr int kFillClusters = 17;  // with the sorting one 144 blocks of 148 SMs
-constexpr size_t kSortSmem = sizeof(uint32_t) * (kSortWarps * kDigits + 2 * kDigits + 32);
-
+//   1. the tokens are sorted, stably, while other blocks write the zeros of rows without a token;
+//   2. a warp walks `run` sorted tokens for 32 * VEC columns and keeps the sum of the present row in registers.  A row whose
+//      tokens all lie there is written there; a row cut by the border between two warps of a block is put together in shared
+//      memory, one cut by the border of a block (a chunk of tokens) leaves partial sums;
+//   3. the rows that were cut by chunks are joined, chunk after chunk.
 struct SortArgs {
   Ids ids;
   int64_t n;
@@ -74,8 +66,11 @@ struct SortArgs {
   uint2* a;            // (id, position) pairs: the last pass leaves them in a
   uint2* b;
   int passes, bits;    // digits and bits of each
-  unsigned char* fill; // bytes to zero, or nullptr
+  unsigned char* fill; // bytes to zero
   int64_t fill_bytes;
+  __device__ __forceinline__ uint32_t key(int64_t id) const {
+    return (uint64_t)id < (uint64_t)rows && id != padding ? (uint32_t)id : (uint32_t)rows;
+  }
 };
 
 __device__ void zero_bytes(unsigned char* p, int64_t bytes, int64_t worker, int64_t workers) {
@@ -87,13 +82,48 @@ __device__ void zero_bytes(unsigned char* p, int64_t bytes, int64_t worker, int6
   if (worker < bytes - tail) p[tail + worker] = 0;
 }
 
-// Digits from the lowest up.  Each of the cluster's 256 warps owns a contiguous range of the pairs: it counts
+// Few tokens: each warp finds the rank of its tokens by comparing them with all, which need no more than one block's shared
+// memory.  No block waits for another.
+constexpr int kRankTokens = 4096;
+constexpr int kRankThreads = 256;
+__global__ void __launch_bounds__(kRankThreads) embedding_rank_kernel(SortArgs a) {
+  __shared__ uint32_t keys[kRankTokens];
+  grid_dependency_trigger();
+  grid_dependency_wait();
+  const int n = (int)a.n, tid = threadIdx.x, lane = tid & 31, warps = gridDim.x * (kRankThreads / 32);
+  const int mine = blockIdx.x * (kRankThreads / 32) + (tid >> 5);
+  if (blockIdx.x * (kRankThreads / 32) < n) {
+    for (int i = tid; i < n; i += kRankThreads) keys[i] = a.key(a.ids[i]);
+    __syncthreads();
+    for (int i = mine; i < n; i += warps) {
+      const uint32_t key = keys[i];
+      int rank = 0;
+#pragma unroll 4
+      for (int j = lane; j < n; j += 32) rank += keys[j] < key + (j < i);  // key is below 2^32 - 1
+      rank = __reduce_add_sync(0xffffffffu, rank);
+      if (lane == 0) a.a[rank] = make_uint2(key, (uint32_t)i);
+    }
+  }
+  zero_bytes(a.fill, a.fill_bytes, (int64_t)blockIdx.x * kRankThreads + tid, (int64_t)gridDim.x * kRankThreads);
+}
+
+// Many tokens: digits from the lowest up, by one cluster.  Each of its 256 warps owns a contiguous range of the pairs: it counts
 // its digits, the counts are summed over warps, blocks (through distributed shared memory) and digits, and
 // the warp then moves its pairs in order, equal digits of a group of 32 ranked by lane.
+// 65536 tokens take XXX us, 16384 take XXX us.
+constexpr int kSortBlocks = 8;
+constexpr int kSortThreads = 1024;
+constexpr int kSortWarps = kSortThreads / 32;
+constexpr int kSortItems = 8;  // pairs of a lane in registers
+constexpr int kDigitBits = 9;  // two passes for tables of up to 2^18 - 1 rows; the counters of 32 warps take 64 KB
+constexpr int kDigits = 1 << kDigitBits;
+constexpr int kFillClusters = 17;  // with the sorting one 144 blocks of 148 SMs
+constexpr size_t kSortSmem = sizeof(uint32_t) * (kSortWarps * kDigits + kSortBlocks * kDigits + kDigits + 32);
+
 __global__ void __launch_bounds__(kSortThreads) embedding_sort_kernel(SortArgs a) {
   extern __shared__ uint32_t counts[];  // [warp][digit]
-  uint32_t* totals = counts + kSortWarps * kDigits;
-  uint32_t* base = totals + kDigits;
+  uint32_t* totals = counts + kSortWarps * kDigits;  // [block][digit]
+  uint32_t* base = totals + kSortBlocks * kDigits;
   uint32_t* scan = base + kDigits;
   grid_dependency_trigger();
   grid_dependency_wait();
@@ -102,47 +132,60 @@ __global__ void __launch_bounds__(kSortThreads) embedding_sort_kernel(SortArgs a
                (int64_t)(gridDim.x - kSortBlocks) * kSortThreads);
     return;
   }
+  cluster_arrive();  // all blocks of the cluster run before one stores into another's shared memory
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t rank = cluster_rank();
   const int64_t each = ((a.n + kSortBlocks * kSortWarps - 1) / (kSortBlocks * kSortWarps) + 31) & ~int64_t(31);
   const int64_t from = min(((int64_t)rank * kSortWarps + warp) * each, a.n), to = min(from + each, a.n);
   uint32_t* mine = counts + warp * kDigits;
   const int digits = 1 << a.bits;
+  const bool kept = each <= 32 * kSortItems;  // a warp's pairs stay in registers from counting to moving
   for (int pass = 0; pass < a.passes; ++pass) {
     const int shift = pass * a.bits;
     // the passes end in a
     const uint2* src = ((a.passes - pass) & 1) ? a.b : a.a;
     uint2* dst = ((a.passes - pass) & 1) ? a.a : a.b;
-    auto pair_at = [&](int64_t i) {
-      if (pass) return __ldcg(src + i);
-      const int64_t id = a.ids[i];
-      const bool counts_in = (uint64_t)id < (uint64_t)a.rows && id != a.padding;
-      return make_uint2(counts_in ? (uint32_t)id : (uint32_t)a.rows, (uint32_t)i);
+    uint2 pair[kSortItems];
+    auto load = [&](int64_t i0) {  // of every 32 pairs from i0 on this lane's
+#pragma unroll
+      for (int u = 0; u < kSortItems; ++u) {
+        const int64_t i = i0 + u * 32 + lane;
+        if (i < to) pair[u] = pass ? __ldcg(src + i) : make_uint2(a.key(a.ids[i]), (uint32_t)i);
+      }
     };
+    auto digit = [&](int64_t i0, int u) { return i0 + u * 32 + lane < to ? (pair[u].x >> shift) & (digits - 1) : digits; };
     for (int d = lane; d < digits; d += 32) mine[d] = 0;
     __syncwarp();
-    for (int64_t i0 = from; i0 < to; i0 += 32) {
-      const bool in = i0 + lane < to;
-      const uint32_t d = in ? (pair_at(i0 + lane).x >> shift) & (digits - 1) : digits;
-      const uint32_t same = __match_any_sync(0xffffffffu, d);
-      if (in && lane == __ffs(same) - 1) mine[d] += __popc(same);
-      __syncwarp();
+    for (int64_t i0 = from; i0 < to; i0 += 32 * kSortItems) {
+      load(i0);
+#pragma unroll
+      for (int u = 0; u < kSortItems; ++u) {
+        if (i0 + u * 32 >= to) break;
+        const uint32_t d = digit(i0, u), same = __match_any_sync(0xffffffffu, d);
+        if (d < digits && lane == __ffs(same) - 1) mine[d] += __popc(same);
+        __syncwarp();
+      }
     }
     __syncthreads();
-    for (int d = tid; d < digits; d += kSortThreads) {
-      uint32_t sum = 0;
+    if (pass == 0) cluster_wait();
+    if (tid < digits) {
+      uint32_t c[kSortWarps], sum = 0;
+#pragma unroll
+      for (int w = 0; w < kSortWarps; ++w) c[w] = counts[w * kDigits + tid];
+#pragma unroll
       for (int w = 0; w < kSortWarps; ++w) {
-        const uint32_t c = counts[w * kDigits + d];
-        counts[w * kDigits + d] = sum;
-        sum += c;
+        counts[w * kDigits + tid] = sum;
+        sum += c[w];
       }
-      totals[d] = sum;
+#pragma unroll
+      for (uint32_t r = 0; r < kSortBlocks; ++r) cluster_store(totals + rank * kDigits + tid, r, sum);
     }
     cluster_sync();
     uint32_t before = 0, all = 0;  // of this thread's digit: in the blocks before this one, in all of them
     if (tid < digits) {
+#pragma unroll
       for (uint32_t r = 0; r < kSortBlocks; ++r) {
-        const uint32_t c = cluster_load(totals + tid, r);
+        const uint32_t c = totals[r * kDigits + tid];
         if (r < rank) before += c;
         all += c;
       }
@@ -157,27 +200,27 @@ __global__ void __launch_bounds__(kSortThreads) embedding_sort_kernel(SortArgs a
     __syncthreads();
     if (tid < digits) {
       uint32_t lower = incl - all;
-      for (int w = 0; w < warp; ++w) lower += scan[w];
+#pragma unroll
+      for (int w = 0; w < kDigits / 32; ++w)
+        if (w < warp) lower += scan[w];
       base[tid] = lower + before;
     }
     __syncthreads();
-    for (int64_t i0 = from; i0 < to; i0 += 32) {
-      const bool in = i0 + lane < to;
-      uint2 pair = make_uint2(0, 0);
-      uint32_t d = digits;
-      if (in) {
-        pair = pair_at(i0 + lane);
-        d = (pair.x >> shift) & (digits - 1);
+    for (int64_t i0 = from; i0 < to; i0 += 32 * kSortItems) {
+      if (!kept) load(i0);
+#pragma unroll
+      for (int u = 0; u < kSortItems; ++u) {
+        if (i0 + u * 32 >= to) break;
+        const uint32_t d = digit(i0, u), same = __match_any_sync(0xffffffffu, d);
+        uint32_t old = 0;
+        if (d < digits) old = mine[d];
+        __syncwarp();
+        if (d < digits && lane == __ffs(same) - 1) mine[d] = old + __popc(same);
+        __syncwarp();
+        if (d < digits) __stcg(dst + base[d] + old + __popc(same & ((1u << lane) - 1u)), pair[u]);
       }
-      const uint32_t same = __match_any_sync(0xffffffffu, d);
-      uint32_t old = 0;
-      if (in) old = mine[d];
-      __syncwarp();
-      if (in && lane == __ffs(same) - 1) mine[d] = old + __popc(same);
-      __syncwarp();
-      if (in) __stcg(dst + base[d] + old + __popc(same & ((1u << lane) - 1u)), pair);
     }
-    cluster_sync();  // the pairs are written for all, and no block reads the totals any more
+    cluster_sync();  // the pairs are written for all, and no block stores totals or counts before all have read theirs
   }
 }
 
@@ -190,81 +233,127 @@ struct SumArgs {
   void* dx;
   float* partial;        // [chunk][2][stride]: sums of a row that began before the chunk, or goes on behind it
   int64_t stride;
-  int chunk;             // tokens of a chunk
+  int run;               // tokens of a warp
   int64_t tiles;         // column tiles of 32 * VEC
 };
 
-constexpr int kSumThreads = 256;
-constexpr int kSumUnroll = 4;
+constexpr int kSumWarps = 8;  // of a chunk
+constexpr int kSumThreads = 32 * kSumWarps;
+constexpr int kSumUnroll = 8;
 
-template <typename O, int VEC>
-__device__ __forceinline__ void put_row(const SumArgs& a, uint32_t row, int64_t col, const float* sum) {
-  O* at = static_cast<O*>(a.dx) + (int64_t)row * a.width + col;
-  Group<O, VEC> o;
-  if (a.accumulate) {
-    o.load(at);
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) o.x[j] = fmaf(sum[j], a.scale, o.x[j]);
-  } else {
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) o.x[j] = sum[j] * a.scale;
-  }
-  o.store(at);
-}
-
-// Bound: HBM, the gathered rows of dy.  kSumUnroll rows are in flight per lane.
+// Bound: HBM, the gathered rows of dy.  kSumUnroll rows are in flight per lane, and what an accumulated row holds already is
+// asked for when its first token is met.
 template <typename T, typename O, int VEC>
 __global__ void __launch_bounds__(kSumThreads) embedding_sum_kernel(SumArgs a) {
+  __shared__ float parts[kSumWarps][32 * VEC];  // the warp's part of a row that began before it
+  __shared__ int through[kSumWarps];            // that row takes all of the warp's tokens and goes on behind it
   grid_dependency_trigger();
   grid_dependency_wait();
-  const int lane = threadIdx.x & 31;
-  const int64_t unit = (int64_t)blockIdx.x * (kSumThreads / 32) + (threadIdx.x >> 5);
-  const int64_t chunk = unit / a.tiles, col = (unit % a.tiles * 32 + lane) * VEC;
-  const int64_t from = chunk * a.chunk, to = min(from + a.chunk, a.n);
-  if (from >= a.n || col >= a.width) return;
-  const T* dy = static_cast<const T*>(a.dy) + col;
-  const uint32_t before = from ? a.sorted[from - 1].x : 0xffffffffu;
-  const uint32_t behind = to < a.n ? a.sorted[to].x : 0xffffffffu;
-  uint32_t row = a.sorted[from].x;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t chunk = blockIdx.x / a.tiles, col = (blockIdx.x % a.tiles * 32 + lane) * VEC;
+  const int64_t from = (chunk * kSumWarps + warp) * a.run, to = min(from + a.run, a.n);
+  const bool here = col < a.width;  // lanes behind the last column see to the tokens alone
+  const uint32_t rows = (uint32_t)a.rows;
+  const T* dy = static_cast<const T*>(a.dy) + (here ? col : 0);
+  O* dx = static_cast<O*>(a.dx) + col;
+  uint32_t row = rows, before = rows, behind = rows;
   float sum[VEC];
+  Group<O, VEC> old;
 #pragma unroll
   for (int j = 0; j < VEC; ++j) sum[j] = 0.f;
-  auto put_partial = [&](int slot) {
-    float* at = a.partial + (chunk * 2 + slot) * a.stride + col;
-    if constexpr (VEC == 8) {
-      reinterpret_cast<float4*>(at)[0] = make_float4(sum[0], sum[1], sum[2], sum[3]);
-      reinterpret_cast<float4*>(at)[1] = make_float4(sum[4], sum[5], sum[6], sum[7]);
-    } else {
+  auto begin = [&](uint32_t r) {
+    row = r;
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) at[j] = sum[j];
-    }
+    for (int j = 0; j < VEC; ++j) sum[j] = 0.f;
+    if (a.accumulate && here && r < rows && r != before) old.load(dx + (int64_t)r * a.width);
   };
-  for (int64_t i0 = from; i0 < to; i0 += kSumUnroll) {
-    uint2 pair[kSumUnroll];
-    Group<T, VEC> g[kSumUnroll];
+  auto put = [&](const float* s, const Group<O, VEC>& was, uint32_t r) {
+    if (!here) return;
+    Group<O, VEC> o;
 #pragma unroll
-    for (int u = 0; u < kSumUnroll; ++u) pair[u] = i0 + u < to ? a.sorted[i0 + u] : make_uint2(0xffffffffu, 0);
+    for (int j = 0; j < VEC; ++j) o.x[j] = a.accumulate ? fmaf(s[j], a.scale, was.x[j]) : s[j] * a.scale;
+    o.store(dx + (int64_t)r * a.width);
+  };
+  auto keep = [&] {
 #pragma unroll
-    for (int u = 0; u < kSumUnroll; ++u)
-      if (pair[u].x < (uint32_t)a.rows) g[u].load(dy + (int64_t)pair[u].y * a.width);
+    for (int j = 0; j < VEC; ++j) parts[warp][j * 32 + lane] = sum[j];
+  };
+  bool through_w = false;
+  if (from < a.n) {
+    before = from ? a.sorted[from - 1].x : rows;
+    behind = to < a.n ? a.sorted[to].x : rows;
+    bool first = true;
+    for (int64_t i0 = from; i0 < to; i0 += 32) {
+      const uint2 mine = i0 + lane < to ? a.sorted[i0 + lane] : make_uint2(rows, 0);
+      const int count = (int)min((int64_t)32, to - i0);
+      for (int q0 = 0; q0 < count; q0 += kSumUnroll) {
+        if (__shfl_sync(0xffffffffu, mine.x, q0) >= rows) break;
+        uint32_t r[kSumUnroll];
+        typename Group<T, VEC>::W g[kSumUnroll];
 #pragma unroll
-    for (int u = 0; u < kSumUnroll; ++u) {
-      if (pair[u].x >= (uint32_t)a.rows) continue;
-      if (pair[u].x != row) {
-        if (row == before) put_partial(0);
-        else put_row<O, VEC>(a, row, col, sum);
-        row = pair[u].x;
+        for (int u = 0; u < kSumUnroll; ++u) {
+          r[u] = __shfl_sync(0xffffffffu, mine.x, q0 + u);
+          const uint32_t at = __shfl_sync(0xffffffffu, mine.y, q0 + u);
+          // without a condition, or the loads would wait for one another: what does not count is loaded all the same
+          g[u] = *reinterpret_cast<const typename Group<T, VEC>::W*>(dy + (int64_t)at * a.width);
+        }
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) sum[j] = 0.f;
+        for (int u = 0; u < kSumUnroll; ++u) {
+          if (r[u] >= rows) break;  // behind the last token that counts
+          if (first) {
+            begin(r[u]);
+            first = false;
+          } else if (r[u] != row) {
+            if (row == before) keep();
+            else put(sum, old, row);
+            begin(r[u]);
+          }
+          float x[VEC];
+          Group<T, VEC>::unpack(g[u], x);
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) sum[j] += x[j];
+        }
       }
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) sum[j] += g[u].x[j];
+    }
+    // the last row: of this warp alone, begun before it, or going on behind it
+    if (row < rows) {
+      through_w = row == before && row == behind && row == a.sorted[from].x;
+      if (row == before) keep();
+      else if (row != behind) put(sum, old, row);
     }
   }
-  if (row >= (uint32_t)a.rows) return;
-  if (row == before) put_partial(0);
-  else if (row == behind) put_partial(1);
-  else put_row<O, VEC>(a, row, col, sum);
+  if (lane == 0) through[warp] = through_w;
+  const bool starts = row < rows && row != before && row == behind;   // a row goes on behind this warp
+  const uint32_t head = warp == 0 && from < a.n ? a.sorted[from].x : rows;
+  const bool enters = head < rows && head == before;                  // a row began before this chunk
+  __syncthreads();
+  if (!(starts || enters)) return;
+  // warp 0 may see to two rows: the one that began before the chunk, and one that begins with it
+  auto follow = [&](int w) {  // adds the parts of warps w, w + 1, ... as far as the row goes on; whether it leaves the chunk
+    for (; w < kSumWarps; ++w) {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) sum[j] += parts[w][j * 32 + lane];
+      if (!through[w]) return false;
+    }
+    return true;
+  };
+  auto put_partial = [&](int slot) {
+    if (!here) return;
+    Group<float, VEC> g;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) g.x[j] = sum[j];
+    g.store(a.partial + (chunk * 2 + slot) * a.stride + col);
+  };
+  if (starts) {
+    if (warp == kSumWarps - 1 || follow(warp + 1)) put_partial(1);
+    else put(sum, old, row);
+  }
+  if (enters) {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) sum[j] = 0.f;
+    follow(0);
+    put_partial(0);
+  }
 }
 
 // The rows that chunks have cut: the block of the chunk in which a row begins adds up its parts.  Eight warps take
@@ -277,17 +366,18 @@ __global__ void __launch_bounds__(kJoinThreads) embedding_join_kernel(SumArgs a)
   __shared__ float4 part[kJoinThreads / 32][32];
   grid_dependency_trigger();
   grid_dependency_wait();
-  const int64_t chunk = blockIdx.x, from = chunk * a.chunk, to = from + a.chunk;
+  const int64_t tokens = (int64_t)kSumWarps * a.run, chunk = blockIdx.x, from = chunk * tokens, to = from + tokens;
   if (to >= a.n) return;
-  const uint32_t row = a.sorted[to].x;
-  if (row >= (uint32_t)a.rows || a.sorted[to - 1].x != row || (from && a.sorted[from - 1].x == row)) return;
+  const uint32_t row = a.sorted[to].x, last = a.sorted[to - 1].x, before = from ? a.sorted[from - 1].x : (uint32_t)a.rows;
+  if (row >= (uint32_t)a.rows || last != row || before == row) return;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t col = (int64_t)blockIdx.y * kJoinCols + lane * 4;
   const float* at = a.partial + col;
   float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
   if (col < a.width) {
     if (warp == 0) sum = *reinterpret_cast<const float4*>(at + (chunk * 2 + 1) * a.stride);
-    for (int64_t c = chunk + 1 + warp; c * a.chunk < a.n && a.sorted[c * a.chunk].x == row; c += kJoinThreads / 32) {
+#pragma unroll 4
+    for (int64_t c = chunk + 1 + warp; c * tokens < a.n && a.sorted[c * tokens].x == row; c += kJoinThreads / 32) {
       const float4 p = *reinterpret_cast<const float4*>(at + c * 2 * a.stride);
       sum.x += p.x;
       sum.y += p.y;
@@ -306,24 +396,26 @@ __global__ void __launch_bounds__(kJoinThreads) embedding_join_kernel(SumArgs a)
     sum.w += part[w][lane].w;
   }
   const float s[4] = {sum.x, sum.y, sum.z, sum.w};
-  for (int j = 0; j < 4 && col + j < a.width; ++j) put_row<O, 1>(a, row, col + j, s + j);
+  O* dx = static_cast<O*>(a.dx) + (int64_t)row * a.width + col;
+  for (int j = 0; j < 4 && col + j < a.width; ++j)
+    dx[j] = Elem<O>::from_f32(a.accumulate ? fmaf(s[j], a.scale, Elem<O>::to_f32(dx[j])) : s[j] * a.scale);
 }
 
-// Elements of a vector access that every row of both arrays allows.
+// Elements of an access that every row of both arrays allows: 16 bytes of the first array's, 2, or 1.
 static int group_width(const void* p, int size_p, const void* q, int size_q, int64_t width) {
-  auto fits = [&](int vec, int bytes_p, int bytes_q) {
-    return width % vec == 0 && reinterpret_cast<uintptr_t>(p) % bytes_p == 0 && reinterpret_cast<uintptr_t>(q) % bytes_q == 0;
+  auto fits = [&](int vec) {
+    return width % vec == 0 && reinterpret_cast<uintptr_t>(p) % std::min(vec * size_p, 16) == 0 &&
+           reinterpret_cast<uintptr_t>(q) % std::min(vec * size_q, 16) == 0;
   };
-  if (fits(8, 16, 16)) return 8;
-  return fits(2, 2 * size_p, 2 * size_q) ? 2 : 1;
+  return fits(16 / size_p) ? 16 / size_p : fits(2) ? 2 : 1;
 }
 
-template <typename F>
+template <typename T, typename F>
 static int with_width(int vec, const F& f) {
   switch (vec) {
-    case 8: return f(std::integral_constant<int, 8>{});
+    case 1: return f(std::integral_constant<int, 1>{});
     case 2: return f(std::integral_constant<int, 2>{});
-    default: return f(std::integral_constant<int, 1>{});
+    default: return f(std::integral_constant<int, 16 / (int)sizeof(T)>{});
   }
 }
 
@@ -332,10 +424,10 @@ static bool range_overflows(int64_t a, int64_t b) {
   return __builtin_mul_overflow(a, b, &r) || r > ((int64_t)1 << 60);
 }
 
-// Tokens of a chunk: long chunks cut fewer rows, and short ones give every SM 32 warps.
-static int chunk_tokens(int64_t n, int64_t tiles) {
-  const int64_t want = n * tiles / (148 * 32) / kSumUnroll * kSumUnroll;
-  return (int)std::min<int64_t>(std::max<int64_t>(want, 2 * kSumUnroll), 256);
+// Tokens of a warp: many of them cut fewer rows, few of them give every SM four blocks.
+static int warp_tokens(int64_t n, int64_t width) {
+  const int64_t tiles = (width + 255) / 256, want = n * tiles / (148 * 4 * kSumWarps) / kSumUnroll * kSumUnroll;
+  return (int)std::min<int64_t>(std::max<int64_t>(want, kSumUnroll), 128);
 }
 
 static size_t round_up(size_t x) { return (x + 255) & ~size_t(255); }
@@ -363,7 +455,7 @@ int rafb200_embedding(const void* x, int x_dtype, int64_t rows, int64_t width, c
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   return with_type(x_dtype, [&](auto t) {
     return with_type(out_dtype, [&](auto o) {
-      return with_width(vec, [&](auto w) {
+      return with_width<decltype(t)>(vec, [&](auto w) {
         using T = decltype(t);
         using O = decltype(o);
         RAFB200_CUDA(launch_dependent(embedding_kernel<T, O, decltype(w)::value>, dim3((unsigned)grid), kLookupThreads, 0, s,
@@ -374,12 +466,11 @@ int rafb200_embedding(const void* x, int x_dtype, int64_t rows, int64_t width, c
   });
 }
 
-// Layout of the workspace: the pairs twice, then the partial sums.  It does not go by the widths of accesses,
-// which depend on addresses: the partial sums are those of the narrowest chunks there can be.
+// The workspace holds the pairs twice, then the partial sums of the chunks.
 size_t rafb200_embedding_dx_workspace_bytes(int64_t n, int64_t width) {
   if (n <= 0 || width <= 0 || n >= ((int64_t)1 << 31) || range_overflows(n, width)) return 0;
-  const int64_t chunks = (n + chunk_tokens(n, (width + 255) / 256) - 1) / chunk_tokens(n, (width + 255) / 256);
-  return 2 * round_up((size_t)n * sizeof(uint2)) + (size_t)chunks * 2 * ((width + 7) & ~7) * sizeof(float);
+  const int64_t tokens = (int64_t)kSumWarps * warp_tokens(n, width), chunks = (n + tokens - 1) / tokens;
+  return 2 * round_up((size_t)n * sizeof(uint2)) + (size_t)chunks * 2 * ((width + 7) & ~int64_t(7)) * sizeof(float);
 }
 
 int rafb200_embedding_dx(const void* dy, int dy_dtype, const void* indices, int index_dtype, int64_t n, int64_t rows,
@@ -408,15 +499,22 @@ int rafb200_embedding_dx(const void* dy, int dy_dtype, const void* indices, int 
   while (rows >> bits) ++bits;
   so.passes = (bits + kDigitBits - 1) / kDigitBits;
   so.bits = (bits + so.passes - 1) / so.passes;
-  unsigned clusters = 1;
   if (!accumulate) {
     so.fill = static_cast<unsigned char*>(dx);
     so.fill_bytes = rows * width * dtype_size(dx_dtype);
-    const int64_t each = (int64_t)kSortBlocks * kSortThreads * 64;  // four stores a thread
-    clusters += (unsigned)std::min<int64_t>((so.fill_bytes + each - 1) / each, kFillClusters);
   }
-  if (const int rc = allow_smem<embedding_sort_kernel>(kSortSmem)) return rc;
-  RAFB200_CUDA(launch_cluster(embedding_sort_kernel, kSortBlocks, clusters * kSortBlocks, kSortThreads, kSortSmem, s, so));
+  // three to six times as fast as the cluster's passes where a warp has one token to compare, and no slower at the border:
+  // XXX
+  if (n <= kRankTokens) {
+    const int64_t ranks = (n + kRankThreads / 32 - 1) / (kRankThreads / 32), fills = so.fill_bytes / (kRankThreads * 64);
+    const unsigned grid = (unsigned)std::min<int64_t>(std::max<int64_t>({ranks, fills, 1}), 148 * 4);
+    RAFB200_CUDA(launch_dependent(embedding_rank_kernel, dim3(grid), kRankThreads, 0, s, so));
+  } else {
+    const int64_t each = (int64_t)kSortBlocks * kSortThreads * 64;  // four stores a thread
+    const unsigned clusters = 1 + (unsigned)std::min<int64_t>((so.fill_bytes + each - 1) / each, kFillClusters);
+    if (const int rc = allow_smem<embedding_sort_kernel>(kSortSmem)) return rc;
+    RAFB200_CUDA(launch_cluster(embedding_sort_kernel, kSortBlocks, clusters * kSortBlocks, kSortThreads, kSortSmem, s, so));
+  }
   if (n == 0) return RAFB200_OK;
 
   const int vec = group_width(dy, dtype_size(dy_dtype), dx, dtype_size(dx_dtype), width);
@@ -432,14 +530,14 @@ int rafb200_embedding_dx(const void* dy, int dy_dtype, const void* indices, int 
   a.partial = reinterpret_cast<float*>(static_cast<char*>(workspace) + 2 * round_up((size_t)n * sizeof(uint2)));
   a.stride = (width + 7) & ~int64_t(7);
   a.tiles = (width + 32 * vec - 1) / (32 * vec);
-  a.chunk = chunk_tokens(n, (width + 255) / 256);
-  const int64_t chunks = (n + a.chunk - 1) / a.chunk;
-  const int64_t grid = (chunks * a.tiles + kSumThreads / 32 - 1) / (kSumThreads / 32), cols = (width + kJoinCols - 1) / kJoinCols;
+  a.run = warp_tokens(n, width);
+  const int64_t tokens = (int64_t)kSumWarps * a.run, chunks = (n + tokens - 1) / tokens;
+  const int64_t grid = chunks * a.tiles, cols = (width + kJoinCols - 1) / kJoinCols;
   RAFB200_REQUIRE(grid < ((int64_t)1 << 31) && cols < 65536, "rafb200_embedding_dx: rows too wide");
   return with_type(dx_dtype, [&](auto o) {
     using O = decltype(o);
     const int rc = with_type(dy_dtype, [&](auto t) {
-      return with_width(vec, [&](auto w) {
+      return with_width<decltype(t)>(vec, [&](auto w) {
         RAFB200_CUDA(launch_dependent(embedding_sum_kernel<decltype(t), O, decltype(w)::value>, dim3((unsigned)grid), kSumThreads,
                                       0, s, a));
         return (int)RAFB200_OK;

@@ -20,94 +20,97 @@ struct Ids {
 };
 inline bool index_dtype_valid(int t) { return t == RAFB200_I32 || t == RAFB200_I64; }
 
-// VEC consecutive elements widened to fp32: 8 (16-byte accesses, which the address must allow), 2 (4 bytes, for
-// 16-bit types) or 1.
+// The bytes of an access of `bytes` bytes, at most 16 of them.
+template <int BYTES>
+struct Word;
+template <>
+struct Word<2> { using type = unsigned short; };
+template <>
+struct Word<4> { using type = uint32_t; };
+template <>
+struct Word<8> { using type = uint2; };
+template <>
+struct Word<16> { using type = uint4; };
+
+// A 32-bit word of two 16-bit elements, widened and rounded.
+template <typename T>
+__device__ __forceinline__ float2 widen(uint32_t w) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) {  // bf16 -> fp32 is a 16-bit shift
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  } else {
+    return __half22float2(*reinterpret_cast<const __half2*>(&w));
+  }
+}
+template <typename T>
+__device__ __forceinline__ uint32_t narrow(float lo, float hi) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+}
+
+// VEC consecutive elements widened to fp32, in accesses of up to 16 bytes, which the address must allow.
 template <typename T, int VEC>
 struct Group {
+  static constexpr int kBytes = VEC * sizeof(T) < 16 ? VEC * sizeof(T) : 16, kWords = VEC * sizeof(T) / kBytes;
+  static constexpr int kPer = VEC / kWords;
+  using W = typename Word<kBytes>::type;
   float x[VEC];
   __device__ __forceinline__ void load(const T* p) {
-    if constexpr (VEC == 1) {
-      x[0] = Elem<T>::to_f32(*p);
-    } else if constexpr (VEC == 2) {
-      if constexpr (sizeof(T) == 2) {
-        const uint32_t r = *reinterpret_cast<const uint32_t*>(p);
-        T h[2];
-        memcpy(h, &r, 4);
-        x[0] = Elem<T>::to_f32(h[0]);
-        x[1] = Elem<T>::to_f32(h[1]);
-      } else {
-        const float2 r = *reinterpret_cast<const float2*>(p);
-        x[0] = r.x;
-        x[1] = r.y;
-      }
-    } else {
-      constexpr int per = 16 / sizeof(T);
 #pragma unroll
-      for (int q = 0; q < VEC / per; ++q) {
-        const uint4 r = reinterpret_cast<const uint4*>(p)[q];
-        unpack<T>(r, x + q * per);
-      }
-    }
+    for (int q = 0; q < kWords; ++q) unpack(reinterpret_cast<const W*>(p)[q], x + q * kPer);
   }
   __device__ __forceinline__ void store(T* p) const {
-    if constexpr (VEC == 1) {
-      *p = Elem<T>::from_f32(x[0]);
-    } else if constexpr (VEC == 2) {
-      if constexpr (sizeof(T) == 2) {
-        const T h[2] = {Elem<T>::from_f32(x[0]), Elem<T>::from_f32(x[1])};
-        uint32_t r;
-        memcpy(&r, h, 4);
-        *reinterpret_cast<uint32_t*>(p) = r;
+#pragma unroll
+    for (int q = 0; q < kWords; ++q) reinterpret_cast<W*>(p)[q] = pack(x + q * kPer);
+  }
+  static __device__ __forceinline__ void unpack(const W& w, float* f) {
+    if constexpr (sizeof(T) == 4) {
+      if constexpr (kBytes == 4) {
+        f[0] = __uint_as_float(w);
       } else {
-        *reinterpret_cast<float2*>(p) = make_float2(x[0], x[1]);
-      }
-    } else {
-      constexpr int per = 16 / sizeof(T);
-#pragma unroll
-      for (int q = 0; q < VEC / per; ++q) reinterpret_cast<uint4*>(p)[q] = pack<T>(x + q * per);
-    }
-  }
-  template <typename U>
-  static __device__ __forceinline__ void unpack(const uint4& r, float* f) {
-    if constexpr (sizeof(U) == 4) {
-      f[0] = __uint_as_float(r.x);
-      f[1] = __uint_as_float(r.y);
-      f[2] = __uint_as_float(r.z);
-      f[3] = __uint_as_float(r.w);
-    } else {
-      const uint32_t w[4] = {r.x, r.y, r.z, r.w};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if constexpr (std::is_same<U, __nv_bfloat16>::value) {  // bf16 -> fp32 is a 16-bit shift
-          f[2 * i] = __uint_as_float(w[i] << 16);
-          f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-        } else {
-          __half2 h;
-          memcpy(&h, &w[i], 4);
-          const float2 g = __half22float2(h);
-          f[2 * i] = g.x;
-          f[2 * i + 1] = g.y;
+        f[0] = __uint_as_float(w.x);
+        f[1] = __uint_as_float(w.y);
+        if constexpr (kBytes == 16) {
+          f[2] = __uint_as_float(w.z);
+          f[3] = __uint_as_float(w.w);
         }
+      }
+    } else if constexpr (kBytes == 2) {
+      f[0] = widen<T>(w).x;
+    } else {
+      uint32_t v[kBytes / 4];
+      if constexpr (kBytes == 4) {
+        v[0] = w;
+      } else {
+        v[0] = w.x;
+        v[1] = w.y;
+        if constexpr (kBytes == 16) {
+          v[2] = w.z;
+          v[3] = w.w;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < kBytes / 4; ++i) {
+        const float2 g = widen<T>(v[i]);
+        f[2 * i] = g.x;
+        f[2 * i + 1] = g.y;
       }
     }
   }
-  template <typename U>
-  static __device__ __forceinline__ uint4 pack(const float* f) {
-    if constexpr (sizeof(U) == 4) {
-      return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+  static __device__ __forceinline__ W pack(const float* f) {
+    if constexpr (sizeof(T) == 4) {
+      if constexpr (kBytes == 4) return __float_as_uint(f[0]);
+      else if constexpr (kBytes == 8) return make_uint2(__float_as_uint(f[0]), __float_as_uint(f[1]));
+      else return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
     } else {
-      uint32_t w[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if constexpr (std::is_same<U, __nv_bfloat16>::value) {
-          const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
-          memcpy(&w[i], &h, 4);
-        } else {
-          const __half2 h = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
-          memcpy(&w[i], &h, 4);
-        }
-      }
-      return make_uint4(w[0], w[1], w[2], w[3]);
+      if constexpr (kBytes == 2) return (unsigned short)narrow<T>(f[0], 0.f);
+      else if constexpr (kBytes == 4) return narrow<T>(f[0], f[1]);
+      else if constexpr (kBytes == 8) return make_uint2(narrow<T>(f[0], f[1]), narrow<T>(f[2], f[3]));
+      else return make_uint4(narrow<T>(f[0], f[1]), narrow<T>(f[2], f[3]), narrow<T>(f[4], f[5]), narrow<T>(f[6], f[7]));
     }
   }
 };
@@ -123,6 +126,12 @@ __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.w
 __device__ __forceinline__ void cluster_sync() {
   cluster_arrive();
   cluster_wait();
+}
+// Stores a word at the same shared-memory address in block `rank` of the cluster.
+__device__ __forceinline__ void cluster_store(void* p, uint32_t rank, uint32_t v) {
+  uint32_t at = (uint32_t)__cvta_generic_to_shared(p);
+  asm volatile("mapa.shared::cluster.u32 %0, %0, %1;" : "+r"(at) : "r"(rank));
+  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(at), "r"(v) : "memory");
 }
 // The word at the same shared-memory address in block `rank` of the cluster.
 __device__ __forceinline__ uint32_t cluster_load(const void* p, uint32_t rank) {
