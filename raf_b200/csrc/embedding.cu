@@ -107,24 +107,23 @@ __global__ void __launch_bounds__(kRankThreads) embedding_rank_kernel(SortArgs a
   zero_bytes(a.fill, a.fill_bytes, (int64_t)blockIdx.x * kRankThreads + tid, (int64_t)gridDim.x * kRankThreads);
 }
 
-// Many tokens: digits from the lowest up, by one cluster.  Each of its 256 warps owns a contiguous range of the pairs: it counts
-// its digits, the counts are summed over warps, blocks (through distributed shared memory) and digits, and
-// the warp then moves its pairs in order, equal digits of a group of 32 ranked by lane.
-// 65536 tokens take XXX us, 16384 take XXX us.
-constexpr int kSortBlocks = 8;
+// Many tokens: digits from the lowest up, by one cluster of 16 blocks.  Each of its 512 warps owns a contiguous range of the pairs:
+// it counts its digits, equal ones of a group of 32 ranked by lane; the counts are summed over warps, blocks (through
+// distributed shared memory) and digits, and the warp then moves its pairs in order.
+// XXX
+constexpr int kSortBlocks = 16;
 constexpr int kSortThreads = 1024;
 constexpr int kSortWarps = kSortThreads / 32;
 constexpr int kSortItems = 8;  // pairs of a lane in registers
 constexpr int kDigitBits = 9;  // two passes for tables of up to 2^18 - 1 rows; the counters of 32 warps take 64 KB
 constexpr int kDigits = 1 << kDigitBits;
-constexpr int kFillClusters = 17;  // with the sorting one 144 blocks of 148 SMs
-constexpr size_t kSortSmem = sizeof(uint32_t) * (kSortWarps * kDigits + kSortBlocks * kDigits + kDigits + 32);
+constexpr int kFillClusters = 15;
+constexpr size_t kSortSmem = sizeof(uint32_t) * (kSortWarps * kDigits + kSortBlocks * kDigits + 32);
 
 __global__ void __launch_bounds__(kSortThreads) embedding_sort_kernel(SortArgs a) {
   extern __shared__ uint32_t counts[];  // [warp][digit]
   uint32_t* totals = counts + kSortWarps * kDigits;  // [block][digit]
-  uint32_t* base = totals + kSortBlocks * kDigits;
-  uint32_t* scan = base + kDigits;
+  uint32_t* scan = totals + kSortBlocks * kDigits;
   grid_dependency_trigger();
   grid_dependency_wait();
   if (blockIdx.x >= kSortBlocks) {
@@ -133,12 +132,11 @@ __global__ void __launch_bounds__(kSortThreads) embedding_sort_kernel(SortArgs a
     return;
   }
   cluster_arrive();  // all blocks of the cluster run before one stores into another's shared memory
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const uint32_t rank = cluster_rank();
-  const int64_t each = ((a.n + kSortBlocks * kSortWarps - 1) / (kSortBlocks * kSortWarps) + 31) & ~int64_t(31);
-  const int64_t from = min(((int64_t)rank * kSortWarps + warp) * each, a.n), to = min(from + each, a.n);
+  const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rank = cluster_rank(), n = (uint32_t)a.n;
+  const uint32_t each = ((n + kSortBlocks * kSortWarps - 1) / (kSortBlocks * kSortWarps) + 31) & ~31u;
+  const uint32_t from = (uint32_t)min((uint64_t)(rank * kSortWarps + warp) * each, (uint64_t)n), to = min(n - from, each) + from;
   uint32_t* mine = counts + warp * kDigits;
-  const int digits = 1 << a.bits;
+  const uint32_t digits = 1u << a.bits, lower_lanes = (1u << lane) - 1u;
   const bool kept = each <= 32 * kSortItems;  // a warp's pairs stay in registers from counting to moving
   for (int pass = 0; pass < a.passes; ++pass) {
     const int shift = pass * a.bits;
@@ -146,37 +144,49 @@ __global__ void __launch_bounds__(kSortThreads) embedding_sort_kernel(SortArgs a
     const uint2* src = ((a.passes - pass) & 1) ? a.b : a.a;
     uint2* dst = ((a.passes - pass) & 1) ? a.a : a.b;
     uint2 pair[kSortItems];
-    auto load = [&](int64_t i0) {  // of every 32 pairs from i0 on this lane's
+    uint32_t place[kSortItems];  // the digit, and the rank among the warp's pairs of this digit << kDigitBits
+    auto load = [&](uint32_t i0) {  // of every 32 pairs from i0 on this lane's
 #pragma unroll
       for (int u = 0; u < kSortItems; ++u) {
-        const int64_t i = i0 + u * 32 + lane;
-        if (i < to) pair[u] = pass ? __ldcg(src + i) : make_uint2(a.key(a.ids[i]), (uint32_t)i);
+        const uint32_t i = i0 + u * 32 + lane;
+        if (i < to) pair[u] = pass ? __ldcg(src + i) : make_uint2(a.key(a.ids[i]), i);
       }
     };
-    auto digit = [&](int64_t i0, int u) { return i0 + u * 32 + lane < to ? (pair[u].x >> shift) & (digits - 1) : digits; };
-    for (int d = lane; d < digits; d += 32) mine[d] = 0;
-    __syncwarp();
-    for (int64_t i0 = from; i0 < to; i0 += 32 * kSortItems) {
-      load(i0);
+    auto count = [&](uint32_t i0) {  // ranks below 2^23: a warp's range, 2^31 / 512 pairs at most
 #pragma unroll
       for (int u = 0; u < kSortItems; ++u) {
         if (i0 + u * 32 >= to) break;
-        const uint32_t d = digit(i0, u), same = __match_any_sync(0xffffffffu, d);
-        if (d < digits && lane == __ffs(same) - 1) mine[d] += __popc(same);
+        const bool in = i0 + u * 32 + lane < to;
+        const uint32_t d = in ? (pair[u].x >> shift) & (digits - 1) : digits, same = __match_any_sync(0xffffffffu, d);
+        const uint32_t below = __popc(same & lower_lanes);
+        uint32_t old = 0;
+        if (in) old = mine[d];
         __syncwarp();
+        if (in && below == 0) mine[d] = old + __popc(same);
+        __syncwarp();
+        place[u] = d | (old + below) << kDigitBits;
       }
+    };
+    auto move = [&](uint32_t i0) {  // to the ranks, and to where the warp's pairs of a digit begin
+#pragma unroll
+      for (int u = 0; u < kSortItems; ++u)
+        if (i0 + u * 32 + lane < to) __stcg(dst + mine[place[u] & (kDigits - 1)] + (place[u] >> kDigitBits), pair[u]);
+    };
+    if (from < to) load(from);
+    for (uint32_t d = lane; d < digits; d += 32) mine[d] = 0;
+    __syncwarp();
+    for (uint32_t i0 = from; i0 < to; i0 += 32 * kSortItems) {
+      if (i0 != from) load(i0);
+      count(i0);
     }
     __syncthreads();
     if (pass == 0) cluster_wait();
+    uint32_t sum = 0, c[kSortWarps];
     if (tid < digits) {
-      uint32_t c[kSortWarps], sum = 0;
 #pragma unroll
       for (int w = 0; w < kSortWarps; ++w) c[w] = counts[w * kDigits + tid];
 #pragma unroll
-      for (int w = 0; w < kSortWarps; ++w) {
-        counts[w * kDigits + tid] = sum;
-        sum += c[w];
-      }
+      for (int w = 0; w < kSortWarps; ++w) sum += c[w];
 #pragma unroll
       for (uint32_t r = 0; r < kSortBlocks; ++r) cluster_store(totals + rank * kDigits + tid, r, sum);
     }
@@ -185,9 +195,9 @@ __global__ void __launch_bounds__(kSortThreads) embedding_sort_kernel(SortArgs a
     if (tid < digits) {
 #pragma unroll
       for (uint32_t r = 0; r < kSortBlocks; ++r) {
-        const uint32_t c = totals[r * kDigits + tid];
-        if (r < rank) before += c;
-        all += c;
+        const uint32_t t = totals[r * kDigits + tid];
+        if (r < rank) before += t;
+        all += t;
       }
     }
     uint32_t incl = all;  // exclusive sums over the digits
@@ -199,25 +209,35 @@ __global__ void __launch_bounds__(kSortThreads) embedding_sort_kernel(SortArgs a
     if (lane == 31) scan[warp] = incl;
     __syncthreads();
     if (tid < digits) {
-      uint32_t lower = incl - all;
+      uint32_t at = incl - all + before;
 #pragma unroll
-      for (int w = 0; w < kDigits / 32; ++w)
-        if (w < warp) lower += scan[w];
-      base[tid] = lower + before;
+      for (uint32_t w = 0; w < kDigits / 32; ++w)
+        if (w < warp) at += scan[w];
+#pragma unroll
+      for (int w = 0; w < kSortWarps; ++w) {
+        counts[w * kDigits + tid] = at;
+        at += c[w];
+      }
     }
     __syncthreads();
-    for (int64_t i0 = from; i0 < to; i0 += 32 * kSortItems) {
-      if (!kept) load(i0);
+    if (kept) {
+      move(from);
+    } else {
+      for (uint32_t i0 = from; i0 < to; i0 += 32 * kSortItems) {
+        load(i0);
 #pragma unroll
-      for (int u = 0; u < kSortItems; ++u) {
-        if (i0 + u * 32 >= to) break;
-        const uint32_t d = digit(i0, u), same = __match_any_sync(0xffffffffu, d);
-        uint32_t old = 0;
-        if (d < digits) old = mine[d];
-        __syncwarp();
-        if (d < digits && lane == __ffs(same) - 1) mine[d] = old + __popc(same);
-        __syncwarp();
-        if (d < digits) __stcg(dst + base[d] + old + __popc(same & ((1u << lane) - 1u)), pair[u]);
+        for (int u = 0; u < kSortItems; ++u) {
+          if (i0 + u * 32 >= to) break;
+          const bool in = i0 + u * 32 + lane < to;
+          const uint32_t d = in ? (pair[u].x >> shift) & (digits - 1) : digits, same = __match_any_sync(0xffffffffu, d);
+          const uint32_t below = __popc(same & lower_lanes);
+          uint32_t old = 0;
+          if (in) old = mine[d];
+          __syncwarp();
+          if (in && below == 0) mine[d] = old + __popc(same);
+          __syncwarp();
+          if (in) __stcg(dst + old + below, pair[u]);
+        }
       }
     }
     cluster_sync();  // the pairs are written for all, and no block stores totals or counts before all have read theirs
@@ -239,14 +259,37 @@ struct SumArgs {
 
 constexpr int kSumWarps = 8;  // of a chunk
 constexpr int kSumThreads = 32 * kSumWarps;
-constexpr int kSumUnroll = 8;
+constexpr int kSumBatch = 4;                  // rows asked for together
+constexpr int kSumAhead = 3;                  // batches on their way
+constexpr int kSumRing = kSumBatch * kSumAhead;
+constexpr int kMostRun = 64;                  // tokens of a warp, at most
 
-// Bound: HBM, the gathered rows of dy.  kSumUnroll rows are in flight per lane, and what an accumulated row holds already is
-// asked for when its first token is met.
+// Copies BYTES of one lane to shared memory: asynchronously where the hardware does (16, 8 or 4 bytes).
+template <int BYTES>
+__device__ __forceinline__ void copy_lane(void* to, const void* from) {
+  if constexpr (BYTES >= 4) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from), "n"(BYTES) : "memory");
+  } else {
+    *static_cast<unsigned short*>(to) = *static_cast<const unsigned short*>(from);
+  }
+}
+
+template <typename W, int VEC>
+struct SumShared {
+  W ring[kSumWarps][kSumRing][32];
+  float parts[kSumWarps][32 * VEC];  // the warp's part of a row that began before it
+  uint2 tokens[kSumWarps][kMostRun];
+  int through[kSumWarps];            // that row takes all of the warp's tokens and goes on behind it
+};
+
+// Bound: HBM, the gathered rows of dy.  Rows come through shared memory by asynchronous copies, kSumRing of them on their
+// way for a lane, which alone reads what it has asked for; what an accumulated row holds already is asked for when its
+// first token is met.
 template <typename T, typename O, int VEC>
-__global__ void __launch_bounds__(kSumThreads) embedding_sum_kernel(SumArgs a) {
-  __shared__ float parts[kSumWarps][32 * VEC];  // the warp's part of a row that began before it
-  __shared__ int through[kSumWarps];            // that row takes all of the warp's tokens and goes on behind it
+__global__ void __launch_bounds__(kSumThreads, 3) embedding_sum_kernel(SumArgs a) {
+  using W = typename Group<T, VEC>::W;
+  extern __shared__ uint4 shared[];
+  auto& [ring, parts, tokens, through] = *reinterpret_cast<SumShared<W, VEC>*>(shared);
   grid_dependency_trigger();
   grid_dependency_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -256,79 +299,78 @@ __global__ void __launch_bounds__(kSumThreads) embedding_sum_kernel(SumArgs a) {
   const uint32_t rows = (uint32_t)a.rows;
   const T* dy = static_cast<const T*>(a.dy) + (here ? col : 0);
   O* dx = static_cast<O*>(a.dx) + col;
-  uint32_t row = rows, before = rows, behind = rows;
+  uint32_t row = rows, before = rows, behind = rows, first = rows;
   float sum[VEC];
   Group<O, VEC> old;
 #pragma unroll
   for (int j = 0; j < VEC; ++j) sum[j] = 0.f;
-  auto begin = [&](uint32_t r) {
-    row = r;
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) sum[j] = 0.f;
-    if (a.accumulate && here && r < rows && r != before) old.load(dx + (int64_t)r * a.width);
-  };
-  auto put = [&](const float* s, const Group<O, VEC>& was, uint32_t r) {
+  auto put = [&] {
     if (!here) return;
     Group<O, VEC> o;
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) o.x[j] = a.accumulate ? fmaf(s[j], a.scale, was.x[j]) : s[j] * a.scale;
-    o.store(dx + (int64_t)r * a.width);
+    for (int j = 0; j < VEC; ++j) o.x[j] = a.accumulate ? fmaf(sum[j], a.scale, old.x[j]) : sum[j] * a.scale;
+    o.store(dx + (int64_t)row * a.width);
   };
   auto keep = [&] {
 #pragma unroll
     for (int j = 0; j < VEC; ++j) parts[warp][j * 32 + lane] = sum[j];
   };
-  bool through_w = false;
   if (from < a.n) {
-    before = from ? a.sorted[from - 1].x : rows;
-    behind = to < a.n ? a.sorted[to].x : rows;
-    bool first = true;
-    for (int64_t i0 = from; i0 < to; i0 += 32) {
-      const uint2 mine = i0 + lane < to ? a.sorted[i0 + lane] : make_uint2(rows, 0);
-      const int count = (int)min((int64_t)32, to - i0);
-      for (int q0 = 0; q0 < count; q0 += kSumUnroll) {
-        if (__shfl_sync(0xffffffffu, mine.x, q0) >= rows) break;
-        uint32_t r[kSumUnroll];
-        typename Group<T, VEC>::W g[kSumUnroll];
+    if (from) before = a.sorted[from - 1].x;
+    if (to < a.n) behind = a.sorted[to].x;
+    int count = 0;  // tokens that count: those that do not are behind all others
 #pragma unroll
-        for (int u = 0; u < kSumUnroll; ++u) {
-          r[u] = __shfl_sync(0xffffffffu, mine.x, q0 + u);
-          const uint32_t at = __shfl_sync(0xffffffffu, mine.y, q0 + u);
-          // without a condition, or the loads would wait for one another: what does not count is loaded all the same
-          g[u] = *reinterpret_cast<const typename Group<T, VEC>::W*>(dy + (int64_t)at * a.width);
-        }
-#pragma unroll
-        for (int u = 0; u < kSumUnroll; ++u) {
-          if (r[u] >= rows) break;  // behind the last token that counts
-          if (first) {
-            begin(r[u]);
-            first = false;
-          } else if (r[u] != row) {
-            if (row == before) keep();
-            else put(sum, old, row);
-            begin(r[u]);
-          }
-          float x[VEC];
-          Group<T, VEC>::unpack(g[u], x);
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) sum[j] += x[j];
-        }
-      }
+    for (int i0 = 0; i0 < kMostRun; i0 += 32) {
+      const uint2 t = from + i0 + lane < to ? a.sorted[from + i0 + lane] : make_uint2(rows, 0);
+      tokens[warp][i0 + lane] = t;
+      count += __popc(__ballot_sync(0xffffffffu, t.x < rows));
     }
-    // the last row: of this warp alone, begun before it, or going on behind it
+    __syncwarp();
+    first = tokens[warp][0].x;
+    auto ask = [&](int i, W* at) {
+#pragma unroll
+      for (int u = 0; u < kSumBatch; ++u)
+        if (i + u < count) copy_lane<sizeof(W)>(at + u * 32, dy + (int64_t)tokens[warp][i + u].y * a.width);
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    W* place = &ring[warp][0][lane];
+#pragma unroll
+    for (int b = 0; b < kSumAhead; ++b) ask(b * kSumBatch, place + b * kSumBatch * 32);
+    for (int i = 0; i < count; i += kSumBatch) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(kSumAhead - 1) : "memory");
+#pragma unroll
+      for (int u = 0; u < kSumBatch; ++u) {
+        if (i + u >= count) break;
+        const uint32_t r = tokens[warp][i + u].x;
+        if (r != row) {
+          if (row < rows) {
+            if (row == before) keep();
+            else put();
+          }
+          row = r;
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) sum[j] = 0.f;
+          if (a.accumulate && here && row != before) old.load(dx + (int64_t)row * a.width);
+        }
+        float x[VEC];
+        Group<T, VEC>::unpack(place[u * 32], x);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) sum[j] += x[j];
+      }
+      ask(i + kSumRing, place);
+      place = place == &ring[warp][kSumRing - kSumBatch][lane] ? &ring[warp][0][lane] : place + kSumBatch * 32;
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    // the last row: begun before this warp, going on behind it, or of this warp alone
     if (row < rows) {
-      through_w = row == before && row == behind && row == a.sorted[from].x;
       if (row == before) keep();
-      else if (row != behind) put(sum, old, row);
+      else if (row != behind) put();
     }
   }
-  if (lane == 0) through[warp] = through_w;
-  const bool starts = row < rows && row != before && row == behind;   // a row goes on behind this warp
-  const uint32_t head = warp == 0 && from < a.n ? a.sorted[from].x : rows;
-  const bool enters = head < rows && head == before;                  // a row began before this chunk
+  if (lane == 0) through[warp] = row < rows && row == before && row == behind && row == first;
+  const bool starts = row < rows && row != before && row == behind;  // a row goes on behind this warp
+  const bool enters = warp == 0 && first < rows && first == before;  // a row began before this chunk
   __syncthreads();
-  if (!(starts || enters)) return;
-  // warp 0 may see to two rows: the one that began before the chunk, and one that begins with it
   auto follow = [&](int w) {  // adds the parts of warps w, w + 1, ... as far as the row goes on; whether it leaves the chunk
     for (; w < kSumWarps; ++w) {
 #pragma unroll
@@ -345,10 +387,10 @@ __global__ void __launch_bounds__(kSumThreads) embedding_sum_kernel(SumArgs a) {
     g.store(a.partial + (chunk * 2 + slot) * a.stride + col);
   };
   if (starts) {
-    if (warp == kSumWarps - 1 || follow(warp + 1)) put_partial(1);
-    else put(sum, old, row);
+    if (follow(warp + 1)) put_partial(1);
+    else put();
   }
-  if (enters) {
+  if (enters) {  // warp 0 may see to this row and to another one that begins with it
 #pragma unroll
     for (int j = 0; j < VEC; ++j) sum[j] = 0.f;
     follow(0);
@@ -426,8 +468,8 @@ static bool range_overflows(int64_t a, int64_t b) {
 
 // Tokens of a warp: many of them cut fewer rows, few of them give every SM four blocks.
 static int warp_tokens(int64_t n, int64_t width) {
-  const int64_t tiles = (width + 255) / 256, want = n * tiles / (148 * 4 * kSumWarps) / kSumUnroll * kSumUnroll;
-  return (int)std::min<int64_t>(std::max<int64_t>(want, kSumUnroll), 128);
+  const int64_t tiles = (width + 255) / 256, want = n * tiles / (148 * 4 * kSumWarps) / 8 * 8;
+  return (int)std::min<int64_t>(std::max<int64_t>(want, 8), kMostRun);
 }
 
 static size_t round_up(size_t x) { return (x + 255) & ~size_t(255); }
@@ -513,6 +555,7 @@ int rafb200_embedding_dx(const void* dy, int dy_dtype, const void* indices, int 
     const int64_t each = (int64_t)kSortBlocks * kSortThreads * 64;  // four stores a thread
     const unsigned clusters = 1 + (unsigned)std::min<int64_t>((so.fill_bytes + each - 1) / each, kFillClusters);
     if (const int rc = allow_smem<embedding_sort_kernel>(kSortSmem)) return rc;
+    if (const int rc = allow_large_cluster<embedding_sort_kernel>()) return rc;
     RAFB200_CUDA(launch_cluster(embedding_sort_kernel, kSortBlocks, clusters * kSortBlocks, kSortThreads, kSortSmem, s, so));
   }
   if (n == 0) return RAFB200_OK;
@@ -538,8 +581,11 @@ int rafb200_embedding_dx(const void* dy, int dy_dtype, const void* indices, int 
     using O = decltype(o);
     const int rc = with_type(dy_dtype, [&](auto t) {
       return with_width<decltype(t)>(vec, [&](auto w) {
-        RAFB200_CUDA(launch_dependent(embedding_sum_kernel<decltype(t), O, decltype(w)::value>, dim3((unsigned)grid), kSumThreads,
-                                      0, s, a));
+        using T = decltype(t);
+        constexpr int kVec = decltype(w)::value;
+        constexpr size_t smem = sizeof(SumShared<typename Group<T, kVec>::W, kVec>);
+        if (const int rc = allow_smem<embedding_sum_kernel<T, O, kVec>>(smem)) return rc;
+        RAFB200_CUDA(launch_dependent(embedding_sum_kernel<T, O, kVec>, dim3((unsigned)grid), kSumThreads, smem, s, a));
         return (int)RAFB200_OK;
       });
     });

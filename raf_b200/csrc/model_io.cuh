@@ -174,6 +174,18 @@ inline int allow_smem(size_t bytes) {
   return RAFB200_OK;
 }
 
+// Lets the kernel run in clusters of 16 blocks.
+template <auto kKernel>
+inline int allow_large_cluster() {
+  static std::atomic<bool> granted[64];
+  int device = 0;
+  RAFB200_CUDA(cudaGetDevice(&device));
+  if (device < 64 && granted[device].load(std::memory_order_relaxed)) return RAFB200_OK;
+  RAFB200_CUDA(cudaFuncSetAttribute(kKernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+  if (device < 64) granted[device].store(true, std::memory_order_relaxed);
+  return RAFB200_OK;
+}
+
 // Calls f with a value of the element type of a dtype code (checked before).
 template <typename F>
 int with_type(int dtype, const F& f) {
