@@ -7,45 +7,50 @@ namespace rafb200 {
 
 // ---- lookup -----------------------------------------------------------------------
 //   out[n, :] = scale * x[id_n, :], a row of zeros where id_n is outside [0, rows)
-// Bound: HBM, the rows read and the rows written.  2^tpr_log threads share a row, so that no element needs a division,
-// and a thread has kLookupRows rows in flight: the load of a row waits for that of its id.
+// Bound: HBM, the rows read and the rows written.  A warp takes kLookupRows rows, whose ids it knows from one load, and has
+// kLookupUnroll accesses of 32 lanes in flight.  65536 rows of 1024 in bf16: XXX us, XXX TB/s.
 constexpr int kLookupThreads = 256;
-constexpr int kLookupRows = 4;
+constexpr int kLookupRows = 2;
+
+template <typename T, typename O, int VEC, int COUNT>
+__device__ __forceinline__ void lookup_groups(const T* from, O* to, int64_t left, float scale) {
+  typename Group<T, VEC>::W w[COUNT];
+  // without a condition, or the loads would wait for one another: behind the row's end its last group again
+#pragma unroll
+  for (int u = 0; u < COUNT; ++u)
+    w[u] = *reinterpret_cast<const typename Group<T, VEC>::W*>(from + min((int64_t)u * 32 * VEC, left));
+#pragma unroll
+  for (int u = 0; u < COUNT; ++u) {
+    Group<O, VEC> o;
+    Group<T, VEC>::unpack(w[u], o.x);
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) o.x[j] *= scale;
+    if (u * 32 * VEC <= left) o.store(to + u * 32 * VEC);
+  }
+}
 
 template <typename T, typename O, int VEC>
 __global__ void __launch_bounds__(kLookupThreads)
-    embedding_kernel(const T* x, Ids ids, int64_t n, int64_t rows, int64_t width, float scale, O* out,
-                     int tpr_log) {
+    embedding_kernel(const T* x, Ids ids, int64_t n, int64_t rows, int64_t width, float scale, O* out) {
+  constexpr int kUnroll = VEC == 1 ? 8 : 4;
   grid_dependency_trigger();
   grid_dependency_wait();
-  const int tpr = 1 << tpr_log, per = kLookupThreads >> tpr_log;
-  const int64_t row0 = (int64_t)blockIdx.x * per * kLookupRows + (threadIdx.x >> tpr_log);
+  const int lane = threadIdx.x & 31;
+  const int64_t first = ((int64_t)blockIdx.x * (kLookupThreads / 32) + (threadIdx.x >> 5)) * kLookupRows;
   int64_t id[kLookupRows];
 #pragma unroll
-  for (int u = 0; u < kLookupRows; ++u) {
-    const int64_t row = row0 + u * per;
-    id[u] = row < n ? ids[row] : -1;
-  }
-  for (int64_t c = (int64_t)(threadIdx.x & (tpr - 1)) * VEC; c < width; c += (int64_t)tpr * VEC) {
-    Group<T, VEC> g[kLookupRows];
+  for (int r = 0; r < kLookupRows; ++r) id[r] = first + r < n ? ids[first + r] : -1;
 #pragma unroll
-    for (int u = 0; u < kLookupRows; ++u) {
-      if ((uint64_t)id[u] < (uint64_t)rows) {
-        g[u].load(x + id[u] * width + c);
-      } else {
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) g[u].x[j] = 0.f;
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < kLookupRows; ++u) {
-      const int64_t row = row0 + u * per;
-      if (row < n) {
-        Group<O, VEC> o;
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) o.x[j] = g[u].x[j] * scale;
-        o.store(out + row * width + c);
-      }
+  for (int r = 0; r < kLookupRows; ++r) {
+    if (first + r >= n) return;
+    O* to = out + (first + r) * width;
+    if ((uint64_t)id[r] < (uint64_t)rows) {
+      const T* from = x + id[r] * width;
+      for (int64_t c = (int64_t)lane * VEC; c < width; c += 32 * VEC * kUnroll)
+        lookup_groups<T, O, VEC, kUnroll>(from + c, to + c, width - VEC - c, scale);
+    } else {
+      Group<O, VEC> zero{};
+      for (int64_t c = (int64_t)lane * VEC; c < width; c += 32 * VEC) zero.store(to + c);
     }
   }
 }
@@ -131,7 +136,7 @@ __global__ void __launch_bounds__(kSortThreads) embedding_sort_kernel(SortArgs a
                (int64_t)(gridDim.x - kSortBlocks) * kSortThreads);
     return;
   }
-  cluster_arrive();  // all blocks of the cluster run before one stores into another's shared memory
+  cluster_arrive_relaxed();  // all blocks of the cluster run before one stores into another's shared memory
   const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rank = cluster_rank(), n = (uint32_t)a.n;
   const uint32_t each = ((n + kSortBlocks * kSortWarps - 1) / (kSortBlocks * kSortWarps) + 31) & ~31u;
   const uint32_t from = (uint32_t)min((uint64_t)(rank * kSortWarps + warp) * each, (uint64_t)n), to = min(n - from, each) + from;
@@ -145,24 +150,47 @@ __global__ void __launch_bounds__(kSortThreads) embedding_sort_kernel(SortArgs a
     uint2* dst = ((a.passes - pass) & 1) ? a.a : a.b;
     uint2 pair[kSortItems];
     uint32_t place[kSortItems];  // the digit, and the rank among the warp's pairs of this digit << kDigitBits
-    auto load = [&](uint32_t i0) {  // of every 32 pairs from i0 on this lane's
+    auto load = [&](uint32_t i0) {  // of every 32 pairs from i0 on this lane's; all loads before the first is looked at
+      const uint32_t last = to - 1;
+      if (pass) {
 #pragma unroll
-      for (int u = 0; u < kSortItems; ++u) {
-        const uint32_t i = i0 + u * 32 + lane;
-        if (i < to) pair[u] = pass ? __ldcg(src + i) : make_uint2(a.key(a.ids[i]), i);
+        for (int u = 0; u < kSortItems; ++u) pair[u] = __ldcg(src + min(i0 + u * 32 + lane, last));
+      } else {
+        int64_t id[kSortItems];
+#pragma unroll
+        for (int u = 0; u < kSortItems; ++u) id[u] = a.ids[min(i0 + u * 32 + lane, last)];
+#pragma unroll
+        for (int u = 0; u < kSortItems; ++u) pair[u] = make_uint2(a.key(id[u]), i0 + u * 32 + lane);
       }
     };
+    // The lanes whose digit is this lane's, from one vote for each bit: 30 instructions, where __match_any_sync took 150 cycles
+    // of a warp's time with 32 different digits.  Lanes without a pair have a digit of their own.
+    auto equals = [&](uint32_t d) {
+      uint32_t same = 0xffffffffu;
+#pragma unroll
+      for (int b = 0; b <= kDigitBits; ++b) {
+        if (b > a.bits) break;
+        const uint32_t vote = __ballot_sync(0xffffffffu, d >> b & 1);
+        same &= d >> b & 1 ? vote : ~vote;
+      }
+      return same;
+    };
     auto count = [&](uint32_t i0) {  // ranks below 2^23: a warp's range, 2^31 / 512 pairs at most
+      uint32_t same[kSortItems];
 #pragma unroll
       for (int u = 0; u < kSortItems; ++u) {
         if (i0 + u * 32 >= to) break;
-        const bool in = i0 + u * 32 + lane < to;
-        const uint32_t d = in ? (pair[u].x >> shift) & (digits - 1) : digits, same = __match_any_sync(0xffffffffu, d);
-        const uint32_t below = __popc(same & lower_lanes);
+        place[u] = i0 + u * 32 + lane < to ? (pair[u].x >> shift) & (digits - 1) : digits;
+        same[u] = equals(place[u]);
+      }
+#pragma unroll
+      for (int u = 0; u < kSortItems; ++u) {
+        if (i0 + u * 32 >= to) break;
+        const uint32_t d = place[u], below = __popc(same[u] & lower_lanes);
         uint32_t old = 0;
-        if (in) old = mine[d];
+        if (d < digits) old = mine[d];
         __syncwarp();
-        if (in && below == 0) mine[d] = old + __popc(same);
+        if (d < digits && below == 0) mine[d] = old + __popc(same[u]);
         __syncwarp();
         place[u] = d | (old + below) << kDigitBits;
       }
@@ -229,7 +257,7 @@ __global__ void __launch_bounds__(kSortThreads) embedding_sort_kernel(SortArgs a
         for (int u = 0; u < kSortItems; ++u) {
           if (i0 + u * 32 >= to) break;
           const bool in = i0 + u * 32 + lane < to;
-          const uint32_t d = in ? (pair[u].x >> shift) & (digits - 1) : digits, same = __match_any_sync(0xffffffffu, d);
+          const uint32_t d = in ? (pair[u].x >> shift) & (digits - 1) : digits, same = equals(d);
           const uint32_t below = __popc(same & lower_lanes);
           uint32_t old = 0;
           if (in) old = mine[d];
@@ -262,7 +290,7 @@ constexpr int kSumThreads = 32 * kSumWarps;
 constexpr int kSumBatch = 4;                  // rows asked for together
 constexpr int kSumAhead = 3;                  // batches on their way
 constexpr int kSumRing = kSumBatch * kSumAhead;
-constexpr int kMostRun = 64;                  // tokens of a warp, at most
+constexpr int kMostRun = 128;                 // tokens of a warp, at most
 
 // Copies BYTES of one lane to shared memory: asynchronously where the hardware does (16, 8 or 4 bytes).
 template <int BYTES>
@@ -319,8 +347,7 @@ __global__ void __launch_bounds__(kSumThreads, 3) embedding_sum_kernel(SumArgs a
     if (from) before = a.sorted[from - 1].x;
     if (to < a.n) behind = a.sorted[to].x;
     int count = 0;  // tokens that count: those that do not are behind all others
-#pragma unroll
-    for (int i0 = 0; i0 < kMostRun; i0 += 32) {
+    for (int i0 = 0; i0 < a.run; i0 += 32) {
       const uint2 t = from + i0 + lane < to ? a.sorted[from + i0 + lane] : make_uint2(rows, 0);
       tokens[warp][i0 + lane] = t;
       count += __popc(__ballot_sync(0xffffffffu, t.x < rows));
@@ -416,10 +443,16 @@ __global__ void __launch_bounds__(kJoinThreads) embedding_join_kernel(SumArgs a)
   const int64_t col = (int64_t)blockIdx.y * kJoinCols + lane * 4;
   const float* at = a.partial + col;
   float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+  int64_t end = chunk + 1;  // the first chunk that does not begin with the row
+  for (uint32_t all = 0xffffffffu; all == 0xffffffffu;) {
+    const int64_t c = end + lane;
+    all = __ballot_sync(0xffffffffu, c * tokens < a.n && a.sorted[c * tokens].x == row);
+    end += __popc(all);
+  }
   if (col < a.width) {
     if (warp == 0) sum = *reinterpret_cast<const float4*>(at + (chunk * 2 + 1) * a.stride);
 #pragma unroll 4
-    for (int64_t c = chunk + 1 + warp; c * tokens < a.n && a.sorted[c * tokens].x == row; c += kJoinThreads / 32) {
+    for (int64_t c = chunk + 1 + warp; c < end; c += kJoinThreads / 32) {
       const float4 p = *reinterpret_cast<const float4*>(at + c * 2 * a.stride);
       sum.x += p.x;
       sum.y += p.y;
@@ -466,10 +499,11 @@ static bool range_overflows(int64_t a, int64_t b) {
   return __builtin_mul_overflow(a, b, &r) || r > ((int64_t)1 << 60);
 }
 
-// Tokens of a warp: many of them cut fewer rows, few of them give every SM four blocks.
+// Tokens of a warp: as many as give every SM its three blocks once.  Many of them cut fewer rows.
 static int warp_tokens(int64_t n, int64_t width) {
-  const int64_t tiles = (width + 255) / 256, want = n * tiles / (148 * 4 * kSumWarps) / 8 * 8;
-  return (int)std::min<int64_t>(std::max<int64_t>(want, 8), kMostRun);
+  const int64_t tiles = (width + 255) / 256, warps = 148 * 3 * kSumWarps;
+  const int64_t want = (n * tiles + warps * kSumBatch - 1) / (warps * kSumBatch) * kSumBatch;
+  return (int)std::min<int64_t>(std::max<int64_t>(want, 2 * kSumBatch), kMostRun);
 }
 
 static size_t round_up(size_t x) { return (x + 255) & ~size_t(255); }
@@ -489,9 +523,7 @@ int rafb200_embedding(const void* x, int x_dtype, int64_t rows, int64_t width, c
   if (n == 0 || width == 0) return RAFB200_OK;
   RAFB200_REQUIRE(indices && out && (x || rows == 0), "rafb200_embedding: NULL argument");
   const int vec = group_width(x, dtype_size(x_dtype), out, dtype_size(out_dtype), width);
-  int tpr_log = 5;
-  while (tpr_log < 8 && ((int64_t)1 << tpr_log) * vec < width) ++tpr_log;
-  const int64_t per_block = (int64_t)(kLookupThreads >> tpr_log) * kLookupRows, grid = (n + per_block - 1) / per_block;
+  const int64_t per_block = kLookupThreads / 32 * kLookupRows, grid = (n + per_block - 1) / per_block;
   RAFB200_REQUIRE(grid < ((int64_t)1 << 31), "rafb200_embedding: too many indices");
   const Ids ids{indices, index_dtype == RAFB200_I64};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -501,7 +533,7 @@ int rafb200_embedding(const void* x, int x_dtype, int64_t rows, int64_t width, c
         using T = decltype(t);
         using O = decltype(o);
         RAFB200_CUDA(launch_dependent(embedding_kernel<T, O, decltype(w)::value>, dim3((unsigned)grid), kLookupThreads, 0, s,
-                                      static_cast<const T*>(x), ids, n, rows, width, scale, static_cast<O*>(out), tpr_log));
+                                      static_cast<const T*>(x), ids, n, rows, width, scale, static_cast<O*>(out)));
         return (int)RAFB200_OK;
       });
     });
