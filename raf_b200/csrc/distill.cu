@@ -502,8 +502,8 @@ template <int WARPS>
 struct Exchange {
   float tops[WARPS];
   float2 sums[WARPS];
-  Running whole;
-  float some;    // sum of the teacher's weights - 1
+  Running part[8];  // of the cluster's blocks
+  float some;       // sum of the teacher's weights - 1
   float4 stats;
 };
 
@@ -542,19 +542,22 @@ __device__ __forceinline__ float4 join(Exchange<NT / 32>& x, Running run, const 
     run.hard += x.sums[w].y;
   }
   if (a.slices_log) {
-    if (threadIdx.x == 0) x.whole = run;
-    cluster_sync();
-    Running all{-INFINITY, 0.f, 0.f};
-    for (int r = 0; r >> a.slices_log == 0; ++r) all.top = fmaxf(all.top, __uint_as_float(cluster_load(&x.whole.top, r)));
-    for (int r = 0; r >> a.slices_log == 0; ++r) {
-      Running part{__uint_as_float(cluster_load(&x.whole.top, r)), __uint_as_float(cluster_load(&x.whole.soft, r)),
-                   S != kNone ? __uint_as_float(cluster_load(&x.whole.hard, r)) : 0.f};
-      rebase<S>(part, all.top, a.c);
-      all.soft += part.soft;
-      all.hard += part.hard;
+    cluster_wait();  // every block of the cluster runs
+    if (threadIdx.x < 1u << a.slices_log) {
+      Running* to = &x.part[blockIdx.x & ((1 << a.slices_log) - 1)];
+      cluster_store(&to->top, threadIdx.x, __float_as_uint(run.top));
+      cluster_store(&to->soft, threadIdx.x, __float_as_uint(run.soft));
+      cluster_store(&to->hard, threadIdx.x, __float_as_uint(run.hard));
     }
-    run = all;
-    cluster_sync();  // read by all before one of them overwrites its logits, joins its next row or ends
+    cluster_sync();  // nothing of another block is looked at from here on
+    for (int r = 0; r >> a.slices_log == 0; ++r) top = fmaxf(top, x.part[r].top);
+    run = Running{top, 0.f, 0.f};
+    for (int r = 0; r >> a.slices_log == 0; ++r) {
+      Running part = x.part[r];
+      rebase<S>(part, top, a.c);
+      run.soft += part.soft;
+      run.hard += part.hard;
+    }
   }
   return make_float4(run.top, run.soft, S != kNone ? run.hard : run.soft, x.some);
 }
@@ -602,6 +605,7 @@ __global__ void __launch_bounds__(NT + 32, kSweepThreads / NT) distill_kernel(Di
     if (tid < NT) leave_out<T, NT, GRAD>(a, row, slice);
     return;
   }
+  if (a.slices_log) cluster_arrive_relaxed();
   const T* z = static_cast<const T*>(a.pred) + row * a.ld;
   T* out = static_cast<T*>(a.out) + row * a.ld_out;
   const Slice<T> s(z, (int)a.v, slice, a.slices_log);
@@ -615,7 +619,7 @@ __global__ void __launch_bounds__(NT + 32, kSweepThreads / NT) distill_kernel(Di
     __syncwarp();
     bar_arrive<NT + 32>(kWeighed);
     if (a.slices_log) {
-      cluster_sync();
+      cluster_wait();
       cluster_sync();
     }
     bar_sync<NT + 32>(kWritten);

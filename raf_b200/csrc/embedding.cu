@@ -123,12 +123,13 @@ constexpr int kSortItems = 8;  // pairs of a lane in registers
 constexpr int kDigitBits = 9;  // two passes for tables of up to 2^18 - 1 rows; the counters of 32 warps take 64 KB
 constexpr int kDigits = 1 << kDigitBits;
 constexpr int kFillClusters = 15;
-constexpr size_t kSortSmem = sizeof(uint32_t) * (kSortWarps * kDigits + kSortBlocks * kDigits + 32);
+constexpr size_t kSortSmem = sizeof(uint32_t) * (kSortWarps * kDigits + (kSortBlocks + 2) * kDigits + 32);
 
 __global__ void __launch_bounds__(kSortThreads) embedding_sort_kernel(SortArgs a) {
   extern __shared__ uint32_t counts[];  // [warp][digit]
   uint32_t* totals = counts + kSortWarps * kDigits;  // [block][digit]
-  uint32_t* scan = totals + kSortBlocks * kDigits;
+  uint32_t* halves = totals + kSortBlocks * kDigits;  // [half of the warps][digit]
+  uint32_t* scan = halves + 2 * kDigits;
   grid_dependency_trigger();
   grid_dependency_wait();
   if (blockIdx.x >= kSortBlocks) {
@@ -209,21 +210,29 @@ __global__ void __launch_bounds__(kSortThreads) embedding_sort_kernel(SortArgs a
     }
     __syncthreads();
     if (pass == 0) cluster_wait();
-    uint32_t sum = 0, c[kSortWarps];
-    if (tid < digits) {
+    // two threads a digit, each for half of the warps
+    const uint32_t digit = tid & (kDigits - 1), half = tid / kDigits;
+    uint32_t* column = counts + half * (kSortWarps / 2) * kDigits + digit;
+    uint32_t sum = 0, c[kSortWarps / 2];
+    if (digit < digits) {
 #pragma unroll
-      for (int w = 0; w < kSortWarps; ++w) c[w] = counts[w * kDigits + tid];
+      for (int w = 0; w < kSortWarps / 2; ++w) c[w] = column[w * kDigits];
 #pragma unroll
-      for (int w = 0; w < kSortWarps; ++w) sum += c[w];
+      for (int w = 0; w < kSortWarps / 2; ++w) sum += c[w];
+      halves[half * kDigits + digit] = sum;
+    }
+    __syncthreads();
+    if (digit < digits) {
+      const uint32_t all = halves[digit] + halves[kDigits + digit];
 #pragma unroll
-      for (uint32_t r = 0; r < kSortBlocks; ++r) cluster_store(totals + rank * kDigits + tid, r, sum);
+      for (uint32_t r = 0; r < kSortBlocks / 2; ++r) cluster_store(totals + rank * kDigits + digit, half * (kSortBlocks / 2) + r, all);
     }
     cluster_sync();
     uint32_t before = 0, all = 0;  // of this thread's digit: in the blocks before this one, in all of them
-    if (tid < digits) {
+    if (digit < digits) {
 #pragma unroll
       for (uint32_t r = 0; r < kSortBlocks; ++r) {
-        const uint32_t t = totals[r * kDigits + tid];
+        const uint32_t t = totals[r * kDigits + digit];
         if (r < rank) before += t;
         all += t;
       }
@@ -236,14 +245,14 @@ __global__ void __launch_bounds__(kSortThreads) embedding_sort_kernel(SortArgs a
     }
     if (lane == 31) scan[warp] = incl;
     __syncthreads();
-    if (tid < digits) {
-      uint32_t at = incl - all + before;
+    if (digit < digits) {
+      uint32_t at = incl - all + before + (half ? halves[digit] : 0);
 #pragma unroll
       for (uint32_t w = 0; w < kDigits / 32; ++w)
-        if (w < warp) at += scan[w];
+        if (w < warp % (kDigits / 32)) at += scan[w];
 #pragma unroll
-      for (int w = 0; w < kSortWarps; ++w) {
-        counts[w * kDigits + tid] = at;
+      for (int w = 0; w < kSortWarps / 2; ++w) {
+        column[w * kDigits] = at;
         at += c[w];
       }
     }
@@ -268,7 +277,8 @@ __global__ void __launch_bounds__(kSortThreads) embedding_sort_kernel(SortArgs a
         }
       }
     }
-    cluster_sync();  // the pairs are written for all, and no block stores totals or counts before all have read theirs
+    // the pairs are written for all, and no block stores totals before all have read theirs
+    if (pass + 1 < a.passes) cluster_sync();
   }
 }
 
