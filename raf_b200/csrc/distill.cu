@@ -206,15 +206,21 @@ __device__ __forceinline__ void copy_wait() {
 }
 
 // The teacher's entries of a row in shared memory: class (-1: absent), weight p, its logarithm of base 2, student's logit
-// there.  Entry k is the label, with weight 0.
+// there.  Entry k is the label, with weight 0.  Behind them a table of 2^table_log classes, more than there are entries.
 struct Entries {
   int* at;
   float* p;
   float* log_p;
   float* z;
+  int* table;
   __device__ __forceinline__ Entries(void* smem, int k)
-      : at(static_cast<int*>(smem)), p(reinterpret_cast<float*>(at + k + 1)), log_p(p + k + 1), z(log_p + k + 1) {}
-  static __host__ __device__ __forceinline__ size_t bytes(int k) { return (size_t)(k + 1) * 16; }
+      : at(static_cast<int*>(smem)), p(reinterpret_cast<float*>(at + k + 1)), log_p(p + k + 1), z(log_p + k + 1), table(reinterpret_cast<int*>(z + k + 1)) {}
+  static __host__ __device__ __forceinline__ int table_log(int k) {
+    int log = 5;
+    while (1 << log < k + k / 4 + 2) ++log;
+    return log;
+  }
+  static __host__ __device__ __forceinline__ size_t bytes(int k) { return (size_t)(k + 1) * 16 + ((size_t)4 << table_log(k)); }
 };
 
 // softmax over the present entries, whose logits p holds before; returns the sum of the weights, 1 or 0 (or NaN).  One warp.
@@ -349,6 +355,17 @@ struct Stream {
   }
 };
 
+template <typename T, Second S>
+__device__ __forceinline__ uint4 gradient_of(const uint4& raw, const Coefficients& co) {
+  if constexpr (sizeof(T) == 4) {
+    const Two a = co.at<S>(Raw<T>::pair(raw, 0)), b = co.at<S>(Raw<T>::pair(raw, 1));
+    return make_uint4(__float_as_uint(a.lo()), __float_as_uint(a.hi()), __float_as_uint(b.lo()), __float_as_uint(b.hi()));
+  } else {
+    return make_uint4(Raw<T>::put(co.at<S>(Raw<T>::pair(raw, 0))), Raw<T>::put(co.at<S>(Raw<T>::pair(raw, 1))),
+                      Raw<T>::put(co.at<S>(Raw<T>::pair(raw, 2))), Raw<T>::put(co.at<S>(Raw<T>::pair(raw, 3))));
+  }
+}
+
 // The gradient of COUNT groups, NT apart; `from` holds the bytes of the first.
 template <typename T, Second S, int NT, int Q, int COUNT>
 __device__ __forceinline__ void write_groups(const char* from, uint32_t bits, uint4* to, const Coefficients& co) {
@@ -356,17 +373,7 @@ __device__ __forceinline__ void write_groups(const char* from, uint32_t bits, ui
 #pragma unroll
   for (int u = 0; u < COUNT; ++u) raw[u] = load_shifted<Q>(from + u * NT * 16, bits);
 #pragma unroll
-  for (int u = 0; u < COUNT; ++u) {
-    uint4 r;
-    if constexpr (sizeof(T) == 4) {
-      const Two a = co.at<S>(Raw<T>::pair(raw[u], 0)), b = co.at<S>(Raw<T>::pair(raw[u], 1));
-      r = make_uint4(__float_as_uint(a.lo()), __float_as_uint(a.hi()), __float_as_uint(b.lo()), __float_as_uint(b.hi()));
-    } else {
-      r = make_uint4(Raw<T>::put(co.at<S>(Raw<T>::pair(raw[u], 0))), Raw<T>::put(co.at<S>(Raw<T>::pair(raw[u], 1))),
-                     Raw<T>::put(co.at<S>(Raw<T>::pair(raw[u], 2))), Raw<T>::put(co.at<S>(Raw<T>::pair(raw[u], 3))));
-    }
-    to[u * NT] = r;
-  }
+  for (int u = 0; u < COUNT; ++u) to[u * NT] = gradient_of<T, S>(raw[u], co);
 }
 // A batch of them, `left` from the first on: the rest together, for one wait for memory.
 template <typename T, Second S, int NT, int Q>
@@ -385,62 +392,92 @@ __device__ __forceinline__ bool alike(const T* z, const T* out) {
 
 // The gradient of a slice of z.  `edge` is this thread's element outside the groups.
 template <typename T, Second S, int NT, int Q>
-__device__ __forceinline__ void write_batches(const Slice<T>& s, const T* z, T* out, const Coefficients& co) {
+__device__ __forceinline__ void write_batches(const Slice<T>& s, const T* z, T* out, const Coefficients& co, int tid) {
   const char* from = reinterpret_cast<const char*>(z + s.at);
   uint4* to = reinterpret_cast<uint4*>(out + s.at);
   const uint32_t bits = (reinterpret_cast<uintptr_t>(from) & 3) * 8;
-  for (int i = threadIdx.x; i < s.groups; i += kDistillUnroll * NT)
+  for (int i = tid; i < s.groups; i += kDistillUnroll * NT)
     write_batch<T, S, NT, Q>(from + (int64_t)i * 16, bits, to + i, (s.groups - i + NT - 1) / NT, co);
+}
+// The same where the gradient's groups are not those of z.
+template <typename T, Second S, int NT>
+__device__ __forceinline__ void write_shifted(const Slice<T>& in, const T* z, T* out, const Coefficients& co, int tid) {
+  const Slice<T> s = in.aligned_at(out);
+  switch ((reinterpret_cast<uintptr_t>(z + s.at) & 15) >> 2) {
+    case 0: write_batches<T, S, NT, 0>(s, z, out, co, tid); break;
+    case 1: write_batches<T, S, NT, 1>(s, z, out, co, tid); break;
+    case 2: write_batches<T, S, NT, 2>(s, z, out, co, tid); break;
+    default: write_batches<T, S, NT, 3>(s, z, out, co, tid); break;
+  }
+  if (tid < s.edges()) {
+    const int j = s.edge_at(tid);
+    out[j] = Elem<T>::from_f32(co.at<S>(Elem<T>::to_f32(z[j])));
+  }
 }
 template <typename T, Second S, int NT>
 __device__ __forceinline__ void write_slice(const Slice<T>& in, const T* z, float edge, T* out, const Coefficients& co, Stream<T, NT>& stream) {
-  if (alike(z, out)) {  // the stream has begun
-    uint4* to = reinterpret_cast<uint4*>(out + in.at);
-    stream.run([&](int i, const uint4* place, int left) {
-      write_batch<T, S, NT, -1>(reinterpret_cast<const char*>(place), 0, to + i, left, co);
-    });
-    if ((int)threadIdx.x < in.edges()) out[in.edge_at(threadIdx.x)] = Elem<T>::from_f32(co.at<S>(edge));
+  if (!alike(z, out)) {
+    write_shifted<T, S, NT>(in, z, out, co, threadIdx.x);
     return;
   }
-  const Slice<T> s = in.aligned_at(out);
-  switch ((reinterpret_cast<uintptr_t>(z + s.at) & 15) >> 2) {
-    case 0: write_batches<T, S, NT, 0>(s, z, out, co); break;
-    case 1: write_batches<T, S, NT, 1>(s, z, out, co); break;
-    case 2: write_batches<T, S, NT, 2>(s, z, out, co); break;
-    default: write_batches<T, S, NT, 3>(s, z, out, co); break;
+  uint4* to = reinterpret_cast<uint4*>(out + in.at);  // the stream has begun
+  stream.run([&](int i, const uint4* place, int left) {
+    write_batch<T, S, NT, -1>(reinterpret_cast<const char*>(place), 0, to + i, left, co);
+  });
+  if ((int)threadIdx.x < in.edges()) out[in.edge_at(threadIdx.x)] = Elem<T>::from_f32(co.at<S>(edge));
+}
+
+// Whether it is known that no class is named twice: each is put into the table, whose places are tried one after the other.  For
+// short lists write_entries() compares sooner than the table is filled (4096 rows of 1000 with 32 entries: 13.9 against
+// 15.9 us for loss and gradient).  One warp.
+__device__ __forceinline__ bool all_different(const Entries& e, int k) {
+  if (k < 64) return false;
+  const int lane = threadIdx.x & 31, log = Entries::table_log(k), places = 1 << log;
+  for (int i = lane; i < places; i += 32) e.table[i] = -1;
+  __syncwarp();
+  bool again = false;
+  for (int i = lane; i <= k; i += 32) {
+    const int j = e.at[i];
+    if (j < 0) continue;
+    uint32_t at = (uint32_t)j * 0x9E3779B1u >> (32 - log);
+    for (int tries = 0; tries < places; ++tries, at = (at + 1) & (places - 1)) {
+      const int old = atomicCAS(&e.table[at], -1, j);
+      again |= old == j;
+      if (old == -1 || old == j) break;
+    }
   }
-  if ((int)threadIdx.x < s.edges()) {
-    const int j = s.edge_at(threadIdx.x);
-    out[j] = Elem<T>::from_f32(co.at<S>(Elem<T>::to_f32(z[j])));
-  }
+  return !__any_sync(0xffffffffu, again);
 }
 
 // The elements that the teacher or the label names, once each however often they are named.  One warp.
 template <typename T, Second S>
-__device__ __forceinline__ void write_entries(const DistillArgs& a, const Entries& e, const Slice<T>& s, T* out, const Coefficients& co) {
+__device__ __forceinline__ void write_entries(const DistillArgs& a, const Entries& e, const Slice<T>& s, T* out, const Coefficients& co,
+                                              bool different) {
   for (int i = threadIdx.x & 31; i <= a.k; i += 32) {
     const int j = e.at[i];
     if (j < 0 || !s.owns(j)) continue;
-    bool again = false;
     float p = e.p[i];
-#pragma unroll 4
-    for (int q = 0; q <= a.k; ++q) {
-      if (e.at[q] != j || q == i) continue;
-      again |= q < i;
-      p += e.p[q];
+    bool hit = i == a.k, again = false;
+    if (!different) {
+      for (int q = 0; q <= a.k; ++q) {
+        if (e.at[q] != j || q == i) continue;
+        again |= q < i;
+        p += e.p[q];
+        hit |= q == a.k;
+      }
     }
     if (again) continue;
     float g = co.at<S>(e.z[i]) - co.teach * p;
-    if (e.at[a.k] == j) g -= co.hit;
+    if (hit) g -= co.hit;
     out[j] = Elem<T>::from_f32(g);
   }
 }
 
 template <typename T, int NT>
-__device__ __forceinline__ void zero_slice(const Slice<T>& s, T* out) {
+__device__ __forceinline__ void zero_slice(const Slice<T>& s, T* out, int tid) {
   uint4* to = reinterpret_cast<uint4*>(out + s.at);
-  for (int i = threadIdx.x; i < s.groups; i += NT) to[i] = make_uint4(0, 0, 0, 0);
-  if ((int)threadIdx.x < s.edges()) out[s.edge_at(threadIdx.x)] = Elem<T>::from_f32(0.f);
+  for (int i = tid; i < s.groups; i += NT) to[i] = make_uint4(0, 0, 0, 0);
+  if (tid < s.edges()) out[s.edge_at(tid)] = Elem<T>::from_f32(0.f);
 }
 
 // Running maximum and sums of a thread's groups.
@@ -465,17 +502,19 @@ struct Sweep {
       if (S != kNone) hard = hard * Two(fh, fh);
       run.top = top;
     }
+#pragma unroll
+    for (int u = 0; u < COUNT; ++u) terms(raw[u], base, c);
+  }
+  // adds the exponentials of a group
+  __device__ __forceinline__ void terms(const uint4& raw, float base, float c) {
     const Two nb(-base, -base), c2(c, c);
 #pragma unroll
-    for (int u = 0; u < COUNT; ++u) {
-#pragma unroll
-      for (int j = 0; j < Raw<T>::kPer / 2; ++j) {
-        const Two x = Raw<T>::pair(raw[u], j) + nb, p = ex2(x * c2);
-        soft = soft + p;
-        if (S == kOwn) hard = hard + ex2(x * Two(kLog2e, kLog2e));
-        if (S == kSquare) hard = fma2(p, p, hard);
-        if (S == kFourth) hard = fma2(p * p, p * p, hard);
-      }
+    for (int j = 0; j < Raw<T>::kPer / 2; ++j) {
+      const Two x = Raw<T>::pair(raw, j) + nb, p = ex2(x * c2);
+      soft = soft + p;
+      if (S == kOwn) hard = hard + ex2(x * Two(kLog2e, kLog2e));
+      if (S == kSquare) hard = fma2(p, p, hard);
+      if (S == kFourth) hard = fma2(p * p, p * p, hard);
     }
   }
   // The groups of a batch that exist, `left` of them from the first on.
@@ -577,19 +616,23 @@ __device__ __forceinline__ bool left_out(const DistillArgs& a, int64_t label) {
 }
 
 template <typename T, int NT, bool GRAD>
-__device__ __forceinline__ void leave_out(const DistillArgs& a, int64_t row, int slice) {
-  if (slice == 0 && threadIdx.x == 0) {
+__device__ __forceinline__ void leave_out(const DistillArgs& a, int64_t row, int slice, int tid) {
+  if (slice == 0 && tid == 0) {
     a.loss[row] = 0.f;
     if (a.stats) a.stats[row] = make_float4(0.f, 1.f, 1.f, -1.f);
   }
   T* out = static_cast<T*>(a.out) + row * a.ld_out;
-  if (GRAD) zero_slice<T, NT>(Slice<T>(out, (int)a.v, slice, a.slices_log), out);
+  if (GRAD) zero_slice<T, NT>(Slice<T>(out, (int)a.v, slice, a.slices_log), out, tid);
 }
 
 // Loss, and with GRAD the gradient, of a row by a cluster of 2^slices_log blocks: one pass with a running maximum and its
 // sums, joined over threads, warps and blocks.
 // GRAD reads the logits a second time, from the L2: the launch sees to it that it holds what the resident blocks work on.
-// XXX
+// 8192 rows of 50257 (bf16, T = 2, labels), loss and gradient: 319 us where gradient rows lie as the logits do, 338 us where
+// they do not (5.2 and 4.9 TB/s of what has to be read and written).  Slices kept in shared memory instead, which
+// leave room for two blocks an SM: 450 us, 590 us with the next row on its way meanwhile - 16 warps an SM are too few for
+// the arithmetic.  The loss alone, 4096 rows of 30522: 55 us (4.6 TB/s), fp32 6.0 TB/s: 16-bit logits give every byte twice the
+// arithmetic.
 template <typename T, Second S, bool GRAD, int NT>
 __global__ void __launch_bounds__(NT + 32, kSweepThreads / NT) distill_kernel(DistillArgs a) {
   extern __shared__ uint4 image[];
@@ -602,7 +645,7 @@ __global__ void __launch_bounds__(NT + 32, kSweepThreads / NT) distill_kernel(Di
   const bool labels = a.labels.p != nullptr;
   const int64_t label = labels ? a.labels[row] : -1;
   if (labels && left_out(a, label)) {  // the same for every block of the cluster
-    if (tid < NT) leave_out<T, NT, GRAD>(a, row, slice);
+    if (tid < NT) leave_out<T, NT, GRAD>(a, row, slice, tid);
     return;
   }
   if (a.slices_log) cluster_arrive_relaxed();
@@ -622,9 +665,10 @@ __global__ void __launch_bounds__(NT + 32, kSweepThreads / NT) distill_kernel(Di
       cluster_wait();
       cluster_sync();
     }
+    const bool different = GRAD && all_different(e, a.k);
     bar_sync<NT + 32>(kWritten);
     const float4 stats = exchange.stats;
-    if (GRAD) write_entries<T, S>(a, e, s, out, coefficients<S>(a, weight, stats, labels));
+    if (GRAD) write_entries<T, S>(a, e, s, out, coefficients<S>(a, weight, stats, labels), different);
     if (slice == 0) put_loss(a, e, row, stats, labels);
     return;
   }
@@ -659,7 +703,7 @@ __global__ void __launch_bounds__(kDpredThreads + 32, 6) distill_dpred_kernel(Di
   const bool labels = a.labels.p != nullptr;
   const int64_t label = labels ? a.labels[row] : -1;
   if (labels && left_out(a, label)) {
-    if (tid < NT) zero_slice<T, NT>(Slice<T>(out, (int)a.v, slice, a.slices_log), out);
+    if (tid < NT) zero_slice<T, NT>(Slice<T>(out, (int)a.v, slice, a.slices_log), out, tid);
     return;
   }
   const Slice<T> s(z, (int)a.v, slice, a.slices_log);
@@ -683,8 +727,89 @@ __global__ void __launch_bounds__(kDpredThreads + 32, 6) distill_dpred_kernel(Di
   for (int i = tid - NT; i <= a.k; i += 32) mine |= e.at[i] >= 0 && s.owns(e.at[i]);
   mine = __any_sync(0xffffffffu, mine);
   if (mine) weigh(e, a.k, a.c);
+  const bool different = mine && all_different(e, a.k);
   bar_sync<NT + 32>(kWritten);
-  if (mine) write_entries<T, S>(a, e, s, out, coefficients<S>(a, weight, stats, labels));
+  if (mine) write_entries<T, S>(a, e, s, out, coefficients<S>(a, weight, stats, labels), different);
+}
+
+// Short rows: a warp takes a row, which its registers hold from the first look to the gradient, and sees to the row's
+// entries too.  Bound by the instructions and the latency of a row's entries, for which an SM has 24 rows on their way.
+// Blocks that share a row took longer at every length that registers hold: 4096 rows of 1000 (bf16, 32 entries,
+// T = 2, labels), loss 14.3 -> 8.0 us, gradient 21.5 -> 11.5 us, both 25 -> 13.9 us; rows of 2040: 14.7 -> 9.0, 21.9 -> 12.7,
+// 26.6 -> 15.4 us.
+constexpr int kShortGroups = 8;  // of a lane
+constexpr int kShortWarps = 4;
+enum Part { kLoss, kDpred, kBoth };
+template <typename T, Second S, Part P>
+__global__ void __launch_bounds__(32 * kShortWarps, 6) distill_short_kernel(DistillArgs a) {
+  extern __shared__ uint4 image[];
+  grid_dependency_trigger();
+  grid_dependency_wait();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t row = (int64_t)blockIdx.x * kShortWarps + warp;
+  if (row >= a.n) return;
+  const Entries e(reinterpret_cast<char*>(image) + warp * Entries::bytes(a.k), a.k);
+  const T* z = static_cast<const T*>(a.pred) + row * a.ld;
+  T* out = static_cast<T*>(a.out) + row * a.ld_out;
+  const Slice<T> s(z, (int)a.v, 0, 0);
+  const uint4* source = reinterpret_cast<const uint4*>(z + s.at) + lane;
+  const uint32_t low = sizeof(T) == 4 ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;  // -infinity
+  uint4 raw[kShortGroups];
+#pragma unroll
+  for (int u = 0; u < kShortGroups; ++u) {
+    raw[u] = make_uint4(low, low, low, low);
+    if (u * 32 + lane < s.groups) raw[u] = source[u * 32];
+  }
+  const float edge = lane < s.edges() ? Elem<T>::to_f32(z[s.edge_at(lane)]) : -INFINITY;
+  const float weight = P != kLoss && a.dy ? a.dy[row * a.dy_step] : 1.f;
+  const bool labels = a.labels.p != nullptr;
+  const int64_t label = labels ? a.labels[row] : -1;
+  float4 stats = P == kDpred ? a.stats[row] : make_float4(0.f, 0.f, 0.f, 0.f);
+  load_entries(a, e, row, z, label);
+  if (labels && left_out(a, label)) {
+    if (P == kDpred) zero_slice<T, 32>(Slice<T>(out, (int)a.v, 0, 0), out, lane);
+    else leave_out<T, 32, P == kBoth>(a, row, 0, lane);
+    return;
+  }
+  const float some = weigh(e, a.k, a.c) - 1.f;
+  if (P != kDpred) {
+    uint32_t most = Raw<T>::max2(raw[0]);
+#pragma unroll
+    for (int u = 1; u < kShortGroups; ++u)
+      if (u * 32 < s.groups) most = Raw<T>::max2(most, Raw<T>::max2(raw[u]));
+    float top = fmaxf(edge, Raw<T>::max1(most));
+#pragma unroll
+    for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+    const float base = base_of(top);
+    Sweep<T, S> sweep;
+#pragma unroll
+    for (int u = 0; u < kShortGroups; ++u)
+      if (u * 32 < s.groups) sweep.terms(raw[u], base, a.c);
+    sweep.finish();
+    float soft = sweep.run.soft, hard = sweep.run.hard;
+    if (lane < s.edges()) {
+      soft += power(edge, base, a.c);
+      if (S != kNone) hard += power(edge, base, kLog2e);
+    }
+    soft = warp_sum(soft);
+    if (S != kNone) hard = warp_sum(hard);
+    stats = make_float4(top, soft, S != kNone ? hard : soft, some);
+    put_loss(a, e, row, stats, labels);
+  }
+  if (P == kLoss) return;
+  const Coefficients co = coefficients<S>(a, weight, stats, labels);
+  if (alike(z, out)) {
+    uint4* to = reinterpret_cast<uint4*>(out + s.at) + lane;
+#pragma unroll
+    for (int u = 0; u < kShortGroups; ++u)
+      if (u * 32 + lane < s.groups) to[u * 32] = gradient_of<T, S>(raw[u], co);
+    if (lane < s.edges()) out[s.edge_at(lane)] = Elem<T>::from_f32(co.at<S>(edge));
+  } else {
+    write_shifted<T, S, 32>(s, z, out, co, lane);
+  }
+  const bool different = all_different(e, a.k);
+  __syncwarp();  // what other lanes have written is overwritten
+  write_entries<T, S>(a, e, s, out, co, different);
 }
 
 static int check_args(const rafb200_distill* d, const char* who) {
@@ -741,6 +866,17 @@ static int launch_rows(const rafb200_distill* d, DistillArgs a, cudaStream_t s) 
   return RAFB200_OK;
 }
 
+// Rows of which a lane holds at most kShortGroups groups.
+static bool short_rows(const rafb200_distill* d) { return row_groups(d) <= 32 * kShortGroups; }
+
+template <typename T, Second S, Part P>
+static int launch_short(const rafb200_distill* d, const DistillArgs& a, cudaStream_t s) {
+  const size_t smem = kShortWarps * Entries::bytes(d->k);
+  if (const int rc = allow_smem<distill_short_kernel<T, S, P>>(smem)) return rc;
+  RAFB200_CUDA(launch_dependent(distill_short_kernel<T, S, P>, dim3((unsigned)((d->n + kShortWarps - 1) / kShortWarps)), 32 * kShortWarps, smem, s, a));
+  return RAFB200_OK;
+}
+
 template <typename F>
 static int with_case(const rafb200_distill* d, const F& f) {
   return with_type(d->pred_dtype, [&](auto t) {
@@ -767,6 +903,7 @@ int rafb200_distill_loss(const rafb200_distill* d, float* loss, float* stats, vo
   a.loss = loss;
   a.stats = reinterpret_cast<float4*>(stats);
   return with_case(d, [&](auto t, auto second) {
+    if (short_rows(d)) return launch_short<decltype(t), decltype(second)::value, kLoss>(d, a, static_cast<cudaStream_t>(stream));
     if (row_groups(d) >= 4096) return launch_rows<decltype(t), decltype(second)::value, false, 256>(d, a, static_cast<cudaStream_t>(stream));
     return launch_rows<decltype(t), decltype(second)::value, false, 128>(d, a, static_cast<cudaStream_t>(stream));
   });
@@ -801,6 +938,7 @@ int rafb200_distill_loss_dpred(const rafb200_distill* d, const float* dy, int dy
   return with_case(d, [&](auto t, auto second) {
     using T = decltype(t);
     constexpr Second S = decltype(second)::value;
+    if (short_rows(d)) return launch_short<T, S, kDpred>(d, a, static_cast<cudaStream_t>(stream));
     const size_t smem = Stream<T, kDpredThreads>::kPlaces * 16 + Entries::bytes(d->k);
     if (const int rc = allow_smem<distill_dpred_kernel<T, S>>(smem)) return rc;
     RAFB200_CUDA(launch_dependent(distill_dpred_kernel<T, S>, dim3((unsigned)(d->n << a.slices_log)), kDpredThreads + 32, smem,
@@ -823,6 +961,7 @@ int rafb200_distill_loss_with_dpred(const rafb200_distill* d, const float* dy, i
   a.out = dpred;
   a.ld_out = ld_dpred;
   return with_case(d, [&](auto t, auto second) {
+    if (short_rows(d)) return launch_short<decltype(t), decltype(second)::value, kBoth>(d, a, static_cast<cudaStream_t>(stream));
     if (row_groups(d) >= 2048) return launch_rows<decltype(t), decltype(second)::value, true, 256>(d, a, static_cast<cudaStream_t>(stream));
     return launch_rows<decltype(t), decltype(second)::value, true, 128>(d, a, static_cast<cudaStream_t>(stream));
   });
