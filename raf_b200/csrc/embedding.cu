@@ -29,6 +29,47 @@ __device__ __forceinline__ void lookup_groups(const T* from, O* to, int64_t left
   }
 }
 
+// Rows of one type that begin anywhere: 16 bytes written at a time, out of the two aligned 16-byte groups that hold them.
+template <typename T, int Q>
+__device__ __forceinline__ void lookup_shifted(const Slice<T>& s, const T* from, T* to, float scale, int lane) {
+  constexpr int kUnroll = 4, kPer = Slice<T>::kPer;
+  const char* source = reinterpret_cast<const char*>(from + s.at);
+  uint4* out = reinterpret_cast<uint4*>(to + s.at);
+  const uint32_t bits = (reinterpret_cast<uintptr_t>(source) & 3) * 8;
+  for (int i = lane; i < s.groups; i += 32 * kUnroll) {
+    uint4 w[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) w[u] = load_shifted<Q>(source + (int64_t)min(i + u * 32, s.groups - 1) * 16, bits);
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      float x[kPer];
+      Group<T, kPer>::unpack(w[u], x);
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) x[j] *= scale;
+      if (i + u * 32 < s.groups) out[i + u * 32] = Group<T, kPer>::pack(x);
+    }
+  }
+}
+template <typename T>
+__device__ __forceinline__ void lookup_anywhere(const T* from, T* to, int width, float scale, int lane) {
+  Slice<T> s(from, width, 0, 0);
+  if (alike(from, static_cast<const T*>(to))) {
+    lookup_shifted<T, -1>(s, from, to, scale, lane);
+  } else {
+    s = s.aligned_at(to);
+    switch ((reinterpret_cast<uintptr_t>(from + s.at) & 15) >> 2) {
+      case 0: lookup_shifted<T, 0>(s, from, to, scale, lane); break;
+      case 1: lookup_shifted<T, 1>(s, from, to, scale, lane); break;
+      case 2: lookup_shifted<T, 2>(s, from, to, scale, lane); break;
+      default: lookup_shifted<T, 3>(s, from, to, scale, lane); break;
+    }
+  }
+  if (lane < s.edges()) {
+    const int j = s.edge_at(lane);
+    to[j] = Elem<T>::from_f32(Elem<T>::to_f32(from[j]) * scale);
+  }
+}
+
 template <typename T, typename O, int VEC>
 __global__ void __launch_bounds__(kLookupThreads)
     embedding_kernel(const T* x, Ids ids, int64_t n, int64_t rows, int64_t width, float scale, O* out) {
@@ -46,6 +87,12 @@ __global__ void __launch_bounds__(kLookupThreads)
     O* to = out + (first + r) * width;
     if ((uint64_t)id[r] < (uint64_t)rows) {
       const T* from = x + id[r] * width;
+      if constexpr (std::is_same<T, O>::value && VEC < 16 / (int)sizeof(T)) {
+        if (width * (int)sizeof(T) >= 512 && width < ((int64_t)1 << 31)) {  // shorter rows leave lanes without a group
+          lookup_anywhere<T>(from, to, (int)width, scale, lane);
+          continue;
+        }
+      }
       for (int64_t c = (int64_t)lane * VEC; c < width; c += 32 * VEC * kUnroll)
         lookup_groups<T, O, VEC, kUnroll>(from + c, to + c, width - VEC - c, scale);
     } else {
@@ -91,6 +138,7 @@ __device__ void zero_bytes(unsigned char* p, int64_t bytes, int64_t worker, int6
 // memory.  No block waits for another.
 constexpr int kRankTokens = 4096;
 constexpr int kRankThreads = 256;
+constexpr int kRankLoads = 8;
 __global__ void __launch_bounds__(kRankThreads) embedding_rank_kernel(SortArgs a) {
   __shared__ uint32_t keys[kRankTokens];
   grid_dependency_trigger();
@@ -98,7 +146,14 @@ __global__ void __launch_bounds__(kRankThreads) embedding_rank_kernel(SortArgs a
   const int n = (int)a.n, tid = threadIdx.x, lane = tid & 31, warps = gridDim.x * (kRankThreads / 32);
   const int mine = blockIdx.x * (kRankThreads / 32) + (tid >> 5);
   if (blockIdx.x * (kRankThreads / 32) < n) {
-    for (int i = tid; i < n; i += kRankThreads) keys[i] = a.key(a.ids[i]);
+    for (int i0 = tid; i0 < n; i0 += kRankThreads * kRankLoads) {
+      int64_t id[kRankLoads];  // all of them asked for before the first is looked at
+#pragma unroll
+      for (int u = 0; u < kRankLoads; ++u) id[u] = a.ids[min(i0 + u * kRankThreads, n - 1)];
+#pragma unroll
+      for (int u = 0; u < kRankLoads; ++u)
+        if (i0 + u * kRankThreads < n) keys[i0 + u * kRankThreads] = a.key(id[u]);
+    }
     __syncthreads();
     for (int i = mine; i < n; i += warps) {
       const uint32_t key = keys[i];
@@ -316,7 +371,7 @@ template <typename W, int VEC>
 struct SumShared {
   W ring[kSumWarps][kSumRing][32];
   float parts[kSumWarps][32 * VEC];  // the warp's part of a row that began before it
-  uint2 tokens[kSumWarps][kMostRun];
+  uint2 tokens[kSumWarps][kMostRun + 1];
   int through[kSumWarps];            // that row takes all of the warp's tokens and goes on behind it
 };
 
@@ -339,19 +394,19 @@ __global__ void __launch_bounds__(kSumThreads, 3) embedding_sum_kernel(SumArgs a
   O* dx = static_cast<O*>(a.dx) + col;
   uint32_t row = rows, before = rows, behind = rows, first = rows;
   float sum[VEC];
-  Group<O, VEC> old;
 #pragma unroll
   for (int j = 0; j < VEC; ++j) sum[j] = 0.f;
-  auto put = [&] {
+  auto put = [&](const Group<O, VEC>& old) {
     if (!here) return;
     Group<O, VEC> o;
 #pragma unroll
     for (int j = 0; j < VEC; ++j) o.x[j] = a.accumulate ? fmaf(sum[j], a.scale, old.x[j]) : sum[j] * a.scale;
     o.store(dx + (int64_t)row * a.width);
   };
-  auto keep = [&] {
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) parts[warp][j * 32 + lane] = sum[j];
+  auto put_late = [&] {  // where what the row holds has not been asked for
+    Group<O, VEC> old{};
+    if (a.accumulate && here) old.load(dx + (int64_t)row * a.width);
+    put(old);
   };
   if (from < a.n) {
     if (from) before = a.sorted[from - 1].x;
@@ -359,9 +414,10 @@ __global__ void __launch_bounds__(kSumThreads, 3) embedding_sum_kernel(SumArgs a
     int count = 0;  // tokens that count: those that do not are behind all others
     for (int i0 = 0; i0 < a.run; i0 += 32) {
       const uint2 t = from + i0 + lane < to ? a.sorted[from + i0 + lane] : make_uint2(rows, 0);
-      tokens[warp][i0 + lane] = t;
+      if (i0 + lane < a.run) tokens[warp][i0 + lane] = t;
       count += __popc(__ballot_sync(0xffffffffu, t.x < rows));
     }
+    if (lane == 0) tokens[warp][a.run] = make_uint2(behind, 0);
     __syncwarp();
     first = tokens[warp][0].x;
     auto ask = [&](int i, W* at) {
@@ -374,34 +430,41 @@ __global__ void __launch_bounds__(kSumThreads, 3) embedding_sum_kernel(SumArgs a
 #pragma unroll
     for (int b = 0; b < kSumAhead; ++b) ask(b * kSumBatch, place + b * kSumBatch * 32);
     for (int i = 0; i < count; i += kSumBatch) {
+      uint32_t r[kSumBatch + 1];
+      Group<O, VEC> old[kSumBatch];
+#pragma unroll
+      for (int u = 0; u <= kSumBatch; ++u) r[u] = i + u <= count ? tokens[warp][i + u].x : rows;
+      if (a.accumulate && here) {  // what the rows that end in this batch hold, all of it asked for together
+#pragma unroll
+        for (int u = 0; u < kSumBatch; ++u) old[u].load(dx + (int64_t)min(r[u], rows - 1) * a.width);
+      }
       asm volatile("cp.async.wait_group %0;" ::"n"(kSumAhead - 1) : "memory");
 #pragma unroll
       for (int u = 0; u < kSumBatch; ++u) {
         if (i + u >= count) break;
-        const uint32_t r = tokens[warp][i + u].x;
-        if (r != row) {
-          if (row < rows) {
-            if (row == before) keep();
-            else put();
-          }
-          row = r;
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) sum[j] = 0.f;
-          if (a.accumulate && here && row != before) old.load(dx + (int64_t)row * a.width);
-        }
+        row = r[u];
         float x[VEC];
         Group<T, VEC>::unpack(place[u * 32], x);
 #pragma unroll
         for (int j = 0; j < VEC; ++j) sum[j] += x[j];
+        if (r[u + 1] != row) {  // the row ends here
+          if (row == before) {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) parts[warp][j * 32 + lane] = sum[j];
+          } else {
+            put(old[u]);
+          }
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) sum[j] = 0.f;
+        }
       }
       ask(i + kSumRing, place);
       place = place == &ring[warp][kSumRing - kSumBatch][lane] ? &ring[warp][0][lane] : place + kSumBatch * 32;
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
-    // the last row: begun before this warp, going on behind it, or of this warp alone
-    if (row < rows) {
-      if (row == before) keep();
-      else if (row != behind) put();
+    if (row < rows && row == behind && row == before) {  // the whole of it between the two borders
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) parts[warp][j * 32 + lane] = sum[j];
     }
   }
   if (lane == 0) through[warp] = row < rows && row == before && row == behind && row == first;
@@ -425,7 +488,7 @@ __global__ void __launch_bounds__(kSumThreads, 3) embedding_sum_kernel(SumArgs a
   };
   if (starts) {
     if (follow(warp + 1)) put_partial(1);
-    else put();
+    else put_late();
   }
   if (enters) {  // warp 0 may see to this row and to another one that begins with it
 #pragma unroll
@@ -572,6 +635,8 @@ int rafb200_embedding_dx(const void* dy, int dy_dtype, const void* indices, int 
                   "rafb200_embedding_dx: workspace smaller than rafb200_embedding_dx_workspace_bytes, or not aligned");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
 
+  const int vec = group_width(dy, dtype_size(dy_dtype), dx, dtype_size(dx_dtype), width);
+  const int64_t tiles = (width + 32 * vec - 1) / (32 * vec);
   SortArgs so{};
   so.ids = Ids{indices, index_dtype == RAFB200_I64};
   so.n = n;
@@ -602,7 +667,6 @@ int rafb200_embedding_dx(const void* dy, int dy_dtype, const void* indices, int 
   }
   if (n == 0) return RAFB200_OK;
 
-  const int vec = group_width(dy, dtype_size(dy_dtype), dx, dtype_size(dx_dtype), width);
   SumArgs a{};
   a.dy = dy;
   a.sorted = so.a;
@@ -614,7 +678,7 @@ int rafb200_embedding_dx(const void* dy, int dy_dtype, const void* indices, int 
   a.dx = dx;
   a.partial = reinterpret_cast<float*>(static_cast<char*>(workspace) + 2 * round_up((size_t)n * sizeof(uint2)));
   a.stride = (width + 7) & ~int64_t(7);
-  a.tiles = (width + 32 * vec - 1) / (32 * vec);
+  a.tiles = tiles;
   a.run = warp_tokens(n, width);
   const int64_t tokens = (int64_t)kSumWarps * a.run, chunks = (n + tokens - 1) / tokens;
   const int64_t grid = chunks * a.tiles, cols = (width + kJoinCols - 1) / kJoinCols;

@@ -115,6 +115,59 @@ struct Group {
   }
 };
 
+// ---- rows at any address ----------------------------------------------------------
+// A block's part of a row: elements [begin, end), of which `groups` groups of 16 bytes from element `at` on are aligned
+// in memory.  The row's first and last elements, which no aligned group holds, are the first and the last block's.
+template <typename T>
+struct Slice {
+  static constexpr int kPer = 16 / sizeof(T);
+  int begin, end, at, groups;
+
+  __device__ __forceinline__ Slice() {}
+  __device__ __forceinline__ Slice(const T* p, int v, int slice, int slices_log) {
+    const int head = min((int)((-(intptr_t)p & 15) / sizeof(T)), v), all = (v - head) / kPer;
+    const int each = (all + (1 << slices_log) - 1) >> slices_log, from = min(slice * each, all);
+    groups = min(each, all - from);
+    at = head + from * kPer;
+    begin = slice ? at : 0;
+    end = slice + 1 == 1 << slices_log ? v : at + groups * kPer;
+  }
+  // The same elements, in groups that are aligned at `p` and whose bytes this slice's groups hold.
+  __device__ __forceinline__ Slice aligned_at(const T* p) const {
+    Slice s;
+    s.begin = begin;
+    s.end = end;
+    s.at = at + (int)((-(intptr_t)(p + at) & 15) / sizeof(T));
+    s.groups = max(at + groups * kPer - s.at, 0) / kPer;
+    if (s.groups == 0) s.at = at;
+    return s;
+  }
+  // Elements outside the groups: thread i < edges() takes edge_at(i).
+  __device__ __forceinline__ int edges() const { return end - begin - groups * kPer; }
+  __device__ __forceinline__ int edge_at(int i) const { return begin + i < at ? begin + i : begin + i + groups * kPer; }
+  __device__ __forceinline__ bool owns(int j) const { return j >= begin && j < end; }
+};
+
+// 16 bytes from an address that is 4 Q + r bytes (r = bits / 8, 0 or 2) behind a 16-byte boundary; Q < 0: at one.
+template <int Q>
+__device__ __forceinline__ uint4 load_shifted(const char* p, uint32_t bits) {
+  if constexpr (Q < 0) {
+    return *reinterpret_cast<const uint4*>(p);
+  } else {
+    const uint4* q = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(p) & ~uintptr_t(15));
+    const uint4 a = q[0], b = q[1];
+    const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+    return make_uint4(__funnelshift_r(w[Q], w[Q + 1], bits), __funnelshift_r(w[Q + 1], w[Q + 2], bits),
+                      __funnelshift_r(w[Q + 2], w[Q + 3], bits), __funnelshift_r(w[Q + 3], w[(Q + 4) & 7], bits));
+  }
+}
+
+// z and out lie at the same distance from a 16-byte boundary: nothing is shifted.
+template <typename T>
+__device__ __forceinline__ bool alike(const T* z, const T* out) {
+  return ((reinterpret_cast<uintptr_t>(z) ^ reinterpret_cast<uintptr_t>(out)) & 15) == 0;
+}
+
 // ---- thread-block clusters ------------------------------------------------------
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
