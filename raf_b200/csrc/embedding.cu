@@ -357,19 +357,24 @@ constexpr int kSumAhead = 3;                  // batches on their way
 constexpr int kSumRing = kSumBatch * kSumAhead;
 constexpr int kMostRun = 128;                 // tokens of a warp, at most
 
-// Copies BYTES of one lane to shared memory: asynchronously where the hardware does (16, 8 or 4 bytes).
+// Copies BYTES (16, 8 or 4) of one lane to shared memory, asynchronously.
 template <int BYTES>
 __device__ __forceinline__ void copy_lane(void* to, const void* from) {
-  if constexpr (BYTES >= 4) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from), "n"(BYTES) : "memory");
-  } else {
-    *static_cast<unsigned short*>(to) = *static_cast<const unsigned short*>(from);
+  asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from), "n"(BYTES) : "memory");
+}
+// The 4 bytes at `from`, as far as they lie in [begin, end), both multiples of 2.
+__device__ __forceinline__ void copy_word(uint32_t* to, const char* from, const char* begin, const char* end) {
+  if (from >= begin && from + 4 <= end) {
+    copy_lane<4>(to, from);
+  } else {  // the array's first or last element, half of a word
+    if (from >= begin && from < end) reinterpret_cast<unsigned short*>(to)[0] = *reinterpret_cast<const unsigned short*>(from);
+    if (from + 2 >= begin && from + 2 < end) reinterpret_cast<unsigned short*>(to)[1] = *reinterpret_cast<const unsigned short*>(from + 2);
   }
 }
 
-template <typename W, int VEC>
+template <typename W, int VEC, bool ANY>
 struct SumShared {
-  W ring[kSumWarps][kSumRing][32];
+  W ring[kSumWarps][kSumRing][ANY ? 33 : 32];
   float parts[kSumWarps][32 * VEC];  // the warp's part of a row that began before it
   uint2 tokens[kSumWarps][kMostRun + 1];
   int through[kSumWarps];            // that row takes all of the warp's tokens and goes on behind it
@@ -378,11 +383,14 @@ struct SumShared {
 // Bound: HBM, the gathered rows of dy.  Rows come through shared memory by asynchronous copies, kSumRing of them on their
 // way for a lane, which alone reads what it has asked for; what an accumulated row holds already is asked for when its
 // first token is met.
-template <typename T, typename O, int VEC>
+// ANY: 16-bit rows that begin at any element (VEC 2).  A lane's two elements are its word of the row's aligned ones, or, where
+// the row begins in the middle of one, that word's second half and the next word's first.
+template <typename T, typename O, int VEC, bool ANY>
 __global__ void __launch_bounds__(kSumThreads, 3) embedding_sum_kernel(SumArgs a) {
   using W = typename Group<T, VEC>::W;
+  constexpr int OUT = ANY ? 1 : VEC, ROW = ANY ? 33 : 32;  // elements of an access to dx; words of a row's place
   extern __shared__ uint4 shared[];
-  auto& [ring, parts, tokens, through] = *reinterpret_cast<SumShared<W, VEC>*>(shared);
+  auto& [ring, parts, tokens, through] = *reinterpret_cast<SumShared<W, VEC, ANY>*>(shared);
   grid_dependency_trigger();
   grid_dependency_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -390,22 +398,33 @@ __global__ void __launch_bounds__(kSumThreads, 3) embedding_sum_kernel(SumArgs a
   const int64_t from = (chunk * kSumWarps + warp) * a.run, to = min(from + a.run, a.n);
   const bool here = col < a.width;  // lanes behind the last column see to the tokens alone
   const uint32_t rows = (uint32_t)a.rows;
-  const T* dy = static_cast<const T*>(a.dy) + (here ? col : 0);
+  const T* dy = static_cast<const T*>(a.dy) + (here || ANY ? col : 0);
+  const char *begin = static_cast<const char*>(a.dy), *end = begin + a.n * a.width * (int64_t)sizeof(T);
   O* dx = static_cast<O*>(a.dx) + col;
   uint32_t row = rows, before = rows, behind = rows, first = rows;
   float sum[VEC];
 #pragma unroll
   for (int j = 0; j < VEC; ++j) sum[j] = 0.f;
-  auto put = [&](const Group<O, VEC>& old) {
-    if (!here) return;
-    Group<O, VEC> o;
+  struct Held {
+    Group<O, OUT> g[VEC / OUT];
+  };
+  auto look = [&](Held& old, uint32_t r) {
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) o.x[j] = a.accumulate ? fmaf(sum[j], a.scale, old.x[j]) : sum[j] * a.scale;
-    o.store(dx + (int64_t)row * a.width);
+    for (int q = 0; q < VEC / OUT; ++q) old.g[q].load(dx + (int64_t)r * a.width + (col + q * OUT < a.width ? q * OUT : 0));
+  };
+  auto put = [&](const Held& old) {
+#pragma unroll
+    for (int q = 0; q < VEC / OUT; ++q) {
+      if (col + q * OUT >= a.width) continue;
+      Group<O, OUT> o;
+#pragma unroll
+      for (int j = 0; j < OUT; ++j) o.x[j] = a.accumulate ? fmaf(sum[q * OUT + j], a.scale, old.g[q].x[j]) : sum[q * OUT + j] * a.scale;
+      o.store(dx + (int64_t)row * a.width + q * OUT);
+    }
   };
   auto put_late = [&] {  // where what the row holds has not been asked for
-    Group<O, VEC> old{};
-    if (a.accumulate && here) old.load(dx + (int64_t)row * a.width);
+    Held old{};
+    if (a.accumulate && here) look(old, row);
     put(old);
   };
   if (from < a.n) {
@@ -422,21 +441,30 @@ __global__ void __launch_bounds__(kSumThreads, 3) embedding_sum_kernel(SumArgs a
     first = tokens[warp][0].x;
     auto ask = [&](int i, W* at) {
 #pragma unroll
-      for (int u = 0; u < kSumBatch; ++u)
-        if (i + u < count) copy_lane<sizeof(W)>(at + u * 32, dy + (int64_t)tokens[warp][i + u].y * a.width);
+      for (int u = 0; u < kSumBatch; ++u) {
+        if (i + u >= count) break;
+        const T* p = dy + (int64_t)tokens[warp][i + u].y * a.width;
+        if constexpr (ANY) {
+          const char* word = reinterpret_cast<const char*>(reinterpret_cast<uintptr_t>(p) & ~uintptr_t(3));
+          if (col <= a.width) copy_word(at + u * ROW, word, begin, end);
+          if (lane == 31 && col + 1 < a.width) copy_word(at + u * ROW + 1, word + 4, begin, end);
+        } else {
+          copy_lane<sizeof(W)>(at + u * ROW, p);
+        }
+      }
       asm volatile("cp.async.commit_group;" ::: "memory");
     };
     W* place = &ring[warp][0][lane];
 #pragma unroll
-    for (int b = 0; b < kSumAhead; ++b) ask(b * kSumBatch, place + b * kSumBatch * 32);
+    for (int b = 0; b < kSumAhead; ++b) ask(b * kSumBatch, place + b * kSumBatch * ROW);
     for (int i = 0; i < count; i += kSumBatch) {
       uint32_t r[kSumBatch + 1];
-      Group<O, VEC> old[kSumBatch];
+      Held old[kSumBatch];
 #pragma unroll
       for (int u = 0; u <= kSumBatch; ++u) r[u] = i + u <= count ? tokens[warp][i + u].x : rows;
       if (a.accumulate && here) {  // what the rows that end in this batch hold, all of it asked for together
 #pragma unroll
-        for (int u = 0; u < kSumBatch; ++u) old[u].load(dx + (int64_t)min(r[u], rows - 1) * a.width);
+        for (int u = 0; u < kSumBatch; ++u) look(old[u], min(r[u], rows - 1));
       }
       asm volatile("cp.async.wait_group %0;" ::"n"(kSumAhead - 1) : "memory");
 #pragma unroll
@@ -444,7 +472,13 @@ __global__ void __launch_bounds__(kSumThreads, 3) embedding_sum_kernel(SumArgs a
         if (i + u >= count) break;
         row = r[u];
         float x[VEC];
-        Group<T, VEC>::unpack(place[u * 32], x);
+        W w = place[u * ROW];
+        if constexpr (ANY) {
+          const uint32_t own = w, next = __shfl_down_sync(0xffffffffu, own, 1);
+          if (reinterpret_cast<uintptr_t>(dy + (int64_t)tokens[warp][i + u].y * a.width) & 2)
+            w = __funnelshift_r(own, lane == 31 ? place[u * ROW + 1] : next, 16);
+        }
+        Group<T, VEC>::unpack(w, x);
 #pragma unroll
         for (int j = 0; j < VEC; ++j) sum[j] += x[j];
         if (r[u + 1] != row) {  // the row ends here
@@ -459,7 +493,7 @@ __global__ void __launch_bounds__(kSumThreads, 3) embedding_sum_kernel(SumArgs a
         }
       }
       ask(i + kSumRing, place);
-      place = place == &ring[warp][kSumRing - kSumBatch][lane] ? &ring[warp][0][lane] : place + kSumBatch * 32;
+      place = place == &ring[warp][kSumRing - kSumBatch][lane] ? &ring[warp][0][lane] : place + kSumBatch * ROW;
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     if (row < rows && row == behind && row == before) {  // the whole of it between the two borders
@@ -636,7 +670,8 @@ int rafb200_embedding_dx(const void* dy, int dy_dtype, const void* indices, int 
   cudaStream_t s = static_cast<cudaStream_t>(stream);
 
   const int vec = group_width(dy, dtype_size(dy_dtype), dx, dtype_size(dx_dtype), width);
-  const int64_t tiles = (width + 32 * vec - 1) / (32 * vec);
+  const int lane_width = vec == 1 ? 4 / dtype_size(dy_dtype) : vec;  // 16-bit rows at odd addresses: words, shifted
+  const int64_t tiles = (width + 32 * lane_width - 1) / (32 * lane_width);
   SortArgs so{};
   so.ids = Ids{indices, index_dtype == RAFB200_I64};
   so.n = n;
@@ -688,10 +723,11 @@ int rafb200_embedding_dx(const void* dy, int dy_dtype, const void* indices, int 
     const int rc = with_type(dy_dtype, [&](auto t) {
       return with_width<decltype(t)>(vec, [&](auto w) {
         using T = decltype(t);
-        constexpr int kVec = decltype(w)::value;
-        constexpr size_t smem = sizeof(SumShared<typename Group<T, kVec>::W, kVec>);
-        if (const int rc = allow_smem<embedding_sum_kernel<T, O, kVec>>(smem)) return rc;
-        RAFB200_CUDA(launch_dependent(embedding_sum_kernel<T, O, kVec>, dim3((unsigned)grid), kSumThreads, smem, s, a));
+        constexpr bool kAny = sizeof(T) == 2 && decltype(w)::value == 1;
+        constexpr int kVec = kAny ? 2 : decltype(w)::value;
+        constexpr size_t smem = sizeof(SumShared<typename Group<T, kVec>::W, kVec, kAny>);
+        if (const int rc = allow_smem<embedding_sum_kernel<T, O, kVec, kAny>>(smem)) return rc;
+        RAFB200_CUDA(launch_dependent(embedding_sum_kernel<T, O, kVec, kAny>, dim3((unsigned)grid), kSumThreads, smem, s, a));
         return (int)RAFB200_OK;
       });
     });
