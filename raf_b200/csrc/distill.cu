@@ -362,22 +362,27 @@ __device__ __forceinline__ void write_shifted(const Slice<T>& in, const T* z, T*
     out[j] = Elem<T>::from_f32(co.at<S>(Elem<T>::to_f32(z[j])));
   }
 }
-template <typename T, Second S, int NT>
+// By the stream, which has begun where z and out are alike, or by loads.
+template <typename T, Second S, int NT, bool STREAMED>
 __device__ __forceinline__ void write_slice(const Slice<T>& in, const T* z, float edge, T* out, const Coefficients& co, Stream<T, NT>& stream) {
   if (!alike(z, out)) {
     write_shifted<T, S, NT>(in, z, out, co, threadIdx.x);
     return;
   }
-  uint4* to = reinterpret_cast<uint4*>(out + in.at);  // the stream has begun
-  stream.run([&](int i, const uint4* place, int left) {
-    write_batch<T, S, NT, -1>(reinterpret_cast<const char*>(place), 0, to + i, left, co);
-  });
+  if constexpr (STREAMED) {
+    uint4* to = reinterpret_cast<uint4*>(out + in.at);
+    stream.run([&](int i, const uint4* place, int left) {
+      write_batch<T, S, NT, -1>(reinterpret_cast<const char*>(place), 0, to + i, left, co);
+    });
+  } else {
+    write_batches<T, S, NT, -1>(in, z, out, co, threadIdx.x);
+  }
   if ((int)threadIdx.x < in.edges()) out[in.edge_at(threadIdx.x)] = Elem<T>::from_f32(co.at<S>(edge));
 }
 
 // Whether it is known that no class is named twice: each is put into the table, whose places are tried one after the other.  For
 // short lists write_entries() compares sooner than the table is filled (4096 rows of 1000 with 32 entries: 13.9 against
-// 15.9 us for loss and gradient).  One warp.
+// 15.9 us for loss and gradient), for 64 entries it does not (8192 rows of 50257: 355 against 340 us).  One warp.
 __device__ __forceinline__ bool all_different(const Entries& e, int k) {
   if (k < 64) return false;
   const int lane = threadIdx.x & 31, log = Entries::table_log(k), places = 1 << log;
@@ -576,8 +581,8 @@ __device__ __forceinline__ void leave_out(const DistillArgs& a, int64_t row, int
 // Loss, and with GRAD the gradient, of a row by a cluster of 2^slices_log blocks: one pass with a running maximum and its
 // sums, joined over threads, warps and blocks.
 // GRAD reads the logits a second time, from the L2: the launch sees to it that it holds what the resident blocks work on.
-// 8192 rows of 50257 (bf16, T = 2, labels), loss and gradient: 319 us where gradient rows lie as the logits do, 338 us where
-// they do not (5.2 and 4.9 TB/s of what has to be read and written).  Slices kept in shared memory instead, which
+// 8192 rows of 50257 (bf16, T = 2, labels), loss and gradient: 327 us (5.1 TB/s of what has to be read and written), with
+// gradient rows that lie otherwise than the logits do.  Slices kept in shared memory instead, which
 // leave room for two blocks an SM: 450 us, 590 us with the next row on its way meanwhile - 16 warps an SM are too few for
 // the arithmetic.  The loss alone, 4096 rows of 30522: 55 us (4.6 TB/s), fp32 6.0 TB/s: 16-bit logits give every byte twice the
 // arithmetic.
@@ -627,12 +632,15 @@ __global__ void __launch_bounds__(NT + 32, kSweepThreads / NT) distill_kernel(Di
   const float weight = GRAD && a.dy ? a.dy[row * a.dy_step] : 1.f;
   Sweep<T, S> sweep;
   stream.run([&](int, const uint4* place, int left) { sweep.batch(place, NT, left, a.c); });
-  if (GRAD && alike(z, out)) stream.begin();
+  // 32-bit logits stream a second time (8192 rows of 50257: 5.5 instead of 5.0 TB/s); 16-bit ones do better with loads (327 us
+  // instead of 340 us)
+  constexpr bool kStreamed = GRAD && sizeof(T) == 4;
+  if (kStreamed && alike(z, out)) stream.begin();
   sweep.finish();
   if (tid < s.edges()) sweep.edge(edge, a.c);
   const float4 stats = join<S, NT>(exchange, sweep.run, a);
   if (tid == 0) exchange.stats = stats;
-  if (GRAD) write_slice<T, S, NT>(s, z, edge, out, coefficients<S>(a, weight, stats, labels), stream);
+  if (GRAD) write_slice<T, S, NT, kStreamed>(s, z, edge, out, coefficients<S>(a, weight, stats, labels), stream);
   bar_arrive<NT + 32>(kWritten);
 }
 
@@ -664,7 +672,7 @@ __global__ void __launch_bounds__(kDpredThreads + 32, 6) distill_dpred_kernel(Di
     if (alike(z, out)) stream.begin();
     const Coefficients co = coefficients<S>(a, weight, stats, labels);
     if (in_place) bar_sync<NT + 32>(kWeighed);  // the entries of this slice are read (those of others are not used here)
-    write_slice<T, S, NT>(s, z, edge, out, co, stream);
+    write_slice<T, S, NT, true>(s, z, edge, out, co, stream);
     bar_arrive<NT + 32>(kWritten);
     return;
   }

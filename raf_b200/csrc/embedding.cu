@@ -7,8 +7,10 @@ namespace rafb200 {
 
 // ---- lookup -----------------------------------------------------------------------
 //   out[n, :] = scale * x[id_n, :], a row of zeros where id_n is outside [0, rows)
-// Bound: HBM, the rows read and the rows written.  A warp takes kLookupRows rows, whose ids it knows from one load, and has
-// kLookupUnroll accesses of 32 lanes in flight.  65536 rows of 1024 in bf16: XXX us, XXX TB/s.
+// Bound: HBM, the rows read and the rows written.  A warp takes kLookupRows rows and has four accesses of 32 lanes in
+// flight, at 32 to 48 registers a thread.  65536 rows of 1024 (bf16, 20000 different ones): 29.5 us, 5.7 TB/s of what has to
+// be read and written, where a copy of as many bytes takes 5.5 TB/s.  Rows of 1023: 38 us; from fp32 into bf16, element by
+// element, 20011 rows of 1023 23 us (2.9 TB/s).
 constexpr int kLookupThreads = 256;
 constexpr int kLookupRows = 2;
 
@@ -135,7 +137,8 @@ __device__ void zero_bytes(unsigned char* p, int64_t bytes, int64_t worker, int6
 }
 
 // Few tokens: each warp finds the rank of its tokens by comparing them with all, which need no more than one block's shared
-// memory.  No block waits for another.
+// memory.  No block waits for another.  1024 tokens take 3.4 us where the cluster's passes take 11.7 us, 2048 4.7 and 12.2 us,
+// 4096 10.9 and 12.4 us: the border.
 constexpr int kRankTokens = 4096;
 constexpr int kRankThreads = 256;
 constexpr int kRankLoads = 8;
@@ -170,7 +173,8 @@ __global__ void __launch_bounds__(kRankThreads) embedding_rank_kernel(SortArgs a
 // Many tokens: digits from the lowest up, by one cluster of 16 blocks.  Each of its 512 warps owns a contiguous range of the pairs:
 // it counts its digits, equal ones of a group of 32 ranked by lane; the counts are summed over warps, blocks (through
 // distributed shared memory) and digits, and the warp then moves its pairs in order.
-// XXX
+// Bound: the latency of a pass's two cluster barriers and of its loads and stores, and the counting, which 16 SMs share: 16384
+// tokens take 13 us, 65536 22 us; eight blocks took 37 us for these.
 constexpr int kSortBlocks = 16;
 constexpr int kSortThreads = 1024;
 constexpr int kSortWarps = kSortThreads / 32;
@@ -381,8 +385,9 @@ struct SumShared {
 };
 
 // Bound: HBM, the gathered rows of dy.  Rows come through shared memory by asynchronous copies, kSumRing of them on their
-// way for a lane, which alone reads what it has asked for; what an accumulated row holds already is asked for when its
-// first token is met.
+// way for a lane, which alone reads what it has asked for; what accumulated rows hold already is asked for together for those
+// that end in a batch.  65536 tokens of 1024 (bf16): 28 us into two rows (4.7 TB/s), 52 us added to 20000 rows of fp32
+// (5.7 TB/s of dy and of the rows read and written).
 // ANY: 16-bit rows that begin at any element (VEC 2).  A lane's two elements are its word of the row's aligned ones, or, where
 // the row begins in the middle of one, that word's second half and the next word's first.
 template <typename T, typename O, int VEC, bool ANY>
@@ -687,8 +692,6 @@ int rafb200_embedding_dx(const void* dy, int dy_dtype, const void* indices, int 
     so.fill = static_cast<unsigned char*>(dx);
     so.fill_bytes = rows * width * dtype_size(dx_dtype);
   }
-  // three to six times as fast as the cluster's passes where a warp has one token to compare, and no slower at the border:
-  // XXX
   if (n <= kRankTokens) {
     const int64_t ranks = (n + kRankThreads / 32 - 1) / (kRankThreads / 32), fills = so.fill_bytes / (kRankThreads * 64);
     const unsigned grid = (unsigned)std::min<int64_t>(std::max<int64_t>({ranks, fills, 1}), 148 * 4);
