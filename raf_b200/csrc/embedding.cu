@@ -351,7 +351,7 @@ struct SumArgs {
   float* partial;        // [chunk][2][stride]: sums of a row that began before the chunk, or goes on behind it
   int64_t stride;
   int run;               // tokens of a warp
-  int64_t tiles;         // column tiles of 32 * VEC
+  uint32_t tiles;        // column tiles of 32 * VEC
 };
 
 constexpr int kSumWarps = 8;  // of a chunk
@@ -376,6 +376,32 @@ __device__ __forceinline__ void copy_word(uint32_t* to, const char* from, const 
   }
 }
 
+// VEC running sums, two an instruction.
+template <int VEC>
+struct Sums {
+  Two s[VEC / 2];
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int j = 0; j < VEC / 2; ++j) s[j] = Two(0.f, 0.f);
+  }
+  template <typename Get>
+  __device__ __forceinline__ void add(const Get& get) {
+#pragma unroll
+    for (int j = 0; j < VEC / 2; ++j) s[j] = s[j] + Two(get(2 * j), get(2 * j + 1));
+  }
+  __device__ __forceinline__ float at(int j) const { return j & 1 ? s[j / 2].hi() : s[j / 2].lo(); }
+};
+template <>
+struct Sums<1> {
+  float s;
+  __device__ __forceinline__ void clear() { s = 0.f; }
+  template <typename Get>
+  __device__ __forceinline__ void add(const Get& get) {
+    s += get(0);
+  }
+  __device__ __forceinline__ float at(int) const { return s; }
+};
+
 template <typename W, int VEC, bool ANY>
 struct SumShared {
   W ring[kSumWarps][kSumRing][ANY ? 33 : 32];
@@ -399,7 +425,7 @@ __global__ void __launch_bounds__(kSumThreads, 3) embedding_sum_kernel(SumArgs a
   grid_dependency_trigger();
   grid_dependency_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t chunk = blockIdx.x / a.tiles, col = (blockIdx.x % a.tiles * 32 + lane) * VEC;
+  const int64_t chunk = blockIdx.x / a.tiles, col = (int64_t)((blockIdx.x - (uint32_t)chunk * a.tiles) * 32 + lane) * VEC;
   const int64_t from = (chunk * kSumWarps + warp) * a.run, to = min(from + a.run, a.n);
   const bool here = col < a.width;  // lanes behind the last column see to the tokens alone
   const uint32_t rows = (uint32_t)a.rows;
@@ -407,9 +433,12 @@ __global__ void __launch_bounds__(kSumThreads, 3) embedding_sum_kernel(SumArgs a
   const char *begin = static_cast<const char*>(a.dy), *end = begin + a.n * a.width * (int64_t)sizeof(T);
   O* dx = static_cast<O*>(a.dx) + col;
   uint32_t row = rows, before = rows, behind = rows, first = rows;
-  float sum[VEC];
+  Sums<VEC> sum;
+  sum.clear();
+  auto keep = [&] {
 #pragma unroll
-  for (int j = 0; j < VEC; ++j) sum[j] = 0.f;
+    for (int j = 0; j < VEC; ++j) parts[warp][j * 32 + lane] = sum.at(j);
+  };
   struct Held {
     Group<O, OUT> g[VEC / OUT];
   };
@@ -423,7 +452,7 @@ __global__ void __launch_bounds__(kSumThreads, 3) embedding_sum_kernel(SumArgs a
       if (col + q * OUT >= a.width) continue;
       Group<O, OUT> o;
 #pragma unroll
-      for (int j = 0; j < OUT; ++j) o.x[j] = a.accumulate ? fmaf(sum[q * OUT + j], a.scale, old.g[q].x[j]) : sum[q * OUT + j] * a.scale;
+      for (int j = 0; j < OUT; ++j) o.x[j] = a.accumulate ? fmaf(sum.at(q * OUT + j), a.scale, old.g[q].x[j]) : sum.at(q * OUT + j) * a.scale;
       o.store(dx + (int64_t)row * a.width + q * OUT);
     }
   };
@@ -484,27 +513,18 @@ __global__ void __launch_bounds__(kSumThreads, 3) embedding_sum_kernel(SumArgs a
             w = __funnelshift_r(own, lane == 31 ? place[u * ROW + 1] : next, 16);
         }
         Group<T, VEC>::unpack(w, x);
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) sum[j] += x[j];
+        sum.add([&](int j) { return x[j]; });
         if (r[u + 1] != row) {  // the row ends here
-          if (row == before) {
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) parts[warp][j * 32 + lane] = sum[j];
-          } else {
-            put(old[u]);
-          }
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) sum[j] = 0.f;
+          if (row == before) keep();
+          else put(old[u]);
+          sum.clear();
         }
       }
       ask(i + kSumRing, place);
       place = place == &ring[warp][kSumRing - kSumBatch][lane] ? &ring[warp][0][lane] : place + kSumBatch * ROW;
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
-    if (row < rows && row == behind && row == before) {  // the whole of it between the two borders
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) parts[warp][j * 32 + lane] = sum[j];
-    }
+    if (row < rows && row == behind && row == before) keep();  // the whole of it between the two borders
   }
   if (lane == 0) through[warp] = row < rows && row == before && row == behind && row == first;
   const bool starts = row < rows && row != before && row == behind;  // a row goes on behind this warp
@@ -512,8 +532,7 @@ __global__ void __launch_bounds__(kSumThreads, 3) embedding_sum_kernel(SumArgs a
   __syncthreads();
   auto follow = [&](int w) {  // adds the parts of warps w, w + 1, ... as far as the row goes on; whether it leaves the chunk
     for (; w < kSumWarps; ++w) {
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) sum[j] += parts[w][j * 32 + lane];
+      sum.add([&](int j) { return parts[w][j * 32 + lane]; });
       if (!through[w]) return false;
     }
     return true;
@@ -522,7 +541,7 @@ __global__ void __launch_bounds__(kSumThreads, 3) embedding_sum_kernel(SumArgs a
     if (!here) return;
     Group<float, VEC> g;
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) g.x[j] = sum[j];
+    for (int j = 0; j < VEC; ++j) g.x[j] = sum.at(j);
     g.store(a.partial + (chunk * 2 + slot) * a.stride + col);
   };
   if (starts) {
@@ -530,8 +549,7 @@ __global__ void __launch_bounds__(kSumThreads, 3) embedding_sum_kernel(SumArgs a
     else put_late();
   }
   if (enters) {  // warp 0 may see to this row and to another one that begins with it
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) sum[j] = 0.f;
+    sum.clear();
     follow(0);
     put_partial(0);
   }
@@ -716,10 +734,10 @@ int rafb200_embedding_dx(const void* dy, int dy_dtype, const void* indices, int 
   a.dx = dx;
   a.partial = reinterpret_cast<float*>(static_cast<char*>(workspace) + 2 * round_up((size_t)n * sizeof(uint2)));
   a.stride = (width + 7) & ~int64_t(7);
-  a.tiles = tiles;
+  a.tiles = (uint32_t)tiles;
   a.run = warp_tokens(n, width);
   const int64_t tokens = (int64_t)kSumWarps * a.run, chunks = (n + tokens - 1) / tokens;
-  const int64_t grid = chunks * a.tiles, cols = (width + kJoinCols - 1) / kJoinCols;
+  const int64_t grid = chunks * tiles, cols = (width + kJoinCols - 1) / kJoinCols;
   RAFB200_REQUIRE(grid < ((int64_t)1 << 31) && cols < 65536, "rafb200_embedding_dx: rows too wide");
   return with_type(dx_dtype, [&](auto o) {
     using O = decltype(o);

@@ -115,6 +115,38 @@ struct Group {
   }
 };
 
+// Two fp32 numbers in a register pair.
+struct Two {
+  uint64_t r;
+  __device__ __forceinline__ Two() {}
+  __device__ __forceinline__ Two(float lo, float hi) { asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi)); }
+  __device__ __forceinline__ float lo() const {
+    float a, b;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(r));
+    return a;
+  }
+  __device__ __forceinline__ float hi() const {
+    float a, b;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(r));
+    return b;
+  }
+};
+__device__ __forceinline__ Two operator+(Two a, Two b) {
+  Two c;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(c.r) : "l"(a.r), "l"(b.r));
+  return c;
+}
+__device__ __forceinline__ Two operator*(Two a, Two b) {
+  Two c;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(c.r) : "l"(a.r), "l"(b.r));
+  return c;
+}
+__device__ __forceinline__ Two fma2(Two a, Two b, Two d) {
+  Two c;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(c.r) : "l"(a.r), "l"(b.r), "l"(d.r));
+  return c;
+}
+
 // ---- rows at any address ----------------------------------------------------------
 // A block's part of a row: elements [begin, end), of which `groups` groups of 16 bytes from element `at` on are aligned
 // in memory.  The row's first and last elements, which no aligned group holds, are the first and the last block's.
