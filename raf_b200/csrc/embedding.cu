@@ -106,12 +106,12 @@ __global__ void __launch_bounds__(kLookupThreads)
 
 // ---- gradient ---------------------------------------------------------------------
 //   dx[r, :] (+)= scale * sum over the n with id_n = r of dy[n, :]
-// Three launches, every sum in an order that the tokens alone fix:
+// Two launches, every sum in an order that the tokens alone fix:
 //   1. the tokens are sorted, stably, while other blocks write the zeros of rows without a token;
 //   2. a warp walks `run` sorted tokens for 32 * VEC columns and keeps the sum of the present row in registers.  A row whose
 //      tokens all lie there is written there; a row cut by the border between two warps of a block is put together in shared
-//      memory, one cut by the border of a block (a chunk of tokens) leaves partial sums;
-//   3. the rows that were cut by chunks are joined, chunk after chunk.
+//      memory, one cut by the border of a block (a chunk of tokens) leaves partial sums, which the last of its blocks to
+//      come adds up, chunk after chunk.
 struct SortArgs {
   Ids ids;
   int64_t n;
@@ -122,6 +122,8 @@ struct SortArgs {
   int passes, bits;    // digits and bits of each
   unsigned char* fill; // bytes to zero
   int64_t fill_bytes;
+  uint32_t* counters;  // to be zeroed too: of the blocks that have left their part of a row
+  int n_counters;
   __device__ __forceinline__ uint32_t key(int64_t id) const {
     return (uint64_t)id < (uint64_t)rows && id != padding ? (uint32_t)id : (uint32_t)rows;
   }
@@ -148,6 +150,8 @@ __global__ void __launch_bounds__(kRankThreads) embedding_rank_kernel(SortArgs a
   grid_dependency_wait();
   const int n = (int)a.n, tid = threadIdx.x, lane = tid & 31, warps = gridDim.x * (kRankThreads / 32);
   const int mine = blockIdx.x * (kRankThreads / 32) + (tid >> 5);
+  if (blockIdx.x == gridDim.x - 1)
+    for (int i = tid; i < a.n_counters; i += kRankThreads) a.counters[i] = 0;
   if (blockIdx.x * (kRankThreads / 32) < n) {
     for (int i0 = tid; i0 < n; i0 += kRankThreads * kRankLoads) {
       int64_t id[kRankLoads];  // all of them asked for before the first is looked at
@@ -200,6 +204,7 @@ __global__ void __launch_bounds__(kSortThreads) embedding_sort_kernel(SortArgs a
   const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rank = cluster_rank(), n = (uint32_t)a.n;
   const uint32_t each = ((n + kSortBlocks * kSortWarps - 1) / (kSortBlocks * kSortWarps) + 31) & ~31u;
   const uint32_t from = (uint32_t)min((uint64_t)(rank * kSortWarps + warp) * each, (uint64_t)n), to = min(n - from, each) + from;
+  for (int i = rank * kSortThreads + tid; i < a.n_counters; i += kSortBlocks * kSortThreads) a.counters[i] = 0;
   uint32_t* mine = counts + warp * kDigits;
   const uint32_t digits = 1u << a.bits, lower_lanes = (1u << lane) - 1u;
   const bool kept = each <= 32 * kSortItems;  // a warp's pairs stay in registers from counting to moving
@@ -350,6 +355,7 @@ struct SumArgs {
   void* dx;
   float* partial;        // [chunk][2][stride]: sums of a row that began before the chunk, or goes on behind it
   int64_t stride;
+  uint32_t* counters;    // [chunk in which the row begins][tile]
   int run;               // tokens of a warp
   uint32_t tiles;        // column tiles of 32 * VEC
 };
@@ -408,12 +414,16 @@ struct SumShared {
   float parts[kSumWarps][32 * VEC];  // the warp's part of a row that began before it
   uint2 tokens[kSumWarps][kMostRun + 1];
   int through[kSumWarps];            // that row takes all of the warp's tokens and goes on behind it
+  struct {
+    int64_t begins, ends;            // chunks [begins, ends) have left their parts of the row, this one as the last; or 0, 0
+    uint32_t row;
+  } joins[2];                        // of the row that began before the chunk, and of the one that goes on behind it
 };
 
 // Bound: HBM, the gathered rows of dy.  Rows come through shared memory by asynchronous copies, kSumRing of them on their
 // way for a lane, which alone reads what it has asked for; what accumulated rows hold already is asked for together for those
-// that end in a batch.  65536 tokens of 1024 (bf16): 28 us into two rows (4.7 TB/s), 52 us added to 20000 rows of fp32
-// (5.7 TB/s of dy and of the rows read and written).
+// that end in a batch.  The sums of cut rows, in a launch of their own, took 2 to 5 us more.  65536 tokens of 1024 (bf16):
+// 32 us into two rows (4.2 TB/s), 54 us added to 20000 rows of fp32 (5.5 TB/s of dy and of the rows read and written).
 // ANY: 16-bit rows that begin at any element (VEC 2).  A lane's two elements are its word of the row's aligned ones, or, where
 // the row begins in the middle of one, that word's second half and the next word's first.
 template <typename T, typename O, int VEC, bool ANY>
@@ -421,7 +431,7 @@ __global__ void __launch_bounds__(kSumThreads, 3) embedding_sum_kernel(SumArgs a
   using W = typename Group<T, VEC>::W;
   constexpr int OUT = ANY ? 1 : VEC, ROW = ANY ? 33 : 32;  // elements of an access to dx; words of a row's place
   extern __shared__ uint4 shared[];
-  auto& [ring, parts, tokens, through] = *reinterpret_cast<SumShared<W, VEC, ANY>*>(shared);
+  auto& [ring, parts, tokens, through, joins] = *reinterpret_cast<SumShared<W, VEC, ANY>*>(shared);
   grid_dependency_trigger();
   grid_dependency_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -526,6 +536,7 @@ __global__ void __launch_bounds__(kSumThreads, 3) embedding_sum_kernel(SumArgs a
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     if (row < rows && row == behind && row == before) keep();  // the whole of it between the two borders
   }
+  if (threadIdx.x < 2) joins[threadIdx.x].ends = 0;
   if (lane == 0) through[warp] = row < rows && row == before && row == behind && row == first;
   const bool starts = row < rows && row != before && row == behind;  // a row goes on behind this warp
   const bool enters = warp == 0 && first < rows && first == before;  // a row began before this chunk
@@ -544,66 +555,76 @@ __global__ void __launch_bounds__(kSumThreads, 3) embedding_sum_kernel(SumArgs a
     for (int j = 0; j < VEC; ++j) g.x[j] = sum.at(j);
     g.store(a.partial + (chunk * 2 + slot) * a.stride + col);
   };
+  // This warp has left the chunk's part of `row`: is it the last to do so?
+  const int64_t length = (int64_t)kSumWarps * a.run;
+  auto left = [&](int which, int64_t begins, bool leaves) {
+    for (bool go = begins < chunk; go;) {  // the chunk in which the row begins: it goes on before that chunk's first token otherwise
+      const int64_t c = begins - lane;
+      const uint32_t on = __ballot_sync(0xffffffffu, c > 0 && a.sorted[c * length - 1].x == row);
+      go = on == 0xffffffffu;
+      begins -= go ? 32 : __ffs(~on) - 1;
+    }
+    int64_t ends = chunk + 1;  // the first chunk that does not begin with the row
+    for (bool go = leaves; go;) {
+      const int64_t c = ends + lane;
+      const uint32_t on = __ballot_sync(0xffffffffu, c * length < a.n && a.sorted[c * length].x == row);
+      go = on == 0xffffffffu;
+      ends += go ? 32 : __ffs(~on) - 1;
+    }
+    __threadfence();
+    __syncwarp();
+    if (lane == 0 && atomicAdd(a.counters + begins * a.tiles + (blockIdx.x - (uint32_t)chunk * a.tiles), 1u) + 1 == (uint32_t)(ends - begins)) {
+      joins[which].begins = begins;
+      joins[which].ends = ends;
+      joins[which].row = row;
+    }
+  };
   if (starts) {
-    if (follow(warp + 1)) put_partial(1);
-    else put_late();
-  }
-  if (enters) {  // warp 0 may see to this row and to another one that begins with it
-    sum.clear();
-    follow(0);
-    put_partial(0);
-  }
-}
-
-// The rows that chunks have cut: the block of the chunk in which a row begins adds up its parts.  Eight warps take
-// every eighth part, and their sums are added in the order of the warps.
-constexpr int kJoinThreads = 256;
-constexpr int kJoinCols = 128;
-
-template <typename O>
-__global__ void __launch_bounds__(kJoinThreads) embedding_join_kernel(SumArgs a) {
-  __shared__ float4 part[kJoinThreads / 32][32];
-  grid_dependency_trigger();
-  grid_dependency_wait();
-  const int64_t tokens = (int64_t)kSumWarps * a.run, chunk = blockIdx.x, from = chunk * tokens, to = from + tokens;
-  if (to >= a.n) return;
-  const uint32_t row = a.sorted[to].x, last = a.sorted[to - 1].x, before = from ? a.sorted[from - 1].x : (uint32_t)a.rows;
-  if (row >= (uint32_t)a.rows || last != row || before == row) return;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t col = (int64_t)blockIdx.y * kJoinCols + lane * 4;
-  const float* at = a.partial + col;
-  float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-  int64_t end = chunk + 1;  // the first chunk that does not begin with the row
-  for (uint32_t all = 0xffffffffu; all == 0xffffffffu;) {
-    const int64_t c = end + lane;
-    all = __ballot_sync(0xffffffffu, c * tokens < a.n && a.sorted[c * tokens].x == row);
-    end += __popc(all);
-  }
-  if (col < a.width) {
-    if (warp == 0) sum = *reinterpret_cast<const float4*>(at + (chunk * 2 + 1) * a.stride);
-#pragma unroll 4
-    for (int64_t c = chunk + 1 + warp; c < end; c += kJoinThreads / 32) {
-      const float4 p = *reinterpret_cast<const float4*>(at + c * 2 * a.stride);
-      sum.x += p.x;
-      sum.y += p.y;
-      sum.z += p.z;
-      sum.w += p.w;
+    if (follow(warp + 1)) {
+      put_partial(1);
+      left(1, chunk, true);
+    } else {
+      put_late();
     }
   }
-  part[warp][lane] = sum;
-  __syncthreads();
-  if (warp || col >= a.width) return;
-#pragma unroll
-  for (int w = 1; w < kJoinThreads / 32; ++w) {
-    sum.x += part[w][lane].x;
-    sum.y += part[w][lane].y;
-    sum.z += part[w][lane].z;
-    sum.w += part[w][lane].w;
+  if (enters) {  // warp 0 may see to this row and to another one that begins with it
+    row = first;
+    sum.clear();
+    const bool leaves = follow(0);
+    put_partial(0);
+    left(0, chunk - 1, leaves);
   }
-  const float s[4] = {sum.x, sum.y, sum.z, sum.w};
-  O* dx = static_cast<O*>(a.dx) + (int64_t)row * a.width + col;
-  for (int j = 0; j < 4 && col + j < a.width; ++j)
-    dx[j] = Elem<O>::from_f32(a.accumulate ? fmaf(s[j], a.scale, Elem<O>::to_f32(dx[j])) : s[j] * a.scale);
+  __syncthreads();
+  for (int which = 0; which < 2; ++which) {  // each warp takes every eighth part; their sums in the order of the warps
+    const int64_t begins = joins[which].begins, ends = joins[which].ends;
+    if (!ends) continue;
+    __threadfence();
+    sum.clear();
+    if (here) {
+      constexpr int kParts = 4;
+      const float* part = a.partial + col;
+      for (int64_t c0 = begins + warp; c0 < ends; c0 += kParts * kSumWarps) {
+        Group<float, VEC> g[kParts];
+#pragma unroll
+        for (int u = 0; u < kParts; ++u) {  // all of them asked for before the first is looked at
+          const int64_t c = min(c0 + u * kSumWarps, ends - 1);
+          g[u].load_coherent(part + (c * 2 + (c == begins)) * a.stride);
+        }
+#pragma unroll
+        for (int u = 0; u < kParts; ++u)
+          if (c0 + u * kSumWarps < ends) sum.add([&](int j) { return g[u].x[j]; });
+      }
+    }
+    keep();
+    __syncthreads();
+    if (warp == 0) {
+      row = joins[which].row;
+      sum.clear();
+      for (int w = 0; w < kSumWarps; ++w) sum.add([&](int j) { return parts[w][j * 32 + lane]; });
+      put_late();
+    }
+    __syncthreads();
+  }
 }
 
 // Elements of an access that every row of both arrays allows: 16 bytes of the first array's, 2, or 1.
@@ -670,11 +691,12 @@ int rafb200_embedding(const void* x, int x_dtype, int64_t rows, int64_t width, c
   });
 }
 
-// The workspace holds the pairs twice, then the partial sums of the chunks.
+// The workspace holds the pairs twice, then the partial sums of the chunks and their counters.
 size_t rafb200_embedding_dx_workspace_bytes(int64_t n, int64_t width) {
   if (n <= 0 || width <= 0 || n >= ((int64_t)1 << 31) || range_overflows(n, width)) return 0;
   const int64_t tokens = (int64_t)kSumWarps * warp_tokens(n, width), chunks = (n + tokens - 1) / tokens;
-  return 2 * round_up((size_t)n * sizeof(uint2)) + (size_t)chunks * 2 * ((width + 7) & ~int64_t(7)) * sizeof(float);
+  return 2 * round_up((size_t)n * sizeof(uint2)) + round_up((size_t)chunks * 2 * ((width + 7) & ~int64_t(7)) * sizeof(float)) +
+         (size_t)chunks * ((width + 31) / 32) * sizeof(uint32_t);  // a tile has 32 columns at least
 }
 
 int rafb200_embedding_dx(const void* dy, int dy_dtype, const void* indices, int index_dtype, int64_t n, int64_t rows,
@@ -702,6 +724,13 @@ int rafb200_embedding_dx(const void* dy, int dy_dtype, const void* indices, int 
   so.padding = padding_idx;
   so.a = static_cast<uint2*>(workspace);
   so.b = reinterpret_cast<uint2*>(static_cast<char*>(workspace) + round_up((size_t)n * sizeof(uint2)));
+  const int run = n ? warp_tokens(n, width) : 1;
+  const int64_t tokens = (int64_t)kSumWarps * run, chunks = (n + tokens - 1) / tokens, grid = chunks * tiles;
+  const int64_t stride = (width + 7) & ~int64_t(7);
+  float* partial = reinterpret_cast<float*>(static_cast<char*>(workspace) + 2 * round_up((size_t)n * sizeof(uint2)));
+  RAFB200_REQUIRE(grid < ((int64_t)1 << 31), "rafb200_embedding_dx: rows too wide");
+  so.counters = reinterpret_cast<uint32_t*>(reinterpret_cast<char*>(partial) + round_up((size_t)chunks * 2 * stride * sizeof(float)));
+  so.n_counters = (int)grid;
   int bits = 1;
   while (rows >> bits) ++bits;
   so.passes = (bits + kDigitBits - 1) / kDigitBits;
@@ -732,16 +761,14 @@ int rafb200_embedding_dx(const void* dy, int dy_dtype, const void* indices, int 
   a.scale = scale;
   a.accumulate = accumulate;
   a.dx = dx;
-  a.partial = reinterpret_cast<float*>(static_cast<char*>(workspace) + 2 * round_up((size_t)n * sizeof(uint2)));
-  a.stride = (width + 7) & ~int64_t(7);
+  a.partial = partial;
+  a.stride = stride;
+  a.counters = so.counters;
   a.tiles = (uint32_t)tiles;
-  a.run = warp_tokens(n, width);
-  const int64_t tokens = (int64_t)kSumWarps * a.run, chunks = (n + tokens - 1) / tokens;
-  const int64_t grid = chunks * tiles, cols = (width + kJoinCols - 1) / kJoinCols;
-  RAFB200_REQUIRE(grid < ((int64_t)1 << 31) && cols < 65536, "rafb200_embedding_dx: rows too wide");
+  a.run = run;
   return with_type(dx_dtype, [&](auto o) {
     using O = decltype(o);
-    const int rc = with_type(dy_dtype, [&](auto t) {
+    return with_type(dy_dtype, [&](auto t) {
       return with_width<decltype(t)>(vec, [&](auto w) {
         using T = decltype(t);
         constexpr bool kAny = sizeof(T) == 2 && decltype(w)::value == 1;
@@ -752,9 +779,6 @@ int rafb200_embedding_dx(const void* dy, int dy_dtype, const void* indices, int 
         return (int)RAFB200_OK;
       });
     });
-    if (rc != RAFB200_OK || chunks == 1) return rc;
-    RAFB200_CUDA(launch_dependent(embedding_join_kernel<O>, dim3((unsigned)(chunks - 1), (unsigned)cols), kJoinThreads, 0, s, a));
-    return (int)RAFB200_OK;
   });
 }
 

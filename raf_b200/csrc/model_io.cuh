@@ -63,6 +63,11 @@ struct Group {
 #pragma unroll
     for (int q = 0; q < kWords; ++q) unpack(reinterpret_cast<const W*>(p)[q], x + q * kPer);
   }
+  // from the L2, where other blocks of the grid have written it
+  __device__ __forceinline__ void load_coherent(const T* p) {
+#pragma unroll
+    for (int q = 0; q < kWords; ++q) unpack(__ldcg(reinterpret_cast<const W*>(p) + q), x + q * kPer);
+  }
   __device__ __forceinline__ void store(T* p) const {
 #pragma unroll
     for (int q = 0; q < kWords; ++q) reinterpret_cast<W*>(p)[q] = pack(x + q * kPer);

@@ -117,7 +117,7 @@ def test_shapes_of_indices():
 
 
 @pytest.mark.parametrize("n,rows,width", [(0, 5, 8), (1, 1, 1), (1, 3, 1024), (7, 2, 3), (31, 513, 64), (257, 2, 1024), (1000, 40, 1023), (3000, 512, 136),
-                                          (20011, 30522, 40), (9000, 2, 264), (4097, 300000, 8), (70001, 1000, 18), (12, 4, 5000)])
+                                          (20011, 30522, 40), (9000, 2, 264), (4097, 300000, 8), (70001, 1000, 18), (12, 4, 5000), (300007, 5000, 6), (140001, 2, 33)])
 @pytest.mark.parametrize("kind", ["uniform", "one", "falling", "words", "outside"])
 def test_gradient(n, rows, width, kind):
     g = torch.Generator(device="cuda").manual_seed(n + 3 * rows + width)
