@@ -355,12 +355,16 @@ def _check_apart(out, *inputs):
 
 
 @contextlib.contextmanager
-def _launching(t, stream):
+def _launching(t, stream, *others):
     """On the tensor's device and the given stream, for allocations too: what a call allocates there is not
-    handed to another stream's work while the call still runs."""
+    handed to another stream's work while the call still runs, nor are the tensors it is given."""
     if stream is not None and stream.device != t.device:
         raise ValueError("the stream belongs to another device than the tensors")
     with torch.cuda.device(t.device), torch.cuda.stream(stream):
+        if stream is not None and not torch.cuda.is_current_stream_capturing():
+            for x in (t,) + others:
+                if x is not None:
+                    x.record_stream(stream)
         yield torch._C._cuda_getCurrentRawStream(t.device.index)
 
 
@@ -400,7 +404,7 @@ def embedding(x, indices, scale=1.0, padding_idx=None, dtype=None, out=None, str
     if torch.is_grad_enabled() and x.requires_grad:
         if out is not None:
             raise ValueError("embedding: out has no gradient; x must not require one")
-        with _launching(x, stream):  # autograd runs backward on the stream that is current here
+        with _launching(x, stream, indices):  # autograd runs backward on the stream that is current here
             return _Embedding.apply(x, indices, scale, padding_idx, dtype)
     shape = indices.shape + x.shape[1:]
     if out is not None:
@@ -410,7 +414,7 @@ def embedding(x, indices, scale=1.0, padding_idx=None, dtype=None, out=None, str
             raise ValueError(f"embedding: out is to be {tuple(shape)} of {dtype}")
         _check_apart(out, x, indices)
         torch.autograd.graph.increment_version(out)
-    with _launching(x, stream) as raw:
+    with _launching(x, stream, indices, out) as raw:
         if out is None:
             out = torch.empty(shape, dtype=dtype, device=x.device)
         check(_lib.load().rafb200_embedding(x.data_ptr(), code, x.shape[0], x.shape[1], indices.data_ptr(), index,
@@ -424,7 +428,8 @@ def embedding_dx(dy, indices, num_weight, scale=1.0, padding_idx=None, dtype=Non
 
     ``out`` takes the result: a gradient that an optimizer or ZeroStep reads.  With ``accumulate`` the sums are
     added to it (a further micro-batch, a matrix product that shares the table), rounded once to its type, and rows
-    without a token stay as they are.  Indices equal to ``padding_idx`` or outside [0, num_weight) count nothing.
+    without a token stay as they are.  Indices equal to ``padding_idx`` or outside [0, num_weight) count nothing (a negative
+    ``padding_idx`` names no row).
     The same call gives the same bits: sums run in an order that the indices fix.
     """
     if stream is None:
@@ -457,7 +462,7 @@ def embedding_dx(dy, indices, num_weight, scale=1.0, padding_idx=None, dtype=Non
     # outside [0, num_weight): nothing is left out
     padding_idx = -1 if padding_idx is None else int(padding_idx)
     lib, n = _lib.load(), indices.numel()
-    with _launching(dy, stream) as raw:
+    with _launching(dy, stream, indices, out) as raw:
         if out is None:
             out = torch.empty((num_weight, width), dtype=dtype, device=dy.device)
         ws = torch.empty(lib.rafb200_embedding_dx_workspace_bytes(n, width), dtype=torch.uint8, device=dy.device)
@@ -566,9 +571,9 @@ def distill_loss(pred, teacher_logits, teacher_ids, labels=None, temperature=1.0
     if torch.is_grad_enabled() and teacher_logits.requires_grad:
         raise ValueError("distill_loss: the teacher gets no gradient; detach its logits")
     if torch.is_grad_enabled() and pred.requires_grad:
-        with _launching(pred, stream):
+        with _launching(pred, stream, teacher_logits, teacher_ids, labels):
             return _DistillLoss.apply(pred, teacher_logits, teacher_ids, labels, temperature, alpha, ignore_index)
-    with _launching(pred, stream) as raw:
+    with _launching(pred, stream, teacher_logits, teacher_ids, labels) as raw:
         loss = torch.empty(pred.shape[:-1], dtype=torch.float32, device=pred.device)
         stats = torch.empty(pred.shape[:-1] + (4,), dtype=torch.float32, device=pred.device)
         check(_lib.load().rafb200_distill_loss(C.byref(d), loss.data_ptr(), stats.data_ptr(), raw))
@@ -594,7 +599,7 @@ def distill_loss_dpred(dy, pred, teacher_logits, teacher_ids, stats, labels=None
     _same_device(pred, stats)
     if stats.shape != pred.shape[:-1] + (4,) or stats.dtype != torch.float32:
         raise ValueError("distill_loss_dpred: stats are those of distill_loss for this pred")
-    with _launching(pred, stream) as raw:
+    with _launching(pred, stream, dy, teacher_logits, teacher_ids, stats, labels, out) as raw:
         out, ld = _gradient_for(pred, out, (dy, teacher_logits, teacher_ids, stats, labels))
         check(_lib.load().rafb200_distill_loss_dpred(C.byref(d), weights, step, float(grad_scale), stats.data_ptr(),
                                                      out.data_ptr(), ld, raw))
@@ -613,7 +618,7 @@ def distill_loss_with_dpred(dy, pred, teacher_logits, teacher_ids, labels=None, 
             check(r)
     d = _distill_args(pred, teacher_logits, teacher_ids, labels, temperature, alpha, ignore_index)
     weights, step = _weights_of(dy, pred)
-    with _launching(pred, stream) as raw:
+    with _launching(pred, stream, dy, teacher_logits, teacher_ids, labels, out) as raw:
         loss = torch.empty(pred.shape[:-1], dtype=torch.float32, device=pred.device)
         out, ld = _gradient_for(pred, out, (dy, teacher_logits, teacher_ids, labels))
         check(_lib.load().rafb200_distill_loss_with_dpred(C.byref(d), weights, step, float(grad_scale), loss.data_ptr(),

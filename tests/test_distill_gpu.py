@@ -179,11 +179,14 @@ def test_a_class_named_twice():
         check(args, both[0], both[1], dy, 2.0, alpha)
 
 
-@pytest.mark.parametrize("k", [1, 31, 33, 1000, 1024])
-def test_long_lists_of_entries(k):
-    pred, teacher, ids, lab, dy = make(3, 2000, k, BF16)
+@pytest.mark.parametrize("v", [2000, 9001, 40000])
+@pytest.mark.parametrize("k", [1, 31, 33, 63, 64, 65, 1000, 1024])
+def test_long_lists_of_entries(v, k):
+    pred, teacher, ids, lab, dy = make(3, v, k, BF16)
     both = op.distill_loss_with_dpred(dy, pred, teacher, ids, temperature=2.0)
     check((pred, teacher, ids, None), both[0], both[1], dy, 2.0)
+    stats = op.distill_loss(pred, teacher, ids, temperature=2.0)[1]
+    check((pred, teacher, ids, None), None, op.distill_loss_dpred(dy, pred, teacher, ids, stats, temperature=2.0), dy, 2.0)
     ids.fill_(7)  # all of them one class
     both = op.distill_loss_with_dpred(dy, pred, teacher, ids, temperature=2.0)
     check((pred, teacher, ids, None), both[0], both[1], dy, 2.0)
@@ -244,6 +247,37 @@ def test_a_term_without_weight_counts_nothing():
     assert float(hard[0][1]) == math.inf and bool(hard[0][[0, 2, 3]].isfinite().all()) and bool(hard[1].isfinite().all())
     assert float(soft[0][0]) == math.inf and bool(soft[0][[1, 2, 3]].isfinite().all()) and bool(soft[1].isfinite().all())
     assert torch.equal(soft[1][2:], op.distill_loss_with_dpred(dy, pred, teacher, ids, temperature=2.0)[1][2:])
+
+
+@pytest.mark.parametrize("n,v,dtype", [(3, 1000003, BF16), (2, 600001, F32), (310, 131073, F16), (200, 70001, F32)])
+def test_rows_that_several_blocks_hold(n, v, dtype):
+    """Few rows, and rows that are too long for the caches of a block each."""
+    pred, teacher, _, lab, dy = make(n, v, 0, dtype, labels=True, pad=3)
+    ids = torch.randint(0, v, (n, 5), device="cuda")
+    teacher = torch.randn(n, 5, device="cuda")
+    ids[:, 0], ids[:, 1] = 0, v - 1
+    how = dict(labels=lab, temperature=2.0, alpha=0.5)
+    both = op.distill_loss_with_dpred(dy, pred, teacher, ids, **how)
+    check((pred, teacher, ids, lab), both[0], both[1], dy, 2.0, 0.5)
+    loss, stats = op.distill_loss(pred, teacher, ids, **how)
+    check((pred, teacher, ids, lab), loss, op.distill_loss_dpred(dy, pred, teacher, ids, stats, **how), dy, 2.0, 0.5)
+
+
+@pytest.mark.parametrize("v", [40, 3001, 30001])
+def test_rows_of_one_value_alone(v):
+    """A row of nothing but the type's lowest value, or of one other, says nothing: every class is as likely."""
+    for dtype in (F32, F16, BF16):
+        pred, teacher, ids, lab, dy = make(4, v, 3, dtype, labels=True)
+        pred[0], pred[1], pred[2] = torch.finfo(dtype).min, torch.finfo(dtype).max, 0.0
+        teacher[3, 1], ids[3, 1] = math.nan, -1  # what is absent may be anything
+        for temperature, alpha in ((1.0, 0.5), (2.0, 0.5), (0.7, 0.5), (1.0, 1.0)):
+            how = dict(labels=lab, temperature=temperature, alpha=alpha)
+            both = op.distill_loss_with_dpred(dy, pred, teacher, ids, **how)
+            same = pred.clone()
+            same[:3] = 0.0  # the definition of a constant row, without what 64 bits make of its subtractions
+            t = teacher.clone()
+            t[3, 1] = 0.0
+            check((same, t, ids, lab), both[0], both[1], dy, temperature, alpha)
 
 
 @pytest.mark.parametrize("shift", [0.0, 300.0, -3000.0])
