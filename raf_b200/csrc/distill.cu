@@ -23,7 +23,7 @@ namespace rafb200 {
 // them.  So two elements are computed by one instruction (f32x2), maxima are taken on the raw pairs, and where the second
 // exponential is a small power of the first (T = 2 or 4) it is multiplied out.
 constexpr int kDistillUnroll = 4;  // the rests of one to three groups are written out
-constexpr int kDistillRing = 3 * kDistillUnroll;  // groups of a thread on their way in
+constexpr int kDistillRing = 2 * kDistillUnroll;  // groups of a thread on their way in: a third batch leaves less L1 (328 -> 338 us)
 constexpr int kSweepThreads = 1024;  // of an SM, at least
 constexpr int kMaxTeacher = 1024;
 constexpr float kLog2e = 1.4426950408889634f;
@@ -550,7 +550,7 @@ __device__ __forceinline__ void leave_out(const DistillArgs& a, int64_t row, int
 // Loss, and with GRAD the gradient, of a row by a cluster of 2^slices_log blocks: one pass with a running maximum and its
 // sums, joined over threads, warps and blocks.
 // GRAD reads the logits a second time, from the L2: the launch sees to it that it holds what the resident blocks work on.
-// 8192 rows of 50257 (bf16, T = 2, labels), loss and gradient: 327 us (5.1 TB/s of what has to be read and written), with
+// 8192 rows of 50257 (bf16, T = 2, labels), loss and gradient: 316 us (5.2 TB/s of what has to be read and written), with
 // gradient rows that lie otherwise than the logits do.  Slices kept in shared memory instead, which
 // leave room for two blocks an SM: 450 us, 590 us with the next row on its way meanwhile - 16 warps an SM are too few for
 // the arithmetic.  The loss alone, 4096 rows of 30522: 55 us (4.6 TB/s), fp32 6.0 TB/s: 16-bit logits give every byte twice the
@@ -601,8 +601,8 @@ __global__ void __launch_bounds__(NT + 32, kSweepThreads / NT) distill_kernel(Di
   const float weight = GRAD && a.dy ? a.dy[row * a.dy_step] : 1.f;
   Sweep<T, S> sweep;
   stream.run([&](int, const uint4* place, int left) { sweep.batch(place, NT, left, a.c); });
-  // 32-bit logits stream a second time (8192 rows of 50257: 5.5 instead of 5.0 TB/s); 16-bit ones do better with loads (327 us
-  // instead of 340 us)
+  // 32-bit logits stream a second time (4096 rows of 50304: 5.5 instead of 5.0 TB/s); 16-bit ones do better with loads (8192
+  // rows of 50257 in bf16: 327 instead of 340 us)
   constexpr bool kStreamed = GRAD && sizeof(T) == 4;
   if (kStreamed && alike(z, out)) stream.begin();
   sweep.finish();
