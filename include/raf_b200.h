@@ -334,7 +334,7 @@ RAFB200_API int rafb200_defuse_tensor(int k, void* const* dst, const int64_t* nu
 /* The two ends of a model                                                    */
 /* ------------------------------------------------------------------------- */
 /* raf.op.embedding with a scale: out[i, :] = scale * x[indices[i], :], rounded once to out_dtype.
- * x [rows, width] and out [n, width] are compact.  An index outside [0, rows) reads as a row of zeros
+ * x [rows, width] and out [n, width] are compact, and out overlaps no input.  An index outside [0, rows) reads as a row of zeros
  * (a shard of the table sees the tokens of other shards so). */
 RAFB200_API int rafb200_embedding(const void* x, int x_dtype, int64_t rows, int64_t width,
                                   const void* indices, int index_dtype, int64_t n, float scale,
@@ -344,7 +344,8 @@ RAFB200_API int rafb200_embedding(const void* x, int x_dtype, int64_t rows, int6
  * to padding_idx and those outside [0, rows) count nothing.
  * Sums are fp32 and rounded once; their order is fixed by the indices alone, so equal calls give
  * equal bits.  `workspace` (16-byte aligned, at least rafb200_embedding_dx_workspace_bytes) is written by
- * the call and holds nothing between calls.  n and rows are below 2^31. */
+ * the call and holds nothing between calls; calls that may run at the same time take one each.  n and rows are
+ * below 2^31; dx overlaps no input. */
 RAFB200_API size_t rafb200_embedding_dx_workspace_bytes(int64_t n, int64_t width);
 RAFB200_API int rafb200_embedding_dx(const void* dy, int dy_dtype, const void* indices, int index_dtype,
                                      int64_t n, int64_t rows, int64_t width, float scale,

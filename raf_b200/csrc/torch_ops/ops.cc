@@ -526,7 +526,6 @@ PyObject* embedding_dx(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (given->dim() != 2 || given->size(0) != rows || given->size(1) != width || given->scalar_type() != type || overlap(ranges))
       return nothing();
   }
-  PyObject* held = given ? Py_NewRef(a[6]) : nullptr;
   at::Tensor made;
   int rc;
   {
@@ -540,11 +539,8 @@ PyObject* embedding_dx(PyObject*, PyObject* const* a, Py_ssize_t n) {
     rc = abi.embedding_dx(dy->const_data_ptr(), code, ids->const_data_ptr(), index, ids->numel(), rows, width, (float)scale, padding,
                           accumulate, out.mutable_data_ptr(), code_of(type), workspace.get(), bytes, current_stream(dev));
   }
-  if (rc != RAFB200_OK) {
-    Py_XDECREF(held);
-    return PyLong_FromLong(rc);
-  }
-  return given ? held : THPVariable_Wrap(std::move(made));
+  if (rc != RAFB200_OK) return PyLong_FromLong(rc);
+  return given ? Py_NewRef(a[6]) : THPVariable_Wrap(std::move(made));
 }
 
 // distill(dy or None, pred, teacher_logits, teacher_ids, stats or None, labels or None, temperature, alpha, ignore_index, grad_scale, what)

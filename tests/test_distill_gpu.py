@@ -1,15 +1,17 @@
 """The distillation loss and its gradient against the definition in 64 bits.
 
-Where the allowances come from, with u = 2^-24 (half a step of fp32) and A the largest |z - max z| log2(e) / T of a
+Where the allowances come from, with u = 2^-24 (half a step of fp32) and A the largest |z - max z| log2(e) / min(T, 1) of a
 row that still matters (2^-126 is flushed to zero):
-  an exponential    its argument is one rounded product and a rounded constant: 2 A u in base 2, 2 A u ln 2 < 2 A u
-                    relative; ex2.approx: 2 ulp = 4 u
-  a sum             a thread adds v / 512 terms of a block's share and merges them over a loop of 4 groups, 32 lanes, 16 warps and 8
-                    blocks: v / 512 + 64 additions, each with a rescaling of 4 u
+  an exponential    its argument is a rounded difference times a rounded constant, rounded: 3 A u in base 2, which is below 3 A u
+                    relative; ex2.approx: 2 ulp = 4 u.  What is multiplied out of it (T = 2, 4) has its argument's error four
+                    times at most with A a quarter, and 16 u + 3 u
+  a sum             a thread of 128 or more keeps two sums of v / 256 terms at most, a lane of a short row sums of 32; they are merged
+                    over 32 lanes, 8 warps, 8 blocks and rests: v / 256 + 64 additions, and a rescaling of 4 u with a batch of 32 terms
+                    and with each merger
   a quotient        both of these, and a rounding
-That is `r` below, relative, for q, r and the teacher's p.  The gradient is a difference of such terms, each off by r of
-itself, and is rounded once to the result's type.  A logarithm (2 ulp of a value below log2(v) + A, which also bounds what
-is subtracted) is off by 4 u (A + log2 v) + r.
+That is `r` below, relative, for q, r and the teacher's p: (v / 512 + 64) * 5 u covers the additions and the rescalings.  The
+gradient is a difference of such terms, each off by r of itself, and is rounded once to the result's type.  A logarithm (2 ulp of
+a value below log2(v) + A, which also bounds what is subtracted) is off by 4 u (A + log2 v) + r.
 """
 import math
 
@@ -306,6 +308,19 @@ def test_more_than_32_bits_of_elements():
     check(args, None, grad[rows], None, 2.0)
     check(args, op.distill_loss_with_dpred(None, pred, teacher, ids, temperature=2.0, out=grad)[0][rows], temperature=2.0)
     check(args, None, grad[rows], None, 2.0)
+
+
+@pytest.mark.parametrize("v", [300, 9001])
+def test_a_class_may_be_the_one_that_is_left_out(v):
+    pred, teacher, ids, lab, dy = make(6, v, 4, BF16, labels=True, index=torch.int32)
+    lab[1:4] = 0
+    lab[4], lab[5] = -100, v + 7  # outside: left out as well
+    how = dict(labels=lab, temperature=2.0, alpha=0.5, ignore_index=0)
+    loss, stats = op.distill_loss(pred, teacher, ids, **how)
+    check((pred, teacher, ids, lab), loss, op.distill_loss_dpred(dy, pred, teacher, ids, stats, **how), dy, 2.0, 0.5, ignore=0)
+    both = op.distill_loss_with_dpred(dy, pred, teacher, ids, **how)
+    check((pred, teacher, ids, lab), both[0], both[1], dy, 2.0, 0.5, ignore=0)
+    assert bool((both[0][1:] == 0).all()) and bool((both[1][1:] == 0).all()) and float(loss[0]) != 0
 
 
 def test_weights_of_rows_and_shapes():
