@@ -9,8 +9,8 @@ namespace rafb200 {
 //   out[n, :] = scale * x[id_n, :], a row of zeros where id_n is outside [0, rows)
 // Bound: HBM, the rows read and the rows written.  A warp takes kLookupRows rows and has four accesses of 32 lanes in
 // flight, at 32 to 48 registers a thread.  65536 rows of 1024 (bf16, 20000 different ones): 29.5 us, 5.7 TB/s of what has to
-// be read and written, where a copy of as many bytes takes 5.5 TB/s.  Rows of 1023: 38 us; from fp32 into bf16, element by
-// element, 20011 rows of 1023 23 us (2.9 TB/s).
+// be read and written, where a copy of as many bytes takes 5.5 TB/s.  Rows of 1023: 40 us; from fp32 into bf16, 20011 rows of
+// 1023 20.4 us (3.2 TB/s).
 constexpr int kLookupThreads = 256;
 constexpr int kLookupRows = 2;
 
@@ -31,45 +31,53 @@ __device__ __forceinline__ void lookup_groups(const T* from, O* to, int64_t left
   }
 }
 
-// Rows of one type that begin anywhere: 16 bytes written at a time, out of the two aligned 16-byte groups that hold them.
-template <typename T, int Q>
-__device__ __forceinline__ void lookup_shifted(const Slice<T>& s, const T* from, T* to, float scale, int lane) {
-  constexpr int kUnroll = 4, kPer = Slice<T>::kPer;
-  const char* source = reinterpret_cast<const char*>(from + s.at);
-  uint4* out = reinterpret_cast<uint4*>(to + s.at);
+// Rows that begin anywhere: kPiece elements at a time, written to aligned addresses out of the aligned 16-byte groups that
+// hold them, the first 4 Q + 0 or 2 bytes behind a boundary (Q < 0: at one).
+template <typename T, typename O>
+constexpr int kPiece = sizeof(T) == 4 && sizeof(O) == 4 ? 4 : 8;
+
+template <typename T, typename O, int Q>
+__device__ __forceinline__ void lookup_pieces(const T* from, O* to, int pieces, float scale, int lane) {
+  constexpr int kPer = 16 / sizeof(T), kParts = kPiece<T, O> / kPer, kUnroll = 4 / kParts;
+  const char* source = reinterpret_cast<const char*>(from);
   const uint32_t bits = (reinterpret_cast<uintptr_t>(source) & 3) * 8;
-  for (int i = lane; i < s.groups; i += 32 * kUnroll) {
-    uint4 w[kUnroll];
+  for (int i = lane; i < pieces; i += 32 * kUnroll) {
+    uint4 w[kUnroll][kParts];
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) w[u] = load_shifted<Q>(source + (int64_t)min(i + u * 32, s.groups - 1) * 16, bits);
+    for (int u = 0; u < kUnroll; ++u)
+#pragma unroll
+      for (int q = 0; q < kParts; ++q)
+        w[u][q] = load_shifted<Q>(source + ((int64_t)min(i + u * 32, pieces - 1) * kParts + q) * 16, bits);
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
-      float x[kPer];
-      Group<T, kPer>::unpack(w[u], x);
+      Group<O, kPiece<T, O>> o;
 #pragma unroll
-      for (int j = 0; j < kPer; ++j) x[j] *= scale;
-      if (i + u * 32 < s.groups) out[i + u * 32] = Group<T, kPer>::pack(x);
+      for (int q = 0; q < kParts; ++q) Group<T, kPer>::unpack(w[u][q], o.x + q * kPer);
+#pragma unroll
+      for (int j = 0; j < kPiece<T, O>; ++j) o.x[j] *= scale;
+      if (i + u * 32 < pieces) o.store(to + (int64_t)(i + u * 32) * kPiece<T, O>);
     }
   }
 }
-template <typename T>
-__device__ __forceinline__ void lookup_anywhere(const T* from, T* to, int width, float scale, int lane) {
-  Slice<T> s(from, width, 0, 0);
-  if (alike(from, static_cast<const T*>(to))) {
-    lookup_shifted<T, -1>(s, from, to, scale, lane);
-  } else {
-    s = s.aligned_at(to);
-    switch ((reinterpret_cast<uintptr_t>(from + s.at) & 15) >> 2) {
-      case 0: lookup_shifted<T, 0>(s, from, to, scale, lane); break;
-      case 1: lookup_shifted<T, 1>(s, from, to, scale, lane); break;
-      case 2: lookup_shifted<T, 2>(s, from, to, scale, lane); break;
-      default: lookup_shifted<T, 3>(s, from, to, scale, lane); break;
+// A row by one warp; 24 elements at least.
+template <typename T, typename O>
+__device__ __forceinline__ void lookup_anywhere(const T* from, O* to, int width, float scale, int lane) {
+  int at = (int)((-(intptr_t)to & 15) / sizeof(O)), pieces = (width - at) / kPiece<T, O>;
+  const uint32_t shift = reinterpret_cast<uintptr_t>(from + at) & 15;
+  if (shift) {  // the first and the last piece element by element: the groups that hold the others lie inside the row
+    at += kPiece<T, O>;
+    pieces -= 2;
+    switch (shift >> 2) {
+      case 0: lookup_pieces<T, O, 0>(from + at, to + at, pieces, scale, lane); break;
+      case 1: lookup_pieces<T, O, 1>(from + at, to + at, pieces, scale, lane); break;
+      case 2: lookup_pieces<T, O, 2>(from + at, to + at, pieces, scale, lane); break;
+      default: lookup_pieces<T, O, 3>(from + at, to + at, pieces, scale, lane); break;
     }
+  } else {
+    lookup_pieces<T, O, -1>(from + at, to + at, pieces, scale, lane);
   }
-  if (lane < s.edges()) {
-    const int j = s.edge_at(lane);
-    to[j] = Elem<T>::from_f32(Elem<T>::to_f32(from[j]) * scale);
-  }
+  const int j = lane < at ? lane : lane + pieces * kPiece<T, O>;  // 30 elements at most
+  if (j < width) to[j] = Elem<O>::from_f32(Elem<T>::to_f32(from[j]) * scale);
 }
 
 template <typename T, typename O, int VEC>
@@ -89,9 +97,9 @@ __global__ void __launch_bounds__(kLookupThreads)
     O* to = out + (first + r) * width;
     if ((uint64_t)id[r] < (uint64_t)rows) {
       const T* from = x + id[r] * width;
-      if constexpr (std::is_same<T, O>::value && VEC < 16 / (int)sizeof(T)) {
-        if (width * (int)sizeof(T) >= 512 && width < ((int64_t)1 << 31)) {  // shorter rows leave lanes without a group
-          lookup_anywhere<T>(from, to, (int)width, scale, lane);
+      if constexpr (VEC < 16 / (int)sizeof(T)) {
+        if (width >= 256 && width < ((int64_t)1 << 31)) {  // shorter rows leave lanes without a piece
+          lookup_anywhere<T, O>(from, to, (int)width, scale, lane);
           continue;
         }
       }

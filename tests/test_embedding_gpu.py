@@ -88,6 +88,23 @@ def test_lookup(n, rows, width, dtype, out_dtype):
         assert bool(((got.double() - want).abs() <= slack + rounding(out_dtype, want.abs() + slack)).all())
 
 
+@pytest.mark.parametrize("width", [255, 256, 257, 300, 1022, 1029])
+@pytest.mark.parametrize("dtype,out_dtype", [(F32, F32), (F32, BF16), (F16, F16), (F16, F32), (BF16, BF16), (BF16, F16)])
+def test_wide_rows_at_any_address(width, dtype, out_dtype):
+    g = torch.Generator(device="cuda").manual_seed(width)
+    n, rows = 57, 30
+    ids = ids_of("outside", n, rows, g)
+    for a, b in ((0, 0), (1, 0), (0, 1), (3, 2), (7, 5)):
+        x = torch.randn(rows * width + a, generator=g, device="cuda").to(dtype)[a:].view(rows, width)
+        room = torch.full((n * width + b + 9,), 7.0, dtype=out_dtype, device="cuda")
+        out = room[b:b + n * width].view(n, width)
+        op.embedding(x, ids, 0.75, dtype=out_dtype, out=out)
+        want = lookup_of(x, ids, 0.75)
+        slack = want.abs() * HALF32
+        assert bool(((out.double() - want).abs() <= slack + rounding(out_dtype, want.abs() + slack)).all())
+        assert bool((room[:b] == 7).all()) and bool((room[b + n * width:] == 7).all())
+
+
 @pytest.mark.parametrize("shift", [1, 2, 4])
 def test_tables_and_results_at_any_address(shift):
     g = torch.Generator(device="cuda").manual_seed(shift)
