@@ -40,7 +40,8 @@ struct DistillArgs {
   Ids labels;       // p == nullptr: none
   const float* dy;  // one weight per row (dy_step 1), one for all (0), or nullptr: 1
   float* loss;
-  float4* stats;    // per row: maximum, sum of exponentials at the temperature, the same at one, sum of the teacher's weights - 1
+  float4* stats;    // per row: maximum, sum of exponentials at the temperature, the same at one; the fourth is within a launch the
+                    // sum of the teacher's weights - 1, which no other launch reads
   void* out;
   int64_t n, v, ld, ld_out, ignore;
   int k, teacher_type, dy_step;
@@ -613,7 +614,8 @@ __global__ void __launch_bounds__(NT + 32, kSweepThreads / NT) distill_kernel(Di
   bar_arrive<NT + 32>(kWritten);
 }
 
-// The gradient from the statistics that the forward pass has left.
+// The gradient from the maximum and the sums that the forward pass has left.  What the teacher's weights sum to (0 for a row
+// without one) is taken from its entries, which are at hand.
 constexpr int kDpredThreads = 128;
 template <typename T, Second S>
 __global__ void __launch_bounds__(kDpredThreads + 32, 6) distill_dpred_kernel(DistillArgs a) {
@@ -631,27 +633,29 @@ __global__ void __launch_bounds__(kDpredThreads + 32, 6) distill_dpred_kernel(Di
     if (tid < NT) zero_slice<T, NT>(Slice<T>(out, (int)a.v, slice, a.slices_log), out, tid);
     return;
   }
+  __shared__ float some;
   const Slice<T> s(z, (int)a.v, slice, a.slices_log);
-  const float4 stats = a.stats[row];
+  float4 stats = a.stats[row];
   const float weight = a.dy ? a.dy[row * a.dy_step] : 1.f;
-  const bool in_place = a.out == a.pred;
   if (tid < NT) {
     const float edge = tid < s.edges() ? Elem<T>::to_f32(z[s.edge_at(tid)]) : 0.f;
     Stream<T, NT> stream(s, z, image);
     if (alike(z, out)) stream.begin();
-    const Coefficients co = coefficients<S>(a, weight, stats, labels);
-    if (in_place) bar_sync<NT + 32>(kWeighed);  // the entries of this slice are read (those of others are not used here)
-    write_slice<T, S, NT, true>(s, z, edge, out, co, stream);
+    bar_sync<NT + 32>(kWeighed);  // out may be pred: the entries of this slice are read (those of others are not used here)
+    stats.w = some;
+    write_slice<T, S, NT, true>(s, z, edge, out, coefficients<S>(a, weight, stats, labels), stream);
     bar_arrive<NT + 32>(kWritten);
     return;
   }
   const Entries e(image + Stream<T, NT>::kPlaces, a.k);
   load_entries(a, e, row, z, label);
-  if (in_place) bar_arrive<NT + 32>(kWeighed);
+  stats.w = weigh(e, a.k, a.c) - 1.f;
+  if (tid == NT) some = stats.w;
+  __syncwarp();
+  bar_arrive<NT + 32>(kWeighed);
   bool mine = false;
   for (int i = tid - NT; i <= a.k; i += 32) mine |= e.at[i] >= 0 && s.owns(e.at[i]);
   mine = __any_sync(0xffffffffu, mine);
-  if (mine) weigh(e, a.k, a.c);
   const bool different = mine && all_different(e, a.k);
   bar_sync<NT + 32>(kWritten);
   if (mine) write_entries<T, S>(a, e, s, out, coefficients<S>(a, weight, stats, labels), different);
@@ -718,9 +722,10 @@ __global__ void __launch_bounds__(32 * kShortWarps, 6) distill_short_kernel(Dist
     }
     soft = warp_sum(soft);
     if (S != kNone) hard = warp_sum(hard);
-    stats = make_float4(top, soft, S != kNone ? hard : soft, some);
-    put_loss(a, e, row, stats, labels);
+    stats = make_float4(top, soft, S != kNone ? hard : soft, 0.f);
   }
+  stats.w = some;
+  if (P != kDpred) put_loss(a, e, row, stats, labels);
   if (P == kLoss) return;
   const Coefficients co = coefficients<S>(a, weight, stats, labels);
   if (alike(z, out)) {

@@ -413,3 +413,19 @@ def test_refusals_on_the_gpu():
     room = torch.zeros(6, 80, device="cuda")
     with pytest.raises(_lib.RafB200Error, match="overlaps"):
         op.distill_loss_with_dpred(dy, room[:, :40], teacher, ids, out=room[:, 40:])
+
+
+@pytest.mark.parametrize("v", [300, 9001, 50257])
+def test_statistics_from_elsewhere(v):
+    """Maximum and sums by another program, nothing in the fourth place: whether a row has a teacher is read from its list."""
+    for labels, temperature in ((False, 2.0), (True, 2.0), (False, 1.0)):
+        pred, teacher, ids, lab, dy = make(7, v, 2, BF16, labels=labels)
+        ids[2:5] = -1
+        ids[5, 0] = v
+        z = pred.double()
+        top = z.amax(1, keepdim=True)
+        stats = torch.stack([top[:, 0], ((z - top) / temperature).exp().sum(1), (z - top).exp().sum(1), torch.zeros_like(dy)], 1).float()
+        how = dict(labels=lab, temperature=temperature, alpha=0.5 if labels else 1.0)
+        for into in (None, pred.clone()):
+            z = pred if into is None else into
+            check((pred, teacher, ids, lab), None, op.distill_loss_dpred(dy, z, teacher, ids, stats, out=into, **how), dy, temperature, how["alpha"])
