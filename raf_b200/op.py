@@ -559,7 +559,8 @@ def distill_loss(pred, teacher_logits, teacher_ids, labels=None, temperature=1.0
     [0, v) is absent.  Without ``labels`` alpha is 1.  A row whose label is ``ignore_index`` or outside [0, v) has loss
     and gradient 0.  Rows of ``pred`` may lie further apart than v (logits padded for a matrix product).
 
-    ``stats`` is what :func:`distill_loss_dpred` takes.  Where ``pred`` requires a gradient, backward calls it.
+    ``stats`` is what :func:`distill_loss_dpred` takes: a row's maximum, sum of ``exp((pred - max) / T)``, sum of
+    ``exp(pred - max)``, and a value that it does not read.  Where ``pred`` requires a gradient, backward calls it.
     """
     if stream is None:
         r = _lib.ops().distill(None, pred, teacher_logits, teacher_ids, None, labels, temperature, alpha, ignore_index, 1.0, 0)
