@@ -15,11 +15,14 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <dlfcn.h>
 
 #include <algorithm>
+#include <memory>
+#include <unordered_set>
 #include <vector>
 
 #include "../../../include/raf_b200.h"
@@ -625,6 +628,29 @@ PyObject* distill(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return out;
 }
 
+// reaches_default_stream(tensor): whether the tensor's autograd graph has a node of the default stream, a leaf's accumulator
+// that a graph built there keeps alive among them.  Backward runs such a node there, and the default stream cannot be part of a
+// capture: the engine's thread would end the process.
+PyObject* reaches_default_stream(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 1 || !THPVariable_Check(a[0])) return nothing();
+  const at::Tensor& t = THPVariable_Unpack(a[0]);
+  if (!t.defined() || !t.is_cuda() || !t.requires_grad()) return nothing();
+  const std::shared_ptr<torch::autograd::Node> first = t.grad_fn() ? t.grad_fn() : torch::autograd::impl::try_get_grad_accumulator(t);
+  std::vector<torch::autograd::Node*> left;
+  std::unordered_set<torch::autograd::Node*> seen;
+  if (first) left.push_back(first.get());
+  while (!left.empty()) {
+    torch::autograd::Node* const node = left.back();
+    left.pop_back();
+    if (!seen.insert(node).second) continue;
+    const auto stream = node->stream();
+    if (stream && stream->device_type() == c10::DeviceType::CUDA && c10::cuda::CUDAStream(*stream).stream() == nullptr) Py_RETURN_TRUE;
+    for (const auto& edge : node->next_edges())
+      if (edge.function) left.push_back(edge.function.get());
+  }
+  Py_RETURN_FALSE;
+}
+
 using Fast = PyObject* (*)(PyObject*, PyObject* const*, Py_ssize_t);
 
 // A C++ exception (the allocator out of memory, first of all) becomes the Python exception that
@@ -654,6 +680,7 @@ PyMethodDef kMethods[] = {
     {"embedding", fast<embedding>(), METH_FASTCALL, "raf.op.embedding"},
     {"embedding_dx", fast<embedding_dx>(), METH_FASTCALL, "raf.op.embedding_dx"},
     {"distill", fast<distill>(), METH_FASTCALL, "the distillation loss and its gradient"},
+    {"reaches_default_stream", fast<reaches_default_stream>(), METH_FASTCALL, "whether backward from a tensor can be captured: not if so"},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_ops", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};

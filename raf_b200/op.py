@@ -368,6 +368,13 @@ def _launching(t, stream, *others):
         yield torch._C._cuda_getCurrentRawStream(t.device.index)
 
 
+def _check_capturable(name, x):
+    """Before a node is put behind x: what backward could not be captured through is refused here, where an exception is one."""
+    if torch.cuda.is_current_stream_capturing() and _lib.ops().reaches_default_stream(x):
+        raise RuntimeError(f"{name}: under capture, but the input's autograd graph reaches into one that was built on the default "
+                           "stream and still lives, so its backward cannot be captured; drop that graph first, or detach the input")
+
+
 class _Embedding(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, indices, scale, padding_idx, dtype):
@@ -387,7 +394,8 @@ def embedding(x, indices, scale=1.0, padding_idx=None, dtype=None, out=None, str
 
     ``x`` is [rows, width] in fp32 / fp16 / bf16, ``indices`` any shape of int32 / int64; the result is of ``dtype``
     (default: x's), rounded once.  An index outside [0, rows) reads as a row of zeros.  Where ``x`` requires a
-    gradient, backward is :func:`embedding_dx`, for which ``padding_idx`` names an index that counts nothing.
+    gradient, backward is :func:`embedding_dx`, for which ``padding_idx`` names an index that counts nothing.  Forward and
+    backward may be captured in one graph while no eager graph of the same leaves lives; else the captured call is refused.
     """
     if out is None and stream is None:
         r = _lib.ops().embedding(x, indices, scale, dtype)
@@ -405,6 +413,7 @@ def embedding(x, indices, scale=1.0, padding_idx=None, dtype=None, out=None, str
         if out is not None:
             raise ValueError("embedding: out has no gradient; x must not require one")
         with _launching(x, stream, indices):  # autograd runs backward on the stream that is current here
+            _check_capturable("embedding", x)
             return _Embedding.apply(x, indices, scale, padding_idx, dtype)
     shape = indices.shape + x.shape[1:]
     if out is not None:
@@ -560,7 +569,8 @@ def distill_loss(pred, teacher_logits, teacher_ids, labels=None, temperature=1.0
     and gradient 0.  Rows of ``pred`` may lie further apart than v (logits padded for a matrix product).
 
     ``stats`` is what :func:`distill_loss_dpred` takes: a row's maximum, sum of ``exp((pred - max) / T)``, sum of
-    ``exp(pred - max)``, and a value that it does not read.  Where ``pred`` requires a gradient, backward calls it.
+    ``exp(pred - max)``, and a value that it does not read.  Where ``pred`` requires a gradient, backward calls it; for a captured backward
+    the condition of :func:`embedding` holds.
     """
     if stream is None:
         r = _lib.ops().distill(None, pred, teacher_logits, teacher_ids, None, labels, temperature, alpha, ignore_index, 1.0, 0)
@@ -573,6 +583,7 @@ def distill_loss(pred, teacher_logits, teacher_ids, labels=None, temperature=1.0
         raise ValueError("distill_loss: the teacher gets no gradient; detach its logits")
     if torch.is_grad_enabled() and pred.requires_grad:
         with _launching(pred, stream, teacher_logits, teacher_ids, labels):
+            _check_capturable("distill_loss", pred)
             return _DistillLoss.apply(pred, teacher_logits, teacher_ids, labels, temperature, alpha, ignore_index)
     with _launching(pred, stream, teacher_logits, teacher_ids, labels) as raw:
         loss = torch.empty(pred.shape[:-1], dtype=torch.float32, device=pred.device)
