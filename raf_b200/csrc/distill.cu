@@ -767,7 +767,7 @@ static DistillArgs device_args(const rafb200_distill* d) {
   a.v = d->v;
   a.ld = d->ld;
   a.ignore = d->ignore_index;
-  a.k = d->k;
+  a.k = d->alpha == 0.0 ? 0 : d->k;  // a teacher without weight is not looked at: 0 times its NaN would be NaN
   a.teacher_type = d->teacher_dtype;
   a.c = (float)(M_LOG2E / d->temperature);
   a.soft_loss = (float)(d->alpha * d->temperature * d->temperature);

@@ -429,3 +429,17 @@ def test_statistics_from_elsewhere(v):
         for into in (None, pred.clone()):
             z = pred if into is None else into
             check((pred, teacher, ids, lab), None, op.distill_loss_dpred(dy, z, teacher, ids, stats, out=into, **how), dy, temperature, how["alpha"])
+
+
+@pytest.mark.parametrize("v", [300, 9001, 40000])
+def test_a_teacher_without_weight_may_hold_anything(v):
+    """alpha = 0: neither loss nor gradient looks at the teacher's logits."""
+    pred, teacher, ids, lab, dy = make(5, v, 5, BF16, labels=True)
+    wild = teacher.clone()
+    wild[0, 1], wild[1], wild[2, 0], wild[3] = math.nan, math.nan, math.inf, -math.inf
+    for temperature in (1.0, 2.0, 3.0, 4.0):
+        how = dict(labels=lab, temperature=temperature, alpha=0.0)
+        loss, stats = op.distill_loss(pred, wild, ids, **how)
+        check((pred, teacher, ids, lab), loss, op.distill_loss_dpred(dy, pred, wild, ids, stats, **how), dy, temperature, 0.0)
+        both = op.distill_loss_with_dpred(dy, pred, wild, ids, **how)
+        check((pred, teacher, ids, lab), both[0], both[1], dy, temperature, 0.0)
