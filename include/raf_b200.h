@@ -361,7 +361,8 @@ RAFB200_API int rafb200_embedding_dx(const void* dy, int dy_dtype, const void* i
  *                   entries (or with logits of -infinity only) has no teacher term.
  *   labels          [n], or NULL (then alpha must be 1).  A row whose label equals ignore_index or lies
  *                   outside [0, v) has loss 0 and gradient 0, whatever its logits hold.
- * Logits of -infinity are classes of probability 0; a row of nothing else, +infinity and NaN give NaN.
+ * Logits of -infinity are classes of probability 0; a row of nothing else, +infinity and NaN give NaN.  A row without either term
+ * has loss 0 and gradient 0, but for a gradient of NaN where a logit is +infinity or NaN.
  * Everything is computed in fp32, exponentials to 2 ulp; the teacher's term is a difference of logarithms times T^2,
  * whose absolute error grows so.
  * A term whose weight (alpha, 1 - alpha) is 0 counts nothing. */

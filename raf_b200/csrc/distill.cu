@@ -236,10 +236,12 @@ __device__ __forceinline__ Coefficients coefficients(const DistillArgs& a, float
   co.base = base_of(stats.x);
   co.teach = w * a.soft_grad;
   co.hit = labels ? w * a.hard : 0.f;
-  co.soft = co.teach * (stats.w + 1.f) / stats.y;
-  co.hard = co.hit / stats.z;
+  // a term that the row does not have is 0, whatever its sums are: those of nothing but -infinity are 0 themselves
+  const bool taught = stats.w != -1.f, hit = labels && a.hard != 0.f;
+  co.soft = taught ? co.teach * (stats.w + 1.f) / stats.y : 0.f;
+  co.hard = hit ? co.hit / stats.z : 0.f;
   if (S == kNone) {  // one exponential serves both terms, or there is one term only
-    co.soft += labels ? co.hit / stats.y : 0.f;
+    co.soft += hit ? co.hit / stats.y : 0.f;
     co.hard = 0.f;
   }
   return co;

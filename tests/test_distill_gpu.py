@@ -443,3 +443,19 @@ def test_a_teacher_without_weight_may_hold_anything(v):
         check((pred, teacher, ids, lab), loss, op.distill_loss_dpred(dy, pred, wild, ids, stats, **how), dy, temperature, 0.0)
         both = op.distill_loss_with_dpred(dy, pred, wild, ids, **how)
         check((pred, teacher, ids, lab), both[0], both[1], dy, temperature, 0.0)
+
+
+@pytest.mark.parametrize("v", [300, 9001, 40000])
+@pytest.mark.parametrize("temperature", [1.0, 2.0])
+def test_a_row_without_any_term_says_nothing(v, temperature):
+    """No teacher, and no labels or no weight for them: loss and gradient 0, for a row of nothing but -infinity too."""
+    pred, teacher, ids, lab, dy = make(5, v, 5, F16, labels=True)
+    pred[:2] = -math.inf
+    ids[0], ids[2], teacher[1] = -1, v, -math.inf
+    for labels in (None, lab):
+        how = dict(labels=labels, temperature=temperature, alpha=1.0)
+        loss, stats = op.distill_loss(pred, teacher, ids, **how)
+        both = op.distill_loss_with_dpred(dy, pred, teacher, ids, **how)
+        for x, d in ((loss, op.distill_loss_dpred(dy, pred, teacher, ids, stats, **how)), both):
+            assert bool((x[:3] == 0).all()) and bool((d[:3] == 0).all())
+            check((pred[3:], teacher[3:], ids[3:], None if labels is None else lab[3:]), x[3:], d[3:], dy[3:], temperature)
