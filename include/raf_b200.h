@@ -379,7 +379,9 @@ typedef struct {
   int pred_dtype, teacher_dtype, ids_dtype, labels_dtype;
 } rafb200_distill;
 /* loss [n] fp32; stats [n, 4] fp32, 16-byte aligned: what rafb200_distill_loss_dpred takes - a row's maximum z, sum of
-   exp((z - max) / T), sum of exp(z - max), and a value that it does not read. */
+   exp((z - max) / T), sum of exp(z - max), and a value that it does not read.  What the loss does not
+   sum up is NaN, and so is a gradient that takes it: the third where T is not 1 and there is no hard term (no labels, or alpha 1),
+   all of them in a row whose label leaves it out. */
 RAFB200_API int rafb200_distill_loss(const rafb200_distill* d, float* loss, float* stats, void* stream);
 /* dpred[i, :] = dy[i] * grad_scale * d loss[i] / d pred[i, :], in pred's type, rows ld_dpred elements
  * apart; what lies between the rows is left alone.  dy: one fp32 weight per row (dy_step 1), one for all rows

@@ -40,8 +40,8 @@ struct DistillArgs {
   Ids labels;       // p == nullptr: none
   const float* dy;  // one weight per row (dy_step 1), one for all (0), or nullptr: 1
   float* loss;
-  float4* stats;    // per row: maximum, sum of exponentials at the temperature, the same at one; the fourth is within a launch the
-                    // sum of the teacher's weights - 1, which no other launch reads
+  float4* stats;    // per row: maximum, sum of exponentials at the temperature, the same at one (NaN if not summed up); the fourth is
+                    // within a launch the sum of the teacher's weights - 1, which no other launch reads
   void* out;
   int64_t n, v, ld, ld_out, ignore;
   int k, teacher_type, dy_step;
@@ -132,6 +132,12 @@ __device__ __forceinline__ void rebase(Running& x, float top, float c) {
   }
   x.top = top;
 }
+
+// What the loss has not summed up is NaN in the statistics: a gradient that takes it (with other labels or another alpha) is NaN
+// rather than one from another sum.
+__device__ __forceinline__ float not_summed() { return __int_as_float(0x7fffffff); }
+// The sum at one where a single one is kept, at the temperature.
+__device__ __forceinline__ float sum_at_one(const DistillArgs& a, float soft) { return a.c == kLog2e ? soft : not_summed(); }
 
 // Copies 16 bytes to shared memory without waiting; a thread waits for all but its last N batches of copies.
 __device__ __forceinline__ void copy_async(void* to, const void* from) {
@@ -523,7 +529,7 @@ __device__ __forceinline__ float4 join(Exchange<NT / 32>& x, Running run, const 
       run.hard += part.hard;
     }
   }
-  return make_float4(run.top, run.soft, S != kNone ? run.hard : run.soft, x.some);
+  return make_float4(run.top, run.soft, S != kNone ? run.hard : sum_at_one(a, run.soft), x.some);
 }
 
 // The loss of a row, by one warp.
@@ -544,7 +550,7 @@ template <typename T, int NT, bool GRAD>
 __device__ __forceinline__ void leave_out(const DistillArgs& a, int64_t row, int slice, int tid) {
   if (slice == 0 && tid == 0) {
     a.loss[row] = 0.f;
-    if (a.stats) a.stats[row] = make_float4(0.f, 1.f, 1.f, -1.f);
+    if (a.stats) a.stats[row] = make_float4(not_summed(), not_summed(), not_summed(), not_summed());
   }
   T* out = static_cast<T*>(a.out) + row * a.ld_out;
   if (GRAD) zero_slice<T, NT>(Slice<T>(out, (int)a.v, slice, a.slices_log), out, tid);
@@ -724,7 +730,7 @@ __global__ void __launch_bounds__(32 * kShortWarps, 6) distill_short_kernel(Dist
     }
     soft = warp_sum(soft);
     if (S != kNone) hard = warp_sum(hard);
-    stats = make_float4(top, soft, S != kNone ? hard : soft, 0.f);
+    stats = make_float4(top, soft, S != kNone ? hard : sum_at_one(a, soft), 0.f);
   }
   stats.w = some;
   if (P != kDpred) put_loss(a, e, row, stats, labels);

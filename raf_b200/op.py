@@ -569,7 +569,8 @@ def distill_loss(pred, teacher_logits, teacher_ids, labels=None, temperature=1.0
     and gradient 0.  Rows of ``pred`` may lie further apart than v (logits padded for a matrix product).
 
     ``stats`` is what :func:`distill_loss_dpred` takes: a row's maximum, sum of ``exp((pred - max) / T)``, sum of
-    ``exp(pred - max)``, and a value that it does not read.  Where ``pred`` requires a gradient, backward calls it; for a captured backward
+    ``exp(pred - max)``, and a value that it does not read.  What this loss does not sum up is NaN, and so is a gradient that
+    takes it: the last sum where T is not 1 and there is no hard term, all of them in a row that its label leaves out.  Where ``pred`` requires a gradient, backward calls it; for a captured backward
     the condition of :func:`embedding` holds.
     """
     if stream is None:

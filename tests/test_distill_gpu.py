@@ -459,3 +459,30 @@ def test_a_row_without_any_term_says_nothing(v, temperature):
         for x, d in ((loss, op.distill_loss_dpred(dy, pred, teacher, ids, stats, **how)), both):
             assert bool((x[:3] == 0).all()) and bool((d[:3] == 0).all())
             check((pred[3:], teacher[3:], ids[3:], None if labels is None else lab[3:]), x[3:], d[3:], dy[3:], temperature)
+
+
+@pytest.mark.parametrize("v", [300, 9001, 40000])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_what_the_statistics_hold(v, dtype):
+    """A row's maximum, its sum at the temperature and its sum at one; NaN in place of what the loss does not sum up, and so is a
+    gradient that takes it."""
+    pred, teacher, ids, lab, dy = make(6, v, 3, dtype, labels=True)
+    z = pred.double()
+    top = z.amax(1)
+    sums = [((z - top[:, None]) / t).exp().sum(1) for t in (1.0, 2.0)]
+    for labels, temperature, alpha in ((None, 1.0, 1.0), (None, 2.0, 1.0), (lab, 1.0, 1.0), (lab, 2.0, 1.0), (lab, 1.0, 0.5), (lab, 2.0, 0.5), (lab, 2.0, 0.0)):
+        stats = op.distill_loss(pred, teacher, ids, labels, temperature, alpha)[1]
+        r, _ = allowances(v, 0, definition(pred, teacher, ids, None, 1.0, 1.0)[3], 1.0, 1.0)
+        assert torch.equal(stats[:, 0].double(), top)
+        assert bool(((stats[:, 1].double() - sums[int(temperature) - 1]).abs() <= r * sums[int(temperature) - 1]).all())
+        if temperature == 1.0 or alpha < 1:
+            assert bool(((stats[:, 2].double() - sums[0]).abs() <= r * sums[0]).all())
+        else:
+            assert bool(stats[:, 2].isnan().all())
+            assert bool(op.distill_loss_dpred(dy, pred, teacher, ids, stats, lab, temperature, 0.5).isnan().all())
+    lab[2], lab[4] = IGNORE, v
+    stats = op.distill_loss(pred, teacher, ids, lab, 2.0, 0.5)[1]
+    left_out = torch.tensor([False, False, True, False, True, False], device="cuda")
+    assert torch.equal(stats[:, :3].isnan().all(1), left_out) and torch.equal(stats[:, :3].isnan().any(1), left_out)
+    assert torch.equal(op.distill_loss_dpred(dy, pred, teacher, ids, stats, temperature=2.0).isnan().all(1), left_out)
+    assert bool((op.distill_loss_dpred(dy, pred, teacher, ids, stats, lab, 2.0, 0.5)[left_out] == 0).all())
