@@ -95,10 +95,16 @@ const at::Tensor* plain(PyObject* o, c10::DeviceIndex& device) {
   return t.device().index() == device && t.is_contiguous() ? &t : nullptr;
 }
 
+// The same without a tangent of forward mode.
+const at::Tensor* primal(PyObject* o, c10::DeviceIndex& device) {
+  const at::Tensor* t = plain(o, device);
+  return t && !t->_fw_grad(0).defined() ? t : nullptr;
+}
+
 // The same where the result belongs to no autograd graph, forward mode included.
 const at::Tensor* data_only(PyObject* o, c10::DeviceIndex& device) {
-  const at::Tensor* t = plain(o, device);
-  return t && !(t->requires_grad() && c10::GradMode::is_enabled()) && !t->_fw_grad(0).defined() ? t : nullptr;
+  const at::Tensor* t = primal(o, device);
+  return t && !(t->requires_grad() && c10::GradMode::is_enabled()) ? t : nullptr;
 }
 
 void* current_stream(c10::DeviceIndex device) { return c10::cuda::getCurrentCUDAStream(device).stream(); }
@@ -506,7 +512,7 @@ PyObject* embedding(PyObject*, PyObject* const* a, Py_ssize_t n) {
 PyObject* embedding_dx(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (n != 8 || !PyLong_Check(a[2])) return nothing();
   c10::DeviceIndex dev = -1;
-  const at::Tensor *dy = data_only(a[0], dev), *ids = plain(a[1], dev), *given = a[6] == Py_None ? nullptr : plain(a[6], dev);
+  const at::Tensor *dy = data_only(a[0], dev), *ids = plain(a[1], dev), *given = a[6] == Py_None ? nullptr : primal(a[6], dev);
   if (!dy || !ids || (a[6] != Py_None && !given)) return nothing();
   at::ScalarType type;
   if (!type_of(a[5], given ? given->scalar_type() : dy->scalar_type(), &type)) return nothing();
@@ -559,7 +565,7 @@ PyObject* distill(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return nothing();
   }
   auto optional = [&](PyObject* o, const at::Tensor*& t) {
-    t = o == Py_None ? nullptr : plain(o, dev);
+    t = o == Py_None ? nullptr : primal(o, dev);
     return o == Py_None || t;
   };
   const at::Tensor *teacher = data_only(a[2], dev), *ids = plain(a[3], dev), *dy, *stats, *labels;

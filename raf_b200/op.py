@@ -12,6 +12,7 @@ import ctypes as C
 from typing import List, Optional, Sequence
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import BF16, F16, F32, I32, I64, check
@@ -338,6 +339,17 @@ def _same_device(*tensors):
         raise ValueError("tensors must be on one device")
 
 
+def _check_values(what, *tensors):
+    """Tensors whose sign or tangent is not at their address: what is computed from there would be without it."""
+    for t in tensors:
+        if t is None:
+            continue
+        if t.is_neg():
+            raise ValueError(f"{what}: a tensor that is still to be negated; resolve_neg() it first")
+        if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
+            raise ValueError(f"{what}: there are no forward-mode derivatives, and a tensor has a tangent")
+
+
 def _span(t):
     """The bytes a tensor of positive strides reaches over."""
     if t.numel() == 0:
@@ -405,6 +417,7 @@ def embedding(x, indices, scale=1.0, padding_idx=None, dtype=None, out=None, str
             check(r)
     _check_cuda(x, indices)
     _same_device(x, indices)
+    _check_values("embedding", x, out)
     if x.dim() != 2:
         raise ValueError("embedding: x is a table, [rows, width]")
     dtype = x.dtype if dtype is None else torch_dtype(dtype)
@@ -449,6 +462,7 @@ def embedding_dx(dy, indices, num_weight, scale=1.0, padding_idx=None, dtype=Non
             check(r)
     _check_cuda(dy, indices)
     _same_device(dy, indices)
+    _check_values("embedding_dx", dy, out)
     if dy.dim() != indices.dim() + 1 or dy.shape[:-1] != indices.shape:
         raise ValueError("embedding_dx: dy has the shape of indices and one dimension more")
     num_weight, width = int(num_weight), dy.shape[-1]
@@ -502,6 +516,7 @@ def _distill_args(pred, teacher_logits, teacher_ids, labels, temperature, alpha,
     given = [teacher_logits, teacher_ids] + ([] if labels is None else [labels])
     _check_cuda(*given)
     _same_device(pred, *given)
+    _check_values("distill_loss", pred, teacher_logits)
     lead = pred.shape[:-1]
     if teacher_logits.dim() != pred.dim() or teacher_logits.shape[:-1] != lead or teacher_ids.shape != teacher_logits.shape:
         raise ValueError("distill_loss: teacher_logits and teacher_ids have pred's shape up to the last dimension, and each other's")
@@ -524,6 +539,7 @@ def _weights_of(dy, pred):
         return None, 0
     _check_cuda(dy)
     _same_device(pred, dy)
+    _check_values("distill_loss", dy)
     if dy.dtype != torch.float32:
         raise TypeError("dy is fp32")
     if dy.dim() == 0:
@@ -538,6 +554,7 @@ def _gradient_for(pred, out, others):
         return torch.empty(pred.shape, dtype=pred.dtype, device=pred.device), pred.shape[-1]
     rows, ld = _rows_of(out, "out")
     _same_device(pred, out)
+    _check_values("distill_loss", out)
     if out.shape != pred.shape or out.dtype != pred.dtype:
         raise ValueError(f"out is to be {tuple(pred.shape)} of {pred.dtype}")
     _check_apart(out, *(t for t in others if t is not None))
@@ -610,6 +627,7 @@ def distill_loss_dpred(dy, pred, teacher_logits, teacher_ids, stats, labels=None
     weights, step = _weights_of(dy, pred)
     _check_cuda(stats)
     _same_device(pred, stats)
+    _check_values("distill_loss", stats)
     if stats.shape != pred.shape[:-1] + (4,) or stats.dtype != torch.float32:
         raise ValueError("distill_loss_dpred: stats are those of distill_loss for this pred")
     with _launching(pred, stream, dy, teacher_logits, teacher_ids, stats, labels, out) as raw:

@@ -486,3 +486,31 @@ def test_what_the_statistics_hold(v, dtype):
     assert torch.equal(stats[:, :3].isnan().all(1), left_out) and torch.equal(stats[:, :3].isnan().any(1), left_out)
     assert torch.equal(op.distill_loss_dpred(dy, pred, teacher, ids, stats, temperature=2.0).isnan().all(1), left_out)
     assert bool((op.distill_loss_dpred(dy, pred, teacher, ids, stats, lab, 2.0, 0.5)[left_out] == 0).all())
+
+
+def test_forward_mode_and_lazy_signs_are_refused():
+    """Tensors whose tangent, or whose sign, is not at their address."""
+    import torch.autograd.forward_ad as fwd
+
+    pred, teacher, ids, lab, dy = make(6, 40, 3, F32, labels=True)
+    stats = op.distill_loss(pred, teacher, ids)[1]
+
+    def calls(z, t, w):
+        plain = z is pred and t is teacher
+        return ([] if plain else [lambda: op.distill_loss(z, t, ids), lambda: op.distill_loss(z, t, ids, stream=torch.cuda.current_stream())]) + [
+            lambda: op.distill_loss_dpred(w, z, t, ids, stats), lambda: op.distill_loss_with_dpred(w, z, t, ids),
+            lambda: op.distill_loss_dpred(w, z, t, ids, stats, out=torch.empty_like(pred))]
+
+    with fwd.dual_level():
+        z, t, w = (fwd.make_dual(x, torch.ones_like(x)) for x in (pred, teacher, dy))
+        for call in calls(z, teacher, dy) + calls(pred, t, dy) + calls(pred, teacher, w):
+            with pytest.raises(ValueError, match="forward"):
+                call()
+        with torch.no_grad(), pytest.raises(ValueError, match="forward"):
+            op.distill_loss(z, teacher, ids)
+        with pytest.raises(ValueError, match="forward"):
+            op.distill_loss(fwd.make_dual(pred.clone().requires_grad_(), torch.ones_like(pred)), teacher, ids)
+        assert torch.equal(op.distill_loss(pred, teacher, ids)[1], stats)
+    for call in calls(torch._neg_view(pred), teacher, dy) + calls(pred, torch._neg_view(teacher), dy) + calls(pred, teacher, torch._neg_view(dy)):
+        with pytest.raises(ValueError, match="negat"):
+            call()

@@ -261,3 +261,31 @@ def test_refusals_on_the_gpu():
     lib = _lib.load()  # a workspace that is too small
     assert lib.rafb200_embedding_dx(dy.data_ptr(), 0, ids.data_ptr(), _lib.I64, 3, 5, 8, 1.0, -1, 0, x.data_ptr(), 0, dy.data_ptr(),
                                     16, None) == 1
+
+
+def test_forward_mode_and_lazy_signs_are_refused():
+    """Tensors whose tangent, or whose sign, is not at their address."""
+    import torch.autograd.forward_ad as fwd
+
+    x, ids = torch.randn(5, 8, device="cuda"), torch.randint(0, 5, (3,), device="cuda")
+    dy, into = torch.randn(3, 8, device="cuda"), torch.zeros(5, 8, device="cuda")
+
+    def calls(x, dy, into):
+        return ([lambda: op.embedding(x, ids), lambda: op.embedding(x, ids, out=torch.empty(3, 8, device="cuda")),
+                 lambda: op.embedding(x, ids, stream=torch.cuda.current_stream())],
+                [lambda: op.embedding_dx(dy, ids, 5), lambda: op.embedding_dx(dy, ids, 5, stream=torch.cuda.current_stream())],
+                [lambda: op.embedding_dx(torch.ones(3, 8, device="cuda"), ids, 5, out=into, accumulate=True)])
+
+    with fwd.dual_level():
+        for call in sum(calls(*(fwd.make_dual(t, torch.ones_like(t)) for t in (x, dy, into))), []):
+            with pytest.raises(ValueError, match="forward"):
+                call()
+        with torch.no_grad(), pytest.raises(ValueError, match="forward"):
+            op.embedding(fwd.make_dual(x, torch.ones_like(x)), ids)
+        with pytest.raises(ValueError, match="forward"):
+            op.embedding(fwd.make_dual(x.clone().requires_grad_(), torch.ones_like(x)), ids)
+        assert torch.equal(op.embedding(x, ids), x[ids])
+    assert bool((into == 0).all())
+    for call in sum(calls(*map(torch._neg_view, (x, dy, into))), []):
+        with pytest.raises(ValueError, match="negat"):
+            call()
