@@ -512,7 +512,7 @@ PyObject* embedding(PyObject*, PyObject* const* a, Py_ssize_t n) {
 PyObject* embedding_dx(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (n != 8 || !PyLong_Check(a[2])) return nothing();
   c10::DeviceIndex dev = -1;
-  const at::Tensor *dy = data_only(a[0], dev), *ids = plain(a[1], dev), *given = a[6] == Py_None ? nullptr : primal(a[6], dev);
+  const at::Tensor *dy = data_only(a[0], dev), *ids = plain(a[1], dev), *given = a[6] == Py_None ? nullptr : data_only(a[6], dev);
   if (!dy || !ids || (a[6] != Py_None && !given)) return nothing();
   at::ScalarType type;
   if (!type_of(a[5], given ? given->scalar_type() : dy->scalar_type(), &type)) return nothing();

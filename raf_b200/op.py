@@ -350,6 +350,11 @@ def _check_values(what, *tensors):
             raise ValueError(f"{what}: there are no forward-mode derivatives, and a tensor has a tangent")
 
 
+def _check_no_graph(what, name, t):
+    if torch.is_grad_enabled() and t is not None and t.requires_grad:
+        raise ValueError(f"{what}: the result is part of no autograd graph, and {name} requires a gradient; detach it")
+
+
 def _span(t):
     """The bytes a tensor of positive strides reaches over."""
     if t.numel() == 0:
@@ -418,6 +423,7 @@ def embedding(x, indices, scale=1.0, padding_idx=None, dtype=None, out=None, str
     _check_cuda(x, indices)
     _same_device(x, indices)
     _check_values("embedding", x, out)
+    _check_no_graph("embedding", "out", out)
     if x.dim() != 2:
         raise ValueError("embedding: x is a table, [rows, width]")
     dtype = x.dtype if dtype is None else torch_dtype(dtype)
@@ -452,7 +458,8 @@ def embedding_dx(dy, indices, num_weight, scale=1.0, padding_idx=None, dtype=Non
     added to it (a further micro-batch, a matrix product that shares the table), rounded once to its type, and rows
     without a token stay as they are.  Indices equal to ``padding_idx`` or outside [0, num_weight) count nothing (a negative
     ``padding_idx`` names no row).
-    The same call gives the same bits: sums run in an order that the indices fix.
+    The same call gives the same bits: sums run in an order that the indices fix.  The result is data, part of no autograd graph:
+    ``dy`` and ``out`` must not require a gradient.
     """
     if stream is None:
         r = _lib.ops().embedding_dx(dy, indices, num_weight, scale, padding_idx, dtype, out, accumulate)
@@ -463,6 +470,8 @@ def embedding_dx(dy, indices, num_weight, scale=1.0, padding_idx=None, dtype=Non
     _check_cuda(dy, indices)
     _same_device(dy, indices)
     _check_values("embedding_dx", dy, out)
+    _check_no_graph("embedding_dx", "dy", dy)
+    _check_no_graph("embedding_dx", "out", out)
     if dy.dim() != indices.dim() + 1 or dy.shape[:-1] != indices.shape:
         raise ValueError("embedding_dx: dy has the shape of indices and one dimension more")
     num_weight, width = int(num_weight), dy.shape[-1]
@@ -555,6 +564,8 @@ def _gradient_for(pred, out, others):
     rows, ld = _rows_of(out, "out")
     _same_device(pred, out)
     _check_values("distill_loss", out)
+    if out is not pred:
+        _check_no_graph("distill_loss", "out", out)
     if out.shape != pred.shape or out.dtype != pred.dtype:
         raise ValueError(f"out is to be {tuple(pred.shape)} of {pred.dtype}")
     _check_apart(out, *(t for t in others if t is not None))
@@ -615,7 +626,8 @@ def distill_loss_dpred(dy, pred, teacher_logits, teacher_ids, stats, labels=None
     """Gradient of :func:`distill_loss`: ``dy * grad_scale * d loss / d pred``, of pred's shape and type.
 
     ``dy`` is fp32, one weight per row, one for all rows (0-dimensional), or None for 1; ``grad_scale`` is the loss scale that
-    the optimizers' own ``grad_scale`` takes back.  ``out`` takes the result and may be ``pred`` itself.
+    the optimizers' own ``grad_scale`` takes back.  ``out`` takes the result and may be ``pred`` itself; another one must not
+    require a gradient.  The result is data, part of no autograd graph.
     """
     if out is None and stream is None:
         r = _lib.ops().distill(dy, pred, teacher_logits, teacher_ids, stats, labels, temperature, alpha, ignore_index, grad_scale, 1)

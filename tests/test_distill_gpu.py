@@ -514,3 +514,20 @@ def test_forward_mode_and_lazy_signs_are_refused():
     for call in calls(torch._neg_view(pred), teacher, dy) + calls(pred, torch._neg_view(teacher), dy) + calls(pred, teacher, torch._neg_view(dy)):
         with pytest.raises(ValueError, match="negat"):
             call()
+
+
+def test_a_gradient_is_not_written_into_a_graph():
+    """out takes data: it requires no gradient itself, unless it is pred, whose graph ends there."""
+    pred, teacher, ids, lab, dy = make(6, 40, 3, F32, labels=True)
+    stats = op.distill_loss(pred, teacher, ids)[1]
+    out = torch.zeros_like(pred).requires_grad_()
+    for call in (lambda: op.distill_loss_dpred(dy, pred, teacher, ids, stats, out=out), lambda: op.distill_loss_with_dpred(dy, pred, teacher, ids, out=out * 2)):
+        with pytest.raises(ValueError, match="gradient"):
+            call()
+    want = op.distill_loss_dpred(dy, pred, teacher, ids, stats)
+    with torch.no_grad():
+        assert torch.equal(op.distill_loss_dpred(dy, pred, teacher, ids, stats, out=out), want)
+    w = pred.clone().requires_grad_()
+    logits = w * 1.0
+    op.distill_loss_dpred(dy, logits, teacher, ids, stats, out=logits)
+    assert torch.equal(logits, want)

@@ -289,3 +289,16 @@ def test_forward_mode_and_lazy_signs_are_refused():
     for call in sum(calls(*map(torch._neg_view, (x, dy, into))), []):
         with pytest.raises(ValueError, match="negat"):
             call()
+
+
+def test_a_gradient_is_not_cut_off_without_a_word():
+    """embedding_dx has no backward, and what is written into out has none either."""
+    ids, dy, dx = torch.randint(0, 5, (3,), device="cuda"), torch.randn(3, 8, device="cuda"), torch.zeros(5, 8, device="cuda")
+    leaf, out = dy.clone().requires_grad_(), dx.clone().requires_grad_()
+    for call in (lambda: op.embedding_dx(leaf, ids, 5), lambda: op.embedding_dx(leaf * 2, ids, 5, out=dx), lambda: op.embedding_dx(dy, ids, 5, out=out),
+                 lambda: op.embedding_dx(dy, ids, 5, out=out * 2, accumulate=True), lambda: op.embedding(dx, ids, out=leaf),
+                 lambda: op.embedding_dx(leaf, ids, 5, stream=torch.cuda.current_stream())):
+        with pytest.raises(ValueError, match="gradient"):
+            call()
+    with torch.no_grad():
+        assert torch.equal(op.embedding_dx(leaf, ids, 5, out=out), op.embedding_dx(dy, ids, 5))
