@@ -14,6 +14,9 @@ gradient is a difference of such terms, each off by r of itself, and is rounded 
 a value below log2(v) + A, which also bounds what is subtracted) is off by 4 u (A + log2 v) + r.
 """
 import math
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -531,3 +534,31 @@ def test_a_gradient_is_not_written_into_a_graph():
     logits = w * 1.0
     op.distill_loss_dpred(dy, logits, teacher, ids, stats, out=logits)
     assert torch.equal(logits, want)
+
+
+ALONE = """
+import sys
+sys.path.insert(0, {tests!r})
+from test_distill_gpu import *
+
+"""
+
+
+def alone(body):
+    """Runs `body` in a process of its own, where no call has gone before."""
+    script = ALONE.format(tests=os.path.dirname(os.path.abspath(__file__))) + body + "\nprint('went through')\n"
+    r = subprocess.run([sys.executable, "-c", script], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "went through" in r.stdout, r.stdout + r.stderr
+
+
+def test_lists_whose_entries_just_fill_the_shared_memory_that_is_given_unasked():
+    """48 KB for what a block asks for and what its kernel declares together: from 32 KB for the logits and 754 entries on that is
+    more, before the entries alone are."""
+    alone("""
+for k in (752, 753, 754, 760, 767, 768):
+    pred, teacher, ids, lab, dy = make(3, 40000, k, BF16)
+    loss, stats = op.distill_loss(pred, teacher, ids)
+    both = op.distill_loss_with_dpred(dy, pred, teacher, ids)
+    check((pred, teacher, ids, None), loss, op.distill_loss_dpred(dy, pred, teacher, ids, stats), dy)
+    check((pred, teacher, ids, None), both[0], both[1], dy)
+""")
