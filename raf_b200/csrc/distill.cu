@@ -794,12 +794,12 @@ static int64_t row_groups(const rafb200_distill* d) { return d->v * dtype_size(d
 
 template <typename T, Second S, bool GRAD, int NT>
 static int launch_rows(const rafb200_distill* d, DistillArgs a, cudaStream_t s) {
-  const size_t smem = (size_t)kDistillRing * NT * 16 + Entries::bytes(d->k);
+  const size_t ring = (size_t)kDistillRing * NT * 16, smem = ring + Entries::bytes(d->k);
   // few rows are cut until every SM has work, while a thread keeps a group
   while (a.slices_log < 3 && (d->n << (a.slices_log + 1)) <= 148 * 2 && row_groups(d) >> (a.slices_log + 1) >= NT) ++a.slices_log;
   // what the resident blocks hold of the logits, to be read again, is to stay in the L2
   while (GRAD && a.slices_log < 3 && row_groups(d) >> a.slices_log > kMostGroups) ++a.slices_log;
-  if (const int rc = allow_smem<distill_kernel<T, S, GRAD, NT>>(smem)) return rc;
+  if (const int rc = allow_smem<distill_kernel<T, S, GRAD, NT>>(smem, ring + Entries::bytes(kMaxTeacher))) return rc;
   RAFB200_CUDA(launch_cluster(distill_kernel<T, S, GRAD, NT>, 1u << a.slices_log, (unsigned)(d->n << a.slices_log), NT + 32, smem, s, a));
   return RAFB200_OK;
 }
@@ -810,7 +810,7 @@ static bool short_rows(const rafb200_distill* d) { return row_groups(d) <= 32 * 
 template <typename T, Second S, Part P>
 static int launch_short(const rafb200_distill* d, const DistillArgs& a, cudaStream_t s) {
   const size_t smem = kShortWarps * Entries::bytes(d->k);
-  if (const int rc = allow_smem<distill_short_kernel<T, S, P>>(smem)) return rc;
+  if (const int rc = allow_smem<distill_short_kernel<T, S, P>>(smem, kShortWarps * Entries::bytes(kMaxTeacher))) return rc;
   RAFB200_CUDA(launch_dependent(distill_short_kernel<T, S, P>, dim3((unsigned)((d->n + kShortWarps - 1) / kShortWarps)), 32 * kShortWarps, smem, s, a));
   return RAFB200_OK;
 }
@@ -877,8 +877,8 @@ int rafb200_distill_loss_dpred(const rafb200_distill* d, const float* dy, int dy
     using T = decltype(t);
     constexpr Second S = decltype(second)::value;
     if (short_rows(d)) return launch_short<T, S, kDpred>(d, a, static_cast<cudaStream_t>(stream));
-    const size_t smem = Stream<T, kDpredThreads>::kPlaces * 16 + Entries::bytes(d->k);
-    if (const int rc = allow_smem<distill_dpred_kernel<T, S>>(smem)) return rc;
+    const size_t ring = Stream<T, kDpredThreads>::kPlaces * 16, smem = ring + Entries::bytes(d->k);
+    if (const int rc = allow_smem<distill_dpred_kernel<T, S>>(smem, ring + Entries::bytes(kMaxTeacher))) return rc;
     RAFB200_CUDA(launch_dependent(distill_dpred_kernel<T, S>, dim3((unsigned)(d->n << a.slices_log)), kDpredThreads + 32, smem,
                                   static_cast<cudaStream_t>(stream), a));
     return (int)RAFB200_OK;

@@ -754,7 +754,7 @@ int rafb200_embedding_dx(const void* dy, int dy_dtype, const void* indices, int 
   } else {
     const int64_t each = (int64_t)kSortBlocks * kSortThreads * 64;  // four stores a thread
     const unsigned clusters = 1 + (unsigned)std::min<int64_t>((so.fill_bytes + each - 1) / each, kFillClusters);
-    if (const int rc = allow_smem<embedding_sort_kernel>(kSortSmem)) return rc;
+    if (const int rc = allow_smem<embedding_sort_kernel>(kSortSmem, kSortSmem)) return rc;
     if (const int rc = allow_large_cluster<embedding_sort_kernel>()) return rc;
     RAFB200_CUDA(launch_cluster(embedding_sort_kernel, kSortBlocks, clusters * kSortBlocks, kSortThreads, kSortSmem, s, so));
   }
@@ -782,7 +782,7 @@ int rafb200_embedding_dx(const void* dy, int dy_dtype, const void* indices, int 
         constexpr bool kAny = sizeof(T) == 2 && decltype(w)::value == 1;
         constexpr int kVec = kAny ? 2 : decltype(w)::value;
         constexpr size_t smem = sizeof(SumShared<typename Group<T, kVec>::W, kVec, kAny>);
-        if (const int rc = allow_smem<embedding_sum_kernel<T, O, kVec, kAny>>(smem)) return rc;
+        if (const int rc = allow_smem<embedding_sum_kernel<T, O, kVec, kAny>>(smem, smem)) return rc;
         RAFB200_CUDA(launch_dependent(embedding_sum_kernel<T, O, kVec, kAny>, dim3((unsigned)grid), kSumThreads, smem, s, a));
         return (int)RAFB200_OK;
       });

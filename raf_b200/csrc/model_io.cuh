@@ -253,16 +253,17 @@ inline cudaError_t launch_cluster(void (*kernel)(Params...), unsigned cluster, u
   return cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);
 }
 
-// Lets the kernel take `bytes` of dynamic shared memory on the current device, asked of the driver when they grow.  48 KB are given
-// unasked, for these and for the kernel's own variables, which are below 1 KB.
+// Lets the kernel take `bytes` of dynamic shared memory on the current device; `most` is what any launch of it takes, and that is
+// asked of the driver, once: of two threads neither can lower the limit that the other needs.  48 KB are given unasked, for these
+// and for the kernel's own variables, which are below 1 KB.
 template <auto kKernel>
-inline int allow_smem(size_t bytes) {
-  static std::atomic<size_t> granted[64];
+inline int allow_smem(size_t bytes, size_t most) {
+  static std::atomic<bool> granted[64];
   int device = 0;
   RAFB200_CUDA(cudaGetDevice(&device));
-  if (bytes <= 47 * 1024 || (device < 64 && granted[device].load(std::memory_order_relaxed) >= bytes)) return RAFB200_OK;
-  RAFB200_CUDA(cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
-  if (device < 64) granted[device].store(bytes, std::memory_order_relaxed);
+  if (bytes <= 47 * 1024 || (device < 64 && granted[device].load(std::memory_order_acquire))) return RAFB200_OK;
+  RAFB200_CUDA(cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most));
+  if (device < 64) granted[device].store(true, std::memory_order_release);
   return RAFB200_OK;
 }
 

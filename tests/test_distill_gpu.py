@@ -562,3 +562,36 @@ for k in (752, 753, 754, 760, 767, 768):
     check((pred, teacher, ids, None), loss, op.distill_loss_dpred(dy, pred, teacher, ids, stats), dy)
     check((pred, teacher, ids, None), both[0], both[1], dy)
 """)
+
+
+def test_first_calls_of_several_threads():
+    """Lists of two lengths above 48 KB, the first of their kernel, at the same time; and the longer one again."""
+    alone("""
+import threading
+
+failed = []
+for dtype in (F32, F16, BF16):
+    pred, teacher, ids, lab, dy = make(3, 300, 1000, dtype, labels=True)
+    stats = torch.ones(3, 4, device="cuda")
+    lists = [(teacher[:, :600].contiguous(), ids[:, :600].contiguous()), (teacher, ids)]
+    for how in (dict(), dict(labels=lab, alpha=0.5, temperature=2.0), dict(labels=lab, alpha=0.5, temperature=4.0), dict(labels=lab, alpha=0.5, temperature=3.0)):
+        for call in (lambda t, i: op.distill_loss(pred, t, i, **how), lambda t, i: op.distill_loss_with_dpred(dy, pred, t, i, **how),
+                     lambda t, i: op.distill_loss_dpred(dy, pred, t, i, stats, **how)):
+            start = threading.Barrier(4)
+
+            def first(*args):
+                start.wait()
+                try:
+                    call(*args)
+                except Exception as e:
+                    failed.append(repr(e))
+
+            threads = [threading.Thread(target=first, args=args) for args in lists * 2]
+            for t in threads:
+                t.start()
+            for t in threads:
+                t.join()
+            call(*lists[1])
+torch.cuda.synchronize()
+assert not failed, failed
+""")
