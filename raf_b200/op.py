@@ -387,7 +387,13 @@ def _launching(t, stream, *others):
 
 def _check_capturable(name, x):
     """Before a node is put behind x: what backward could not be captured through is refused here, where an exception is one."""
-    if torch.cuda.is_current_stream_capturing() and _lib.ops().reaches_default_stream(x):
+    if not torch.cuda.is_current_stream_capturing():
+        return
+    reaches = _lib.ops().reaches_default_stream(x)
+    if reaches is None:  # the stream of a node is not to be had from Python
+        raise RuntimeError(f"{name}: under capture, whether a backward could be captured is known to the native module alone, and "
+                           "raf_b200._ops is not available; detach the input, or build the module")
+    if reaches:
         raise RuntimeError(f"{name}: under capture, but the input's autograd graph reaches into one that was built on the default "
                            "stream and still lives, so its backward cannot be captured; drop that graph first, or detach the input")
 
@@ -412,7 +418,8 @@ def embedding(x, indices, scale=1.0, padding_idx=None, dtype=None, out=None, str
     ``x`` is [rows, width] in fp32 / fp16 / bf16, ``indices`` any shape of int32 / int64; the result is of ``dtype``
     (default: x's), rounded once.  An index outside [0, rows) reads as a row of zeros.  Where ``x`` requires a
     gradient, backward is :func:`embedding_dx`, for which ``padding_idx`` names an index that counts nothing.  Forward and
-    backward may be captured in one graph while no eager graph of the same leaves lives; else the captured call is refused.
+    backward may be captured in one graph while no eager graph of the same leaves lives; else, and where raf_b200._ops, which
+    looks for one, is missing, the captured call is refused.
     """
     if out is None and stream is None:
         r = _lib.ops().embedding(x, indices, scale, dtype)

@@ -98,3 +98,32 @@ print("as captured")
 def test_a_captured_backward():
     r = subprocess.run([sys.executable, "-c", BACKWARD], capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and "as captured" in r.stdout, r.stdout + r.stderr
+
+
+WITHOUT = """
+import torch
+from raf_b200 import _lib, op
+
+_lib._ops = _lib._GeneralWay()
+table = torch.randn(500, 500, device="cuda", requires_grad=True)
+ids = torch.randint(0, 500, (60,), device="cuda")
+teacher, classes = torch.randn(60, 8, device="cuda"), torch.randint(0, 500, (60, 8), device="cuda")
+logits = torch.randn(60, 500, device="cuda", requires_grad=True)
+for call in (lambda: op.embedding(table, ids), lambda: op.distill_loss(logits, teacher, classes)):
+    call()
+    try:
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            call()
+    except RuntimeError as e:
+        assert "native module" in str(e), e
+    else:
+        raise SystemExit("was not refused")
+    with torch.cuda.graph(torch.cuda.CUDAGraph()), torch.no_grad():
+        call()
+print("refused")
+"""
+
+
+def test_a_captured_call_without_the_native_module():
+    r = subprocess.run([sys.executable, "-c", WITHOUT], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "refused" in r.stdout, r.stdout + r.stderr

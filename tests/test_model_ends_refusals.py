@@ -68,3 +68,12 @@ def test_distill_arguments():
     assert calls(out=AT - 4, stats=None) == (1, 1, 1)  # and ends inside it
     assert calls(out=AT, ld_out=11, stats=None) == (1, 1, 1)  # at pred's address, with other rows
     assert lib.rafb200_distill_loss(None, AT, AT, None) == 1
+
+
+def test_without_the_native_module_no_captured_graph(monkeypatch):
+    """Whether a captured backward would end the process the native module alone can say."""
+    x = torch.zeros(3, requires_grad=True)
+    monkeypatch.setattr(_lib, "_ops", _lib._GeneralWay())
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(RuntimeError, match="native module"):
+        op._check_capturable("embedding", x)
