@@ -302,3 +302,16 @@ def test_a_gradient_is_not_cut_off_without_a_word():
             call()
     with torch.no_grad():
         assert torch.equal(op.embedding_dx(leaf, ids, 5, out=out), op.embedding_dx(dy, ids, 5))
+
+
+@pytest.mark.parametrize("rows", [255, 256, 511, 512, 513, 262143, 262144, 262145, (1 << 27) - 1])
+@pytest.mark.parametrize("n", [4096, 4097, 9999])
+def test_every_digit_of_an_id_is_sorted(n, rows):
+    """Tables at the borders of the sort's digits, with as many tokens as are ranked by comparison and with more."""
+    g = torch.Generator(device="cuda").manual_seed(n + rows)
+    ids = torch.randint(0, rows, (n,), generator=g, device="cuda")
+    ids[::3] = torch.tensor([rows - 1, 0, rows // 2, rows - 1, rows, -1, 1, rows - 2], device="cuda").repeat(n)[:ids[::3].numel()]
+    dy = torch.randn(n, 1 if rows > 1 << 20 else 3, generator=g, device="cuda")
+    got = op.embedding_dx(dy, ids, rows)
+    check_gradient(got, dy, ids, rows, 1.0)
+    assert torch.equal(got, op.embedding_dx(dy, ids, rows))
