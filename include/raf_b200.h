@@ -363,8 +363,9 @@ RAFB200_API int rafb200_embedding_dx(const void* dy, int dy_dtype, const void* i
  *                   outside [0, v) has loss 0 and gradient 0, whatever its logits hold.
  * Logits of -infinity are classes of probability 0; a row of nothing else, +infinity and NaN give NaN.  A row without either term
  * has loss 0 and gradient 0, but for a gradient of NaN where a logit is +infinity or NaN.
- * Everything is computed in fp32, exponentials to 2 ulp; the teacher's term is a difference of logarithms times T^2,
- * whose absolute error grows so.
+ * Everything is computed in fp32.  The exponential of a logit d T below the maximum is off by at most (3 d + 4) 2^-24 of itself, at one
+ * beside T = 2 or 4, where it is multiplied out, by (3 d + 9) or (3 d + 19) 2^-24; below 2^-126 it may be 0.  The teacher's term is a
+ * difference of logarithms times T^2, whose absolute error grows so.
  * A term whose weight (alpha, 1 - alpha) is 0 counts nothing. */
 typedef struct {
   const void* pred;

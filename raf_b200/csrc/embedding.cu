@@ -147,8 +147,11 @@ __device__ void zero_bytes(unsigned char* p, int64_t bytes, int64_t worker, int6
 }
 
 // Few tokens: each warp finds the rank of its tokens by comparing them with all, which need no more than one block's shared
-// memory.  No block waits for another.  1024 tokens take 3.4 us where the cluster's passes take 11.7 us, 2048 4.7 and 12.2 us,
-// 4096 10.9 and 12.4 us: the border.
+// memory.  No block waits for another.  The launch alone, without zeros to write: 1024 tokens take 3.4 us where the cluster's passes
+// take 11.7 us, 2048 4.7 and 12.2 us, 4096 10.9 and 12.4 us.  Whole calls with a result to zero (30522 rows of 1024, bf16), ranked and
+// sorted: 1000 tokens 20.1 and 22.3 us, 2048 21.7 and 23.2 us, 3000 24.6 and 23.6 us, 4096 28.5 and 24.6 us one behind the other;
+// with cold caches, from 512 tokens on, 18.5 and 22.5, 20.5 and 26.6 (1000), 22.5 and 26.6 (2048), 26.6 and 26.6 (3000), 28.7 and 28.7 us: the
+// border.
 constexpr int kRankTokens = 4096;
 constexpr int kRankThreads = 256;
 constexpr int kRankLoads = 8;
@@ -430,8 +433,10 @@ struct SumShared {
 
 // Bound: HBM, the gathered rows of dy.  Rows come through shared memory by asynchronous copies, kSumRing of them on their
 // way for a lane, which alone reads what it has asked for; what accumulated rows hold already is asked for together for those
-// that end in a batch.  The sums of cut rows, in a launch of their own, took 2 to 5 us more.  65536 tokens of 1024 (bf16):
-// 32 us into two rows (4.2 TB/s), 54 us added to 20000 rows of fp32 (5.5 TB/s of dy and of the rows read and written).
+// that end in a batch.  The sums of cut rows, in a launch of their own, took 2 to 5 us more.  65536 tokens of 1024 (bf16), from
+// the end of the sort on: into two rows 34 us with cold caches (3.9 TB/s), 28 us among calls that leave a part of dy in the L2 (4.8 TB/s);
+// 54 us added to 20000 rows of fp32 (5.5 TB/s of dy and of the rows read and written).  Rows of 1023, two columns a lane: 127 us for
+// the whole call, where rows of 1024 take 59 us into 30522 rows of bf16.
 // ANY: 16-bit rows that begin at any element (VEC 2).  A lane's two elements are its word of the row's aligned ones, or, where
 // the row begins in the middle of one, that word's second half and the next word's first.
 template <typename T, typename O, int VEC, bool ANY>
