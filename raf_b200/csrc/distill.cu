@@ -842,9 +842,9 @@ int rafb200_distill_loss(const rafb200_distill* d, float* loss, float* stats, vo
   a.stats = reinterpret_cast<float4*>(stats);
   return with_case(d, [&](auto t, auto second) {
     if (short_rows(d)) return launch_short<decltype(t), decltype(second)::value, kLoss>(d, a, static_cast<cudaStream_t>(stream));
-    // Blocks of 128 threads and of 256, 4096 rows, loss alone: of 312 groups 18 and 29 us, of 2048 41 and 43, of 3000 and 3815 (16-bit) 53 and 49,
-    // 59 and 59 us, of 4096 (fp32) 66 and 57, of 5000 78 and 70, of 10000 129 and 117 us.  For 300 rows the same within 2 us up to 3815, then
-    // 14 and 12 us, 25 and 21 us.
+    // Blocks of 128 threads and of 256, 4096 rows, the loss alone: of 312 groups 18 and 29 us, of 2048 41 and 43, of 3000 and 3815 (16-bit)
+    // 53 and 49, 59 and 59, of 4096 (fp32) 66 and 57, of 5000 78 and 70, of 10000 129 and 117 us.  300 rows take the same within 2 us
+    // up to 3815 groups, then 14 and 12 us (5000), 21 and 16 us (10000).
     if (row_groups(d) >= 4096) return launch_rows<decltype(t), decltype(second)::value, false, 256>(d, a, static_cast<cudaStream_t>(stream));
     return launch_rows<decltype(t), decltype(second)::value, false, 128>(d, a, static_cast<cudaStream_t>(stream));
   });
@@ -903,8 +903,8 @@ int rafb200_distill_loss_with_dpred(const rafb200_distill* d, const float* dy, i
   a.ld_out = ld_dpred;
   return with_case(d, [&](auto t, auto second) {
     if (short_rows(d)) return launch_short<decltype(t), decltype(second)::value, kBoth>(d, a, static_cast<cudaStream_t>(stream));
-    // Blocks of 128 threads and of 256, 4096 rows: of 1125 groups 45 and 57 us, of 2048 (16-bit) 64 and 70, of 2250 (fp32) 72 and 70, of 3000 90 and 88,
-    // of 3815 119 and 107, of 6282 207 and 168 us.  Fewer rows at a time leave the second look at them to the L2.
+    // Blocks of 128 threads and of 256, 4096 rows: of 1125 groups 45 and 57 us, of 2048 (16-bit) 64 and 70, of 2250 (fp32) 72 and 70, of
+    // 3000 90 and 88, of 3815 119 and 107, of 6282 207 and 168 us.  Fewer rows at a time leave the second look at them to the L2.
     if (row_groups(d) >= 2048) return launch_rows<decltype(t), decltype(second)::value, true, 256>(d, a, static_cast<cudaStream_t>(stream));
     return launch_rows<decltype(t), decltype(second)::value, true, 128>(d, a, static_cast<cudaStream_t>(stream));
   });

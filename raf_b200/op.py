@@ -605,8 +605,8 @@ def distill_loss(pred, teacher_logits, teacher_ids, labels=None, temperature=1.0
 
     ``stats`` is what :func:`distill_loss_dpred` takes: a row's maximum, sum of ``exp((pred - max) / T)``, sum of
     ``exp(pred - max)``, and a value that it does not read.  What this loss does not sum up is NaN, and so is a gradient that
-    takes it: the last sum where T is not 1 and there is no hard term, all of them in a row that its label leaves out.  Where ``pred`` requires a gradient, backward calls it; for a captured backward
-    the condition of :func:`embedding` holds.
+    takes it: the last sum where T is not 1 and there is no hard term, all of them in a row that its label leaves out.  Where
+    ``pred`` requires a gradient, backward calls it; for a captured backward the condition of :func:`embedding` holds.
     """
     if stream is None:
         r = _lib.ops().distill(None, pred, teacher_logits, teacher_ids, None, labels, temperature, alpha, ignore_index, 1.0, 0)
